@@ -102,6 +102,7 @@ struct Launch {
 struct Out {
   bool is_static = false;
   Ref value;                                         // static
+  Py_ssize_t argument = -1;                          // the argument that the launches updated in place: the result is its tensor
   std::vector<int64_t> sizes, strides;
   at::TensorOptions options;
   std::vector<std::pair<Py_ssize_t, Ref>> slots;     // what a result's impl holds besides its buffer
@@ -251,7 +252,7 @@ PyObject* make(PyObject*, PyObject* a) {
     }
     t->scratch = static_cast<size_t>(integer(item(a, 6)));
     o = item(a, 7);
-    for (Py_ssize_t i = 0; i < size(o); ++i) {       // (value,) or (torch tensor, example impl)
+    for (Py_ssize_t i = 0; i < size(o); ++i) {       // (value,), (torch tensor, example impl) or (torch tensor, example impl, argument)
       PyObject* l = item(o, i);
       Out r;
       if (size(l) == 1) {
@@ -262,6 +263,10 @@ PyObject* make(PyObject*, PyObject* a) {
         r.sizes = x.sizes().vec();
         r.strides = x.strides().vec();
         r.options = x.options();
+        if (size(l) == 3) {
+          r.argument = static_cast<Py_ssize_t>(integer(item(l, 2)));
+          if (r.argument < 0 || r.argument >= static_cast<Py_ssize_t>(t->leaves.size())) { PyErr_SetString(PyExc_IndexError, "an argument"); throw Fail(); }
+        }
         PyObject* like = item(l, 1);
         Ref names(PyObject_GetAttrString(reinterpret_cast<PyObject*>(g_impl), "__slots__"));
         if (names.p == nullptr) throw Fail();
@@ -512,6 +517,7 @@ PyObject* call(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     for (size_t i = 0; i < t->outs.size(); ++i) {
       const Out& o = t->outs[i];
       if (o.is_static) { results.emplace_back(); continue; }
+      if (o.argument >= 0) { results.push_back(held[t->pins.size() + static_cast<size_t>(o.argument)]); continue; }
       results.push_back(at::empty_strided(o.sizes, o.strides, o.options));
       bases[leaves.size() + i] = static_cast<char*>(results.back().data_ptr());
     }

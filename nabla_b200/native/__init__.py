@@ -22,7 +22,8 @@ _status: dict[int, torch.Tensor] = {}
 _debug_rec: dict[int, torch.Tensor] = {}
 # translation units of each library (each has its own nb_debug_bind_<tu> / nb_debug_enabled_<tu>)
 _DEBUG_UNITS = {"libnb_gemm.so": ("gemm",), "libnb_kernels.so": ("fused", "elementwise"),
-                "libnb_attention.so": ("attention",), "libnb_comm.so": ("comm",)}
+                "libnb_attention.so": ("attention",), "libnb_serving.so": ("kv_cache", "cached_attention", "logits"),
+                "libnb_comm.so": ("comm",)}
 
 
 class NativeLibraryMissing(RuntimeError):
@@ -234,12 +235,12 @@ from .gemm import gemm_bf16, gemm_supported  # noqa: E402,F401
 
 def total_launches() -> int:
     """Number of launches of this package's own kernels issued so far by this process
-    (GEMM, attention, fused kernels, peer-memory collectives and fused GEMM+collective)."""
+    (GEMM, attention, fused and serving kernels, peer-memory collectives and fused GEMM+collective)."""
     import sys
 
     n = 0
     for name in ("nabla_b200.native.gemm", "nabla_b200.native.kernels", "nabla_b200.native.attention",
-                 "nabla_b200.parallel.symm"):
+                 "nabla_b200.native.serving", "nabla_b200.parallel.symm"):
         m = sys.modules.get(name)
         if m is not None:
             n += getattr(m, "launch_count", 0)

@@ -869,7 +869,7 @@ class CompiledFunction:
             if rec.tape is None and rec.cuda_graph is not None and tds is not None and rec.copy_out is not None:
                 rec.tape = tape.graph_call(rec, tensors, tds) or False
                 rec.tape_of_graph = bool(rec.tape)
-                rec.tape_counts = (0, rec.copy_in.launches + rec.copy_out.launches, 0) if rec.tape else ()
+                rec.tape_counts = (0, rec.copy_in.launches + rec.copy_out.launches, 0, 0) if rec.tape else ()
             self._taped = (rec.tape, rec, True) if rec.tape and tds is not None else None
             return out
         # (a call that was to be captured and whose launches are written down instead comes here too)
@@ -995,9 +995,9 @@ def _tell_stream(rec: "_Recorded") -> None:
 
 @_functools.lru_cache(None)                         # (a taped call asks)
 def _counted_modules() -> tuple:
-    from ..native import attention, gemm, kernels
+    from ..native import attention, gemm, kernels, serving
 
-    return gemm, kernels, attention
+    return gemm, kernels, attention, serving
 
 
 _LEAF_KINDS = {"bias_grads", "sum_axes", "next_step", "scale_gemm", "gemm_scale"}

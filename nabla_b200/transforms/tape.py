@@ -24,7 +24,8 @@ from ..core.tensor.impl import TensorImpl
 LAUNCHES = frozenset("""nb_gemm_bf16 nb_gemm_dual_bf16 nb_attn_fwd nb_attn_bwd nb_layernorm_fwd nb_layernorm_bwd nb_colsum nb_colsum_group nb_softmax
     nb_lse_pick_fwd nb_lse_pick_bwd nb_adamw nb_adamw_group nb_adam_hyper nb_mean_diff nb_sgd nb_embedding_gather nb_embedding_scatter_add
     nb_cast nb_activation nb_nf4_dequant nb_nf4_dequant_codes nb_pool2d_fwd nb_pool2d_bwd nb_pool2d_select nb_conv2d_direct nb_conv_flip
-    nb_conv2d_wgrad_direct nb_sgemm nb_sum_slices nb_binary nb_unary nb_reduce nb_cumsum""".split())
+    nb_conv2d_wgrad_direct nb_sgemm nb_sum_slices nb_binary nb_unary nb_reduce nb_cumsum nb_kv_write nb_kv_read nb_cached_attention
+    nb_adjust_logits""".split())
 # functions of sizes alone
 QUERIES = frozenset("""nb_layernorm_bwd_nblocks nb_colsum_nparts nb_conv2d_wgrad_slices nb_sgemm_slices nb_reduce_splits
     nb_embedding_scatter_work""".split())
@@ -232,7 +233,7 @@ def _tape(rec, tensors, tds, r: _Recorder, result_buffers):
     if any(a[1] > b[0] for a, b in zip(order, order[1:])) or any(lo < s[1] and s[0] < hi for s in order for lo, hi in constants):
         raise _Refused("arguments that share memory")       # of this call; the next may be told apart
     allocated = r.allocated
-    # results: whole allocations of this run, one each
+    # results: whole allocations of this run, one each, or arguments that it updated in place
     outs, result_of = [], {}
     n_in = len(tensors)
     for k, (impl, static, bufs) in enumerate(zip(rec.out_impls, rec.out_static, result_buffers)):
@@ -243,6 +244,10 @@ def _tape(rec, tensors, tds, r: _Recorder, result_buffers):
         if b is None:
             raise _Refused("a result in pieces")
         lo, hi = _span(b)
+        passed = next((i for i, t in enumerate(bases) if t is b), None)
+        if passed is not None:
+            outs.append((b, TensorImpl.result_like(impl, [b]), passed))
+            continue
         own = [i for i, s in enumerate(allocated) if s == (lo, hi) and lo != hi]
         if not own or b.storage_offset() or b.data_ptr() != lo or own[-1] in result_of or _extent(b) != (lo, lo + _dense_bytes(b)) \
                 or not _is_whole(b, hi - lo):
