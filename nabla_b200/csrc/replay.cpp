@@ -112,6 +112,8 @@ struct Tape {
   std::vector<Tree> args;
   std::vector<Leaf> leaves;
   std::vector<std::pair<std::string, Ref>> env;      // (name, bytes or None)
+  struct Apart { int a, b; ptrdiff_t bytes; };
+  std::vector<Apart> apart;                          // arguments in each other's memory (views of one tensor): how far they start from each other
   std::vector<Pin> pins;
   std::vector<at::Tensor> kept;                      // what the launches' fixed addresses lie in: alive as long as a call is at it
   int device = 0;
@@ -181,7 +183,7 @@ Tree read_tree(PyObject* o) {                        // (kind, keys or None, chi
 
 void release(PyObject* cap) { delete static_cast<Tape*>(PyCapsule_GetPointer(cap, "nb_tape")); }
 
-// make(args, leaves, env, device, deterministic, launches, scratch, outs, out_tree, graph, captured impls, kept tensors): see transforms/tape.py
+// make(args, leaves, env, device, deterministic, launches, scratch, outs, out_tree, graph, captured impls, kept tensors, apart): see transforms/tape.py
 PyObject* make(PyObject*, PyObject* a) {
   auto t = std::make_unique<Tape>();
   try {
@@ -308,6 +310,11 @@ PyObject* make(PyObject*, PyObject* a) {
     }
     o = item(a, 11);
     for (Py_ssize_t i = 0; i < size(o); ++i) t->kept.push_back(tensor(item(o, i)));
+    o = item(a, 12);
+    for (Py_ssize_t i = 0; i < size(o); ++i) {       // (argument, argument, bytes from the first one's start to the second one's)
+      PyObject* l = item(o, i);
+      t->apart.push_back({static_cast<int>(integer(item(l, 0))), static_cast<int>(integer(item(l, 1))), static_cast<ptrdiff_t>(integer(item(l, 2)))});
+    }
   } catch (const Fail&) {
     return nullptr;
   } catch (const std::exception& e) {
@@ -486,6 +493,8 @@ PyObject* call(PyObject*, PyObject* const* argv, Py_ssize_t argc) {
     held.push_back(*x);
     bases[i] = static_cast<char*>(x->data_ptr());
   }
+  for (const Tape::Apart& p : t->apart)              // which of the two a pointer was reckoned from does not matter as long as this holds
+    if (bases[static_cast<size_t>(p.b)] - bases[static_cast<size_t>(p.a)] != p.bytes) Py_RETURN_NOTIMPLEMENTED;
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(t->device)).stream();
   int code = 0;
   if (t->replay.p != nullptr) {

@@ -229,9 +229,13 @@ def _tape(rec, tensors, tds, r: _Recorder, result_buffers):
     if any(len(a._buffers) != 1 for a in _captured(rec)):
         raise _Refused("a captured tensor in pieces")
     constants = [_span(t) for t in _constants(rec)]
-    order = sorted(s for s in spans if s[0] != s[1])
-    if any(a[1] > b[0] for a, b in zip(order, order[1:])) or any(lo < s[1] and s[0] < hi for s in order for lo, hi in constants):
+    full = [i for i, s in enumerate(spans) if s[0] != s[1]]
+    meet = [(i, j) for k, i in enumerate(full) for j in full[k + 1:] if spans[i][0] < spans[j][1] and spans[j][0] < spans[i][1]]
+    if any(spans[i][0] == spans[j][0] for i, j in meet) or any(lo < spans[i][1] and spans[i][0] < hi for i in full for lo, hi in constants):
         raise _Refused("arguments that share memory")       # of this call; the next may be told apart
+    # views of one tensor (keys and values of a packed projection): a pointer may have been reckoned from either, so the tape is for calls
+    # whose views start as far from each other as these
+    apart = [(i, j, bases[j].data_ptr() - bases[i].data_ptr()) for i, j in meet]
     allocated = r.allocated
     # results: whole allocations of this run, one each, or arguments that it updated in place
     outs, result_of = [], {}
@@ -330,7 +334,7 @@ def _tape(rec, tensors, tds, r: _Recorder, result_buffers):
                 out.append(e)
         launches.append((address, rc, name, out))
     return module().make((tuple(tree_of(td) for td in tds), _leaves(tensors), _environment(), device, config.is_deterministic(), launches,
-                          scratch, outs, tree_of(rec.out_treedef), None, [a for a in _captured(rec) if a.literal is None], rec.owned or []))
+                          scratch, outs, tree_of(rec.out_treedef), None, [a for a in _captured(rec) if a.literal is None], rec.owned or [], apart))
 
 
 def _extent(t: torch.Tensor) -> tuple[int, int]:
@@ -381,6 +385,6 @@ def graph_call(rec, tensors: list, tds: tuple):
         graph = (rec.cuda_graph.replay, address, [(t.data_ptr(), n) for t, n in zip(ins.fixed, ins.size)],
                  [(t.data_ptr(), n) for t, n in zip(outs_.fixed, outs_.size)])
         return module().make((tuple(tree_of(td) for td in tds), _leaves(tensors), _environment(), device, config.is_deterministic(), [], 0, outs,
-                              tree_of(rec.out_treedef), graph, [], [*ins.fixed, *outs_.fixed, *(rec.owned or [])]))
+                              tree_of(rec.out_treedef), graph, [], [*ins.fixed, *outs_.fixed, *(rec.owned or [])], []))
     except _Refused:
         return None

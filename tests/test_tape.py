@@ -441,3 +441,45 @@ def test_many_small_blocks_in_a_row(rows, dim):
         assert all(torch.equal(x, y) for x, y in zip(outs, want[k % 3])), k
     x = want[0][0].double()
     assert torch.allclose(want[0][1].double(), torch.nn.functional.cross_entropy(x, sets[0][1]), rtol=1e-5)
+
+
+def test_views_of_one_tensor_as_arguments():
+    """Keys and values of a packed projection lie in each other's memory: written down for views that start as far apart, others go another way."""
+    import nabla_b200 as nb
+
+    from nabla_b200.nn import functional as F
+
+    f = nb.compile(lambda k, v, q: F.scaled_dot_product_attention(q, k, v))
+    packed, other = (torch.randn(1, 2, 40, 3, 64, device="cuda").to(BF16) for _ in range(2))
+    q = _wrap(torch.randn(1, 2, 40, 64, device="cuda").to(BF16))
+
+    def check(k, v):
+        assert torch.equal(f(_wrap(k), _wrap(v), q).to_torch(), F.scaled_dot_product_attention(q, _wrap(k), _wrap(v)).to_torch())
+
+    views = lambda t, i, j: (t[:, :, :, i], t[:, :, :, j])  # noqa: E731
+    for _ in range(3):
+        check(*views(packed, 0, 1))
+    assert _taped(f), f.tape_refused
+    check(*views(other, 0, 1))
+    assert _taped(f)
+    for k, v in (views(packed, 0, 2), views(packed, 1, 0), (packed[:, :, :, 0], other[:, :, :, 1]), views(other, 2, 2), views(packed, 0, 1)):
+        check(k, v)
+
+
+def test_results_that_are_arguments_updated_in_place():
+    import nabla_b200 as nb
+    from nabla_b200.nn import functional as F
+
+    f = nb.compile(lambda cache, k, table, past: F.kv_cache_write(cache, k, k, table, past))
+    table, past = (_wrap(torch.zeros(s, dtype=torch.int32, device="cuda")) for s in ((1, 1), (1,)))
+    caches = [F.init_kv_cache(1, 2, 64, 16, device=table.device) for _ in range(2)]
+    for cache in caches * 3:
+        k = torch.randn(1, 3, 2, 64, device="cuda")
+        before = {n: t.to_torch() for n, t in cache.items()}
+        got = f(cache, _wrap(k), table, past)
+        for n in cache:
+            assert got[n].to_torch() is before[n] and got[n].to_torch().data_ptr() == before[n].data_ptr()
+        want = F.kv_cache_write({n: _wrap(torch.zeros_like(t)) for n, t in before.items()}, _wrap(k), _wrap(k), table, past)
+        first = lambda t: t.to_torch().reshape(1, 2, -1)[..., : 3 * 64]  # noqa: E731
+        assert all(torch.equal(first(got[n]), first(want[n])) for n in got)
+    assert _taped(f), f.tape_refused
