@@ -37,7 +37,7 @@ struct Table {
   }
 };
 
-// Tokens that a sequence has, from 0 to what its row of the table has room for (below 2^31).
+// Tokens that a sequence has, from 0 to what its row of the table has room for (below 2^30).
 __device__ __forceinline__ int clamp_tokens(long long n, long long most) { return static_cast<int>(n < 0 ? 0 : n > most ? most : n); }
 
 template <typename T>

@@ -6,6 +6,7 @@ Arguments are torch CUDA tensors whose shapes and types ``ops/serving.py`` has c
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -23,7 +24,8 @@ def _L():
         sig = {
             "nb_kv_write": [c_vp] * 9 + [c_int] * 8 + [c_ll] * 6 + [c_int, c_vp],
             "nb_kv_read": [c_vp] * 9 + [c_int] * 9 + [c_vp],
-            "nb_cached_attention": [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_int, c_vp],
+            "nb_cached_attention": [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_int, c_vp, c_int, c_vp],
+            "nb_cached_attention_splits": [c_int] * 8,
             "nb_adjust_logits": [c_vp] * 9 + [c_ll, c_vp] + [c_int] * 6 + [c_vp],
         }
         for name, args in sig.items():
@@ -51,7 +53,7 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     """(batch, tokens, heads, head_dim) whose rows can be read 16 bytes at a time where they are, else a copy."""
     v = 16 // t.element_size()
     ok = t.stride(3) == 1 and not t.data_ptr() & 15 and all(t.stride(i) % v == 0 for i in range(3) if t.shape[i] > 1)
-    return t if ok else t.contiguous()
+    return t if ok else t.clone(memory_format=torch.contiguous_format)       # (contiguous() keeps a dense one that starts off a boundary)
 
 
 def _dense(*ts: torch.Tensor) -> None:
@@ -89,10 +91,20 @@ def cached_attention(q, k_codes, k_scale, v_codes, v_scale, table, past, count, 
     b, t, hq, d = q.shape
     blocks, h, n, _ = k_codes.shape
     out = torch.empty((b, t, hq, d), dtype=q.dtype, device=q.device)
+    fp32 = int(q.dtype == torch.float32)
+    splits = _splits(b, t, hq, h, d, n, table.shape[1], fp32)
+    # fp32 results of the ranges: outputs and the logarithms of their weights; a cluster of up to 8 blocks needs none
+    part = torch.empty(splits * b * t * hq * (d + 1), dtype=torch.float32, device=q.device) if splits > 8 else None
     _ok(_L().nb_cached_attention(ptr(q), ptr(k_codes), ptr(k_scale), ptr(v_codes), ptr(v_scale), ptr(out), ptr(table), ptr(past), ptr(count),
                                  _wide(table, past, count), b, t, hq, h, d, n, blocks, table.shape[1], *q.stride()[:3], float(scale), int(causal),
-                                 int(q.dtype == torch.float32), stream_ptr()), "cached_attention")
+                                 splits, ptr(part), fp32, stream_ptr()), "cached_attention", 2 if splits > 8 else 1)
     return out
+
+
+@functools.lru_cache(1024)
+def _splits(*sizes: int) -> int:
+    """A function of the sizes alone."""
+    return _L().nb_cached_attention_splits(*sizes)
 
 
 def adjust_logits(logits, history, length, prompt, repetition, presence, frequency, bias, allowed):

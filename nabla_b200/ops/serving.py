@@ -265,7 +265,7 @@ def _cache(cache) -> tuple[tuple[Tensor, ...], tuple[int, ...]]:
 def _places(table, first, count, batch, first_name: str, n: int):
     _tensor(table, "block_table", _WHOLE, (batch, None))
     _need(_shape(table)[1] >= 1, "block_table has no columns")
-    _need(_shape(table)[1] * n < 1 << 31, "a sequence has fewer than 2^31 positions")
+    _need(_shape(table)[1] * n < 1 << 30, "a sequence has fewer than 2^30 positions")
     _tensor(first, first_name, _WHOLE, (batch,))
     if count is not None:
         _tensor(count, "count", _WHOLE, (batch,))

@@ -300,6 +300,11 @@ def test_writing_into_the_cache(case, device):
     for name in ("k", "v"):
         assert got[name].to_torch() is cache[name] and got[name + "_scale"].to_torch() is cache[name + "_scale"]
         check_written(cache, before, want, name)
+    # keys and values that start off a boundary
+    odd = [torch.zeros(x.numel() + 1, device=device, dtype=dtype)[1:].view(x.shape).copy_(x) for x in (k, v)]
+    third = {name: x.clone() for name, x in before.items()}
+    F.kv_cache_write(wrap(third), T(odd[0]), T(odd[1]), T(table), T(past_t), count_t)
+    assert all(torch.equal(third[name], cache[name]) for name in cache)
     # a copy is left alone, and comes out the same
     copy = {name: x.clone() for name, x in before.items()}
     again = F.kv_cache_write(wrap(copy), T(k), T(v), T(table), T(past_t), count_t, inplace=False)
