@@ -22,8 +22,9 @@ struct AttendArgs {
   void* out;                     // [batch][new][heads][D], dense
   int batch, fresh, heads, kv_heads, block_log, causal;
   float scale_log2;              // softmax scale * log2(e)
-  int splits;                    // ranges of keys
-  float *part_o, *part_w;        // of ranges that no cluster joins: [splits][batch][kv_heads][new * group] output, and log2 of the sum of its weights
+  int splits, cluster;           // ranges of keys, one block each; blocks of a cluster, which join theirs
+  float *part_o, *part_w;        // where there are several clusters: [splits / cluster][batch][kv_heads][new * group] output over their ranges, and
+                                 // log2 of the sum of its weights
 };
 
 // Four neighbouring numbers of row r (token r / group, head r % group) of cache head h.
@@ -37,6 +38,13 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, int b, int h, int
     __nv_bfloat162 u = __floats2bfloat162_rn(x.x, x.y), w = __floats2bfloat162_rn(x.z, x.w);
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&u), *reinterpret_cast<uint32_t*>(&w));
   }
+}
+
+template <int D>
+__device__ __forceinline__ void store_part(const AttendArgs& a, int part, int b, int h, int r, int c, float4 x, float weight) {
+  const long long at = (((long long)part * a.batch + b) * a.kv_heads + h) * a.fresh * (a.heads / a.kv_heads) + r;
+  reinterpret_cast<float4*>(a.part_o)[at * (D / 4) + c] = x;
+  if (c == 0) a.part_w[at] = weight;
 }
 
 // ---------------------------------------------------------------- matrix instructions on codes
@@ -71,139 +79,142 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void copy16_async(uint32_t smem, const void* p) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(p) : "memory");
+// The transpose of an 8 x 8 tile of 16-bit numbers, lane (g, t) with numbers 2t and 2t + 1 of row g.
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
 }
-__device__ __forceinline__ void copy4_async(uint32_t smem, const void* p) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem), "l"(p) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
+// Codes are read once by a block, past L1. (The address comes from the table, so these cannot move ahead of the wait for the grid ahead.)
+__device__ __forceinline__ uint4 ldg16(const void* p) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  asm("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-__device__ __forceinline__ uint2 lds8(uint32_t a) {
+__device__ __forceinline__ uint2 ldg8(const void* p) {
   uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 
 // ---------------------------------------------------------------- few rows
-// Up to 16 rows (tokens times heads of a group) of one sequence and cache head, over one of `splits` ranges of its keys. Each of the four warps
-// takes every fourth step of 32 keys: it fetches codes and scales some steps ahead into a ring of its own, so warps never wait for one
-// another, and keeps its own maximum, sum and output until the end. Bound by memory: every code is read once from HBM, and per 16 codes
-// some 20 arithmetic and 2 matrix instructions are issued, whatever the number of rows.
-constexpr int FEW_ROWS = 16, FEW_WARPS = 4, STEP = 32;
+// Up to 8 * RT rows (tokens times heads of a group) of one sequence and cache head, over one of `splits` ranges of its keys. The codes are the
+// large operand of the products: S^T = K Q^T (16 keys by 8 rows) and O^T = V^T P^T (16 dims by 8 rows), so no part of a product is padding when
+// there are 8 rows, and what is made of a code serves all rows. Fragments are read from global memory as the instruction wants them, whole
+// sectors at a time; a product's reduction may run in any order, so a lane's 16 bytes of a key are the four dims each of four k-steps, and
+// its 16 bytes of four values are rows of eight output tiles. Each of the four warps takes every fourth step of 32 keys and keeps its own
+// reference, sum and output until the end; keys of the next step are on their way from when this step's are used up, so are values.
+constexpr int FEW_WARPS = 4, STEP = 32;
+// Four-float piece c of a row of outputs in shared memory: pieces are turned so that the 8 lanes that an access serves at once meet different banks
+// (lane (g, t) writes pieces g * D / 32 ... of rows 2t and 2t + 1).
 template <int D>
+__device__ __forceinline__ int out_at(int r, int c) { return r * (D / 4) + (c ^ (D == 128 ? r >> 1 & 3 : (r >> 1 & 1) | (r & 4))); }
+template <int D, int RT>
 struct Few {
-  static constexpr int STAGES = D == 128 ? 3 : 5;
-  static constexpr int STAGE = 2 * STEP * D;                     // bytes: keys, then values
-  static constexpr int RING = STAGES * (STAGE + 16);             // and the scales of two halves: keys', values'
-  static constexpr int JOIN = FEW_WARPS * FEW_ROWS * (D + 2) * 4 + FEW_ROWS * (D + 1) * 4;
-  static constexpr int SMEM = RING * FEW_WARPS > JOIN ? RING * FEW_WARPS : JOIN;
+  static constexpr int ROWS = 8 * RT;
+  static constexpr int SMEM = (FEW_WARPS * ROWS * (D + 2) + ROWS * (D + 1)) * 4;
 };
-// Byte of 16-byte piece c of row r in a tile of codes. Rows of 128: keys are read 8 rows x 4 pieces at a time, values rows 2t at piece g; rows of 64
-// lie in pairs. The pieces of a 128-byte line are turned so that the 8 (16) lanes that a shared-memory access serves at once meet different banks.
-template <int D>
-__device__ __forceinline__ int key_at(int r, int c) { return D == 128 ? r * 128 + ((c ^ ((r & 1) << 2)) << 4) : r * 64 + (c << 4); }
-template <int D>
-__device__ __forceinline__ int value_at(int r, int c) {
-  return D == 128 ? r * 128 + ((c ^ (((r >> 1) & 3) << 1)) << 4) : (r >> 1) * 128 + (((((r & 1) << 2) | c) ^ (((r >> 1) & 3) << 1)) << 4);
-}
-// Four-float piece c of a row of outputs in shared memory, turned likewise.
-template <int D>
-__device__ __forceinline__ int out_at(int r, int c) {
-  return D == 128 ? r * 32 + (c ^ (r & 7) ^ ((c >> 3) << 1)) : r * 16 + (c ^ (r & 1) ^ (((c >> 3) & 1) << 1));
-}
 
-template <typename T, int D, bool CLUSTER>
-__global__ void __launch_bounds__(32 * FEW_WARPS, 2) attend_few_kernel(const AttendArgs a) {
-  using L = Few<D>;
+template <typename T, int D, int RT, bool CLUSTER>
+__global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_kernel(const AttendArgs a) {
   constexpr bool EXACT = sizeof(T) == 4;              // fp32: two parts, codes less their offset before the product
-  constexpr int PARTS = EXACT ? 2 : 1, KSTEPS = D / 16, PIECES = D / 64, NT = D / 8;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int PARTS = EXACT ? 2 : 1, KSTEPS = D / 16, PIECES = D / 64, MT = D / 16, ROWS = 8 * RT;
+  extern __shared__ __align__(16) uint8_t smem[];
   follow_grid();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int group = a.heads / a.kv_heads, tiles = (a.fresh * group + FEW_ROWS - 1) / FEW_ROWS;
+  const int group = a.heads / a.kv_heads, tiles = (a.fresh * group + ROWS - 1) / ROWS;
   const int sp = blockIdx.x % a.splits, h = blockIdx.x / a.splits % a.kv_heads, tile = blockIdx.x / a.splits / a.kv_heads % tiles,
             b = blockIdx.x / a.splits / a.kv_heads / tiles;
   const int room = a.table.columns << a.block_log, past = clamp_tokens(a.past.at(b), room);
   const int count = clamp_tokens(a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
-  const int row0 = tile * FEW_ROWS, rows = min(FEW_ROWS, a.fresh * group - row0);       // row r: token r / group, head r % group
-  const int live = min(rows, count * group - row0);                                     // rows from here on are zero
-  const int first = row0 / group, last = (row0 + live - 1) / group;
+  const int row0 = tile * ROWS, rows = min(ROWS, a.fresh * group - row0);       // row r: token r / group, head r % group
+  const int live = min(rows, count * group - row0);                             // rows from here on are zero
   // keys that the last row sees
-  const int keys = live <= 0 ? 0 : static_cast<int>(min((long long)room, (long long)past + (a.causal ? last + 1 : count)));
+  const int keys = live <= 0 ? 0 : static_cast<int>(min((long long)room, (long long)past + (a.causal ? (row0 + live - 1) / group + 1 : count)));
   const int per = (keys + a.splits * STEP - 1) / (a.splits * STEP) * STEP;
   const int k0 = min(keys, sp * per), k1 = min(keys, k0 + per);
   const int steps = (k1 - k0 + STEP - 1) / STEP, mine = (steps - warp + FEW_WARPS - 1) / FEW_WARPS;
-  // rows g and g + 8 of this lane: the last key that each sees
-  int lim[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) lim[i] = a.causal ? min(keys - 1, past + (row0 + g + 8 * i) / group) : keys - 1;
-  const int all_see = a.causal ? min(keys - 1, past + first) : keys - 1;     // keys up to here are seen by every row
-
-  // ---- the ring: step n of this warp holds keys k0 + (n * 4 + warp) * 32 ...
-  const uint32_t ring = static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + warp * L::RING;
-  uint32_t there = 0;                                 // two bits per stage: is there a block behind each half
-  int ids[2] = {-1, -1};
+  const int all_see = a.causal ? min(keys - 1, past + row0 / group) : keys - 1;     // keys up to here are seen by every row
   const int n = 1 << a.block_log;
-  auto find = [&](int step) {                         // blocks of a step, one step before its codes are asked for
-    const int at = k0 + (step * FEW_WARPS + warp) * STEP;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) ids[i] = step < mine && at + 16 * i < k1 ? a.table.block(b, (at + 16 * i) >> a.block_log) : -1;
-  };
-  auto fetch = [&](int step, int stage) {
-    const uint32_t to = ring + stage * (L::STAGE + 16);
-    const int at = k0 + (step * FEW_WARPS + warp) * STEP;
-    there = (there & ~(3u << (2 * stage))) | ((ids[0] >= 0 ? 1u : 0u) | (ids[1] >= 0 ? 2u : 0u)) << (2 * stage);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (ids[i] < 0) continue;
-      const long long unit = (long long)ids[i] * a.kv_heads + h;
-      const long long from = ((unit << a.block_log) + ((at + 16 * i) & (n - 1))) * D;
-#pragma unroll
-      for (int u = 0; u < 16 * D / 512; ++u) {
-        const int piece = u * 32 + lane, r = piece / (D / 16), c = piece % (D / 16);
-        copy16_async(to + key_at<D>(16 * i + r, c), a.codes[0] + from + piece * 16);
-        copy16_async(to + STEP * D + value_at<D>(16 * i + r, c), a.codes[1] + from + piece * 16);
-      }
-      if (lane < 2) copy4_async(to + L::STAGE + (lane * 2 + i) * 4, (lane ? a.scales[1] : a.scales[0]) + unit);
-    }
-  };
-  find(0);
-#pragma unroll
-  for (int s = 0; s < L::STAGES - 1; ++s) {
-    fetch(s, s);
-    copies_commit();
-    find(s + 1);
-  }
 
-  // ---- queries: lane (g, t) holds dims 16 (t + 4 p) + 4 s + {0, 1} and {2, 3} of rows g and g + 8 for k-step 4 p + s
-  uint32_t qa[PARTS][KSTEPS][4];
-  float mul[2], offset[2] = {0.f, 0.f};
+  // ---- where a step's codes lie
+  struct Place { int id[2]; };
+  auto find = [&](int step) {
+    Place p = {{-1, -1}};
+    const int at = k0 + (step * FEW_WARPS + warp) * STEP;
+    if (step < mine) {
+      p.id[0] = a.table.block(b, at >> a.block_log);
+      if (at + 16 < k1) p.id[1] = n == 16 ? a.table.block(b, (at + 16) >> a.block_log) : p.id[0];
+    }
+    return p;
+  };
+  auto unit = [&](const Place& p, int i) { return (long long)p.id[i] * a.kv_heads + h; };
+  auto from = [&](const Place& p, int i, int step) {
+    return ((unit(p, i) << a.block_log) + ((k0 + (step * FEW_WARPS + warp) * STEP + 16 * i) & (n - 1))) * D;
+  };
+  uint4 kr[2][2][PIECES], vr[2][4];                   // [16 keys each][keys g and g + 8], [keys 2t, 2t + 1, 2t + 8, 2t + 9]
+  float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int r = row0 + g + 8 * i;
-    float x[KSTEPS][4];
+#pragma unroll
+    for (int p = 0; p < 2 * PIECES; ++p) kr[i][p / PIECES][p % PIECES] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) vr[i][r] = make_uint4(0, 0, 0, 0);
+  }
+  auto get_keys = [&](const Place& p, int step) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (p.id[i] >= 0) {
+        const int8_t* at = a.codes[0] + from(p, i, step) + g * D + t * 16;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int c = 0; c < PIECES; ++c) kr[i][u][c] = ldg16(at + u * 8 * D + c * 64);
+        ks[i] = a.scales[0][unit(p, i)];
+      }
+  };
+  auto get_values = [&](const Place& p, int step) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (p.id[i] >= 0) {
+        const int8_t* at = a.codes[1] + from(p, i, step) + 2 * t * D + g * (D / 8);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int8_t* row = at + ((r & 1) + 8 * (r >> 1)) * D;
+          if (D == 128) {
+            vr[i][r] = ldg16(row);
+          } else {
+            const uint2 x = ldg8(row);
+            vr[i][r].x = x.x, vr[i][r].y = x.y;
+          }
+        }
+      }
+  };
+  Place now = find(0);
+  get_keys(now, 0);
+  get_values(now, 0);
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (now.id[i] >= 0) vs[i] = a.scales[1][unit(now, i)];
+  Place next = find(1);
+
+  // ---- queries as the small operand: lane (g, t) holds dims 16 (t + 4 p) + 4 s + {0, 1} and {2, 3} of row g for k-step 4 p + s
+  uint32_t qb[RT][PARTS][KSTEPS][2];
+  float mul[RT][2], offset[RT][2];                    // of rows 2t and 2t + 1
+  int lim[RT][2];                                     // the last key that they see
+#pragma unroll
+  for (int u = 0; u < RT; ++u) {
+    const int r = row0 + 8 * u + g;
+    float x[KSTEPS][4], top = 0.f;
     const T* q = static_cast<const T*>(a.q) + b * a.q_sb + (long long)(r / group) * a.q_st + (long long)(h * group + r % group) * a.q_sh;
-    float top = 0.f;
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      float y[8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (g + 8 * i < live) {
-          load8(q + 16 * (t + 4 * p) + 8 * u, y);
-        } else {
+      for (int w = 0; w < 2; ++w) {
+        float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        if (8 * u + g < live) load8(q + 16 * (t + 4 * p) + 8 * w, y);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = 0.f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[4 * p + 2 * u + e / 4][e % 4] = y[e], top = fmaxf(top, fabsf(y[e]));
+        for (int e = 0; e < 8; ++e) x[4 * p + 2 * w + e / 4][e % 4] = y[e], top = fmaxf(top, fabsf(y[e]));
       }
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
@@ -212,209 +223,200 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) attend_few_kernel(const Att
     int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
     ex = ex == 128 || top == 0.f ? 8 : max(ex, -110);
     const float up = __uint_as_float(static_cast<uint32_t>(127 + (8 - ex)) << 23);
-    mul[i] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - (8 - ex)) << 23);
+    const float back = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - (8 - ex)) << 23);
     float sum = 0.f;
 #pragma unroll
-    for (int k = 0; k < KSTEPS; ++k) {
+    for (int k = 0; k < KSTEPS; ++k)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float u = x[k][2 * e] * up, w = x[k][2 * e + 1] * up;
-        const uint32_t hi = pack_half2(u, w);
-        qa[0][k][2 * e + i] = hi;
-        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-        if (EXACT) qa[PARTS - 1][k][2 * e + i] = pack_half2(u - back.x, w - back.y);
-        sum += back.x + back.y;
+        const float y = x[k][2 * e] * up, z = x[k][2 * e + 1] * up;
+        const uint32_t hi = pack_half2(y, z);
+        qb[u][0][k][e] = hi;
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        if (EXACT) qb[u][PARTS - 1][k][e] = pack_half2(y - f.x, z - f.y);
+        sum += f.x + f.y;
       }
-    }
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    if (!EXACT) offset[i] = 1152.f * sum;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {                     // row 2t + e is that of lanes (2t + e, .)
+      mul[u][e] = __shfl_sync(0xffffffffu, back, 8 * t + 4 * e);
+      offset[u][e] = EXACT ? 0.f : 1152.f * __shfl_sync(0xffffffffu, sum, 8 * t + 4 * e);
+      lim[u][e] = a.causal ? min(keys - 1, past + (row0 + 8 * u + 2 * t + e) / group) : keys - 1;
+    }
   }
 
-  float o[NT][4];
+  float o[RT][MT][4];                                 // [16 dims each][dim 2j, row 2t; row 2t + 1; dim 2j + 1 likewise] of lane g's dims
+  float m[RT][2], l[RT][2];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  int stage = 0;
+  for (int u = 0; u < RT; ++u) {
+    m[u][0] = m[u][1] = -INFINITY, l[u][0] = l[u][1] = 0.f;
+#pragma unroll
+    for (int j = 0; j < MT; ++j) o[u][j][0] = o[u][j][1] = o[u][j][2] = o[u][j][3] = 0.f;
+  }
 #pragma unroll 1
   for (int step = 0; step < mine; ++step) {
-    copies_wait<L::STAGES - 2>();
-    __syncwarp();                                     // all lanes' copies of this step, and all lanes are through with the step before
-    {
-      const int ahead = step + L::STAGES - 1, into = stage == 0 ? L::STAGES - 1 : stage - 1;
-      fetch(ahead, into);
-      copies_commit();
-      find(ahead + 1);
-    }
-    const uint32_t at = ring + stage * (L::STAGE + 16);
-    const uint32_t blocks = there >> (2 * stage) & 3;
-    stage = stage == L::STAGES - 1 ? 0 : stage + 1;
-    if (blocks == 0) continue;
-    const int key0 = k0 + (step * FEW_WARPS + warp) * STEP;
-    float s[4][4];                                    // [8 keys each][row g: keys 2t, 2t + 1; row g + 8: the same]
+    float s[RT][2][4];                                // [16 keys each][key g: rows 2t, 2t + 1; key g + 8: the same]
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int u = 0; u < RT; ++u) s[u][i][0] = s[u][i][1] = s[u][i][2] = s[u][i][3] = 0.f;
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
-        const uint4 w4 = lds16(at + key_at<D>(8 * j + g, t + 4 * p));
-        const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        const uint32_t w[2][4] = {{kr[i][0][p].x, kr[i][0][p].y, kr[i][0][p].z, kr[i][0][p].w}, {kr[i][1][p].x, kr[i][1][p].y, kr[i][1][p].z, kr[i][1][p].w}};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint32_t c = w[k] ^ 0x80808080u;
-          uint32_t b0 = widen(c, 0x4140), b1 = widen(c, 0x4342);
-          if (EXACT) b0 = half2_minus(b0, BIAS2), b1 = half2_minus(b1, BIAS2);
+          const uint32_t x = w[0][k] ^ 0x80808080u, y = w[1][k] ^ 0x80808080u;
+          uint32_t c[4] = {widen(x, 0x4140), widen(y, 0x4140), widen(x, 0x4342), widen(y, 0x4342)};
+          if (EXACT)
 #pragma unroll
-          for (int u = 0; u < PARTS; ++u) mma16816(s[j], qa[u][4 * p + k], b0, b1);
+            for (int e = 0; e < 4; ++e) c[e] = half2_minus(c[e], BIAS2);
+#pragma unroll
+          for (int u = 0; u < RT; ++u)
+#pragma unroll
+            for (int f = 0; f < PARTS; ++f) mma16816(s[u][i], c, qb[u][f][4 * p + k][0], qb[u][f][4 * p + k][1]);
         }
       }
     }
-    const uint4 sc = lds16(at + L::STAGE);
+    const float sk[2] = {ks[0], ks[1]};
+    get_keys(next, step + 1);
+
+    const int key0 = k0 + (step * FEW_WARPS + warp) * STEP;
     float per_value[2], lg[2];                        // 1 / s_v, log2 s_v
+    bool grow = false, small = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bool is = blocks >> i & 1;
-      const float sk = __uint_as_float(i ? sc.y : sc.x);
-      float sv = __uint_as_float(i ? sc.w : sc.z);
-      if (sv < LEAST_SCALE) sv = LEAST_SCALE;
+      const bool is = now.id[i] >= 0;
+      const float sv = vs[i] < LEAST_SCALE ? LEAST_SCALE : vs[i];
       lg[i] = __log2f(sv);
-      per_value[i] = is ? __fdividef(1.f, sv) : 0.f;
+      per_value[i] = __fdividef(1.f, sv);
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float f = mul[r] * sk, c = EXACT ? lg[i] : fmaf(-offset[r], f, lg[i]);
+      for (int u = 0; u < RT; ++u)
 #pragma unroll
-        for (int j = 2 * i; j < 2 * i + 2; ++j)
-#pragma unroll
-          for (int e = 2 * r; e < 2 * r + 2; ++e) s[j][e] = is ? fmaf(s[j][e], f, c) : -INFINITY;
-      }
+        for (int r = 0; r < 2; ++r) {
+          const float f = mul[u][r] * sk[i], c = EXACT ? lg[i] : fmaf(-offset[u][r], f, lg[i]);
+          s[u][i][r] = is ? fmaf(s[u][i][r], f, c) : -INFINITY;
+          s[u][i][2 + r] = is ? fmaf(s[u][i][2 + r], f, c) : -INFINITY;
+        }
     }
     if (key0 + STEP - 1 > all_see) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int u = 0; u < RT; ++u)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (key0 + 8 * j + 2 * t + (e & 1) > lim[e >> 1]) s[j][e] = -INFINITY;
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key0 + 16 * i + 8 * (e >> 1) + g > lim[u][e & 1]) s[u][i][e] = -INFINITY;
     }
     // the reference that weights are taken against follows the maximum only when that has grown by 2^8: weights stay below 2^8
-    bool grow = false;
-    float top[2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      top[r] = fmaxf(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])),
-                     fmaxf(fmaxf(s[2][2 * r], s[2][2 * r + 1]), fmaxf(s[3][2 * r], s[3][2 * r + 1])));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-      top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      grow |= top[r] > m[r] + 8.f || (m[r] == -INFINITY && top[r] > -INFINITY);
-    }
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float x = fmaxf(s[u][0][r], s[u][0][2 + r]), y = fmaxf(s[u][1][r], s[u][1][2 + r]), top = fmaxf(x, y), low = m[u][r] - 100.f;
+        grow |= top > m[u][r] + 8.f;                  // (of nothing to something too)
+        small |= (x < low && x > -INFINITY) || (y < low && y > -INFINITY);
+      }
     if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        // in two steps: the factor alone may fall out of the range of fp32
-        const float now = fmaxf(m[r], top[r]), f = m[r] == now ? 1.f : ex2(0.5f * (m[r] - now));
-        m[r] = now;
-        l[r] = l[r] * f * f;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) o[j][2 * r] = o[j][2 * r] * f * f, o[j][2 * r + 1] = o[j][2 * r + 1] * f * f;
-      }
-    }
-    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-    uint32_t pa[PARTS][2][4];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float sum[2] = {0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int u = 0; u < RT; ++u)
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-          const float u = ex2(s[2 * i + j][2 * r] - base[r]), w = ex2(s[2 * i + j][2 * r + 1] - base[r]);
-          sum[r] += u + w;
-          const uint32_t hi = pack_half2(u, w);
-          pa[0][i][2 * j + r] = hi;
+          float top = fmaxf(fmaxf(s[u][0][r], s[u][0][2 + r]), fmaxf(s[u][1][r], s[u][1][2 + r]));
+#pragma unroll
+          for (int w = 4; w < 32; w <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          // in two steps: the factor alone may fall out of the range of fp32
+          const float to = fmaxf(m[u][r], top), f = m[u][r] == to ? 1.f : ex2(0.5f * (m[u][r] - to));
+          m[u][r] = to;
+          l[u][r] = l[u][r] * f * f;
+#pragma unroll
+          for (int j = 0; j < MT; ++j) o[u][j][r] = o[u][j][r] * f * f, o[u][j][2 + r] = o[u][j][2 + r] * f * f;
+        }
+      small = true;                                   // (looked at under the reference before)
+    }
+    uint32_t pb[RT][PARTS][2][2];
+    const bool apart = __any_sync(0xffffffffu, small);
+#pragma unroll
+    for (int u = 0; u < RT; ++u) {
+      const float base[2] = {m[u][0] == -INFINITY ? 0.f : m[u][0], m[u][1] == -INFINITY ? 0.f : m[u][1]};
+      if (apart) {                                    // weights that are lost in fp32 may count once their value's scale is taken out
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (s[u][i][e] != -INFINITY) l[u][e & 1] += ex2(s[u][i][e] - base[e & 1] - lg[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[u][i][e] = ex2(s[u][i][e] - base[e & 1]);
+        if (!apart)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float sum = s[u][i][r] + s[u][i][2 + r];
+            if (sum != 0.f) l[u][r] = fmaf(sum, per_value[i], l[u][r]);     // a row that sees none of these keys does not see their scale either
+          }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {                 // keys g + 8 k of rows 2t, 2t + 1, turned to keys 2t, 2t + 1 (+ 8 k) of row g
+          const uint32_t hi = pack_half2(s[u][i][2 * k], s[u][i][2 * k + 1]);
+          pb[u][0][i][k] = turn8x8(hi);
           if (EXACT) {
-            const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-            pa[PARTS - 1][i][2 * j + r] = pack_half2(u - back.x, w - back.y);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+            pb[u][PARTS - 1][i][k] = turn8x8(pack_half2(s[u][i][2 * k] - f.x, s[u][i][2 * k + 1] - f.y));
           }
         }
-      bool small = false;                             // weights that are lost in fp32 may count once their value's scale is taken out
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float most = fmaxf(fmaxf(s[2 * i][2 * r], s[2 * i][2 * r + 1]), fmaxf(s[2 * i + 1][2 * r], s[2 * i + 1][2 * r + 1]));
-        small |= most < base[r] - 100.f && most > -INFINITY;
-      }
-      if (__any_sync(0xffffffffu, small)) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = s[2 * i + e / 2][2 * r + e % 2];
-            if (x != -INFINITY) l[r] += ex2(x - base[r] - lg[i]);
-          }
-      } else {
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-          if (sum[r] != 0.f) l[r] = fmaf(sum[r], per_value[i], l[r]);     // a row that sees none of these keys does not see their scale either
       }
     }
-    // lane (g, t): dims g * D / 8 ... of keys 2t, 2t + 1, 2t + 8, 2t + 9; the tile of 8 dims number j takes dims j, D / 8 + j, 2 D / 8 + j ...
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      if (!(blocks >> i & 1)) continue;               // what lies there was never written: not even times zero
-      uint32_t w[4][D / 32];
+      uint32_t w[4][4];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = 16 * i + 2 * t + (r & 1) + 8 * (r >> 1);
-        if (D == 128) {
-          const uint4 x = lds16(at + STEP * D + value_at<D>(row, g));
-          w[r][0] = x.x, w[r][1] = x.y, w[r][D / 32 - 2] = x.z, w[r][D / 32 - 1] = x.w;
-        } else {
-          const uint2 x = lds8(at + STEP * D + value_at<D>(row, g >> 1) + 8 * (g & 1));
-          w[r][0] = x.x, w[r][1] = x.y;
-        }
-      }
+      for (int r = 0; r < 4; ++r) w[r][0] = vr[i][r].x, w[r][1] = vr[i][r].y, w[r][2] = vr[i][r].z, w[r][3] = vr[i][r].w;
 #pragma unroll
-      for (int k = 0; k < D / 32; ++k) {
+      for (int j = 0; j < MT; ++j) {                  // dims 2 j and 2 j + 1 of this lane's
+        const uint32_t sel = j & 1 ? 0x7362 : 0x5140;
+        const uint32_t x = __byte_perm(w[0][j / 2], w[1][j / 2], sel) ^ 0x80808080u, y = __byte_perm(w[2][j / 2], w[3][j / 2], sel) ^ 0x80808080u;
+        const uint32_t c[4] = {half2_minus(widen(x, 0x4140), BIAS2), half2_minus(widen(x, 0x4342), BIAS2), half2_minus(widen(y, 0x4140), BIAS2),
+                               half2_minus(widen(y, 0x4342), BIAS2)};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {                 // dims 4 k + 2 e and + 1
-          const uint32_t sel = e ? 0x7362 : 0x5140;
-          const uint32_t x = __byte_perm(w[0][k], w[1][k], sel) ^ 0x80808080u, y = __byte_perm(w[2][k], w[3][k], sel) ^ 0x80808080u;
+        for (int u = 0; u < RT; ++u)
 #pragma unroll
-          for (int f = 0; f < 2; ++f) {
-            const uint32_t b0 = half2_minus(widen(x, f ? 0x4342 : 0x4140), BIAS2), b1 = half2_minus(widen(y, f ? 0x4342 : 0x4140), BIAS2);
-#pragma unroll
-            for (int u = 0; u < PARTS; ++u) mma16816(o[4 * k + 2 * e + f], pa[u][i], b0, b1);
-          }
-        }
+          for (int f = 0; f < PARTS; ++f) mma16816(o[u][j], c, pb[u][f][i][0], pb[u][f][i][1]);
       }
     }
+    get_values(next, step + 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (next.id[i] >= 0) vs[i] = a.scales[1][unit(next, i)];
+    now = next;
+    next = find(step + 2);
   }
 
   // ---- join the warps in a fixed order, as ranges are joined: by the sums of their weights
-  copies_wait<0>();
-  __syncthreads();
   float4* so = reinterpret_cast<float4*>(smem);                                   // [warp][row][D]
-  float* sm = reinterpret_cast<float*>(smem) + FEW_WARPS * FEW_ROWS * D;           // [warp][row] log2 of the sum of weights (over s_v)
-  float* sl = sm + FEW_WARPS * FEW_ROWS;                                           //             one over their sum
-  float* to = sl + FEW_WARPS * FEW_ROWS;                                           // CLUSTER: [row][D] of this block
-  float* tl = to + FEW_ROWS * D;                                                   //          [row] log2 of the sum of weights
+  float* sm = reinterpret_cast<float*>(smem) + FEW_WARPS * ROWS * D;               // [warp][row] log2 of the sum of weights (over s_v)
+  float* sl = sm + FEW_WARPS * ROWS;                                               //             one over their sum
+  float* to = sl + FEW_WARPS * ROWS;                                               // CLUSTER: [row][D] of this block
+  float* tl = to + ROWS * D;                                                       //          [row] log2 of the sum of weights
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const int row = g + 8 * r;
-    if (t == 0) {
-      sm[warp * FEW_ROWS + row] = l[r] == 0.f ? -INFINITY : m[r] + __log2f(l[r]);
-      sl[warp * FEW_ROWS + row] = l[r] == 0.f ? 0.f : 1.f / l[r];
-    }
-    if (row < live)
+  for (int u = 0; u < RT; ++u)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)                     // dims (2 t + e) * D / 8 ...
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int w = 4; w < 32; w <<= 1) l[u][r] += __shfl_xor_sync(0xffffffffu, l[u][r], w);
+      const int row = 8 * u + 2 * t + r;
+      if (g == 0) {
+        sm[warp * ROWS + row] = l[u][r] == 0.f ? -INFINITY : m[u][r] + __log2f(l[u][r]);
+        sl[warp * ROWS + row] = l[u][r] == 0.f ? 0.f : 1.f / l[u][r];
+      }
+      if (row < live)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
-          so[warp * FEW_ROWS * (D / 4) + out_at<D>(row, (2 * t + e) * (D / 32) + c)] =
-              make_float4(o[4 * c][2 * r + e], o[4 * c + 1][2 * r + e], o[4 * c + 2][2 * r + e], o[4 * c + 3][2 * r + e]);
-  }
+          so[warp * ROWS * (D / 4) + out_at<D>(row, g * (D / 32) + c)] =
+              make_float4(o[u][2 * c][r], o[u][2 * c][2 + r], o[u][2 * c + 1][r], o[u][2 * c + 1][2 + r]);
+    }
   __syncthreads();
-  constexpr int PER = FEW_ROWS * (D / 4) / (32 * FEW_WARPS);
+  constexpr int PER = ROWS * (D / 4) / (32 * FEW_WARPS);
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int i = u * 32 * FEW_WARPS + threadIdx.x, row = i / (D / 4), c = i % (D / 4);
@@ -423,14 +425,14 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) attend_few_kernel(const Att
     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
     if (row < live) {
 #pragma unroll
-      for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, sm[w * FEW_ROWS + row]);
+      for (int w = 0; w < FEW_WARPS; ++w) top = fmaxf(top, sm[w * ROWS + row]);
       const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
       for (int w = 0; w < FEW_WARPS; ++w) {
-        float f = ex2(sm[w * FEW_ROWS + row] - ref);
-        const float4 y = so[w * FEW_ROWS * (D / 4) + out_at<D>(row, c)];
+        float f = ex2(sm[w * ROWS + row] - ref);
+        const float4 y = so[w * ROWS * (D / 4) + out_at<D>(row, c)];
         sum += f;
-        f *= sl[w * FEW_ROWS + row];
+        f *= sl[w * ROWS + row];
         x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
       }
     }
@@ -441,9 +443,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) attend_few_kernel(const Att
       reinterpret_cast<float4*>(to)[i] = x;
       if (c == 0) tl[row] = weight;
     } else if (a.splits > 1) {
-      const long long at = (((long long)sp * a.batch + b) * a.kv_heads + h) * a.fresh * group + row0 + row;
-      reinterpret_cast<float4*>(a.part_o)[at * (D / 4) + c] = x;
-      if (c == 0) a.part_w[at] = weight;
+      store_part<D>(a, sp, b, h, row0 + row, c, x, weight);
     } else {
       store_out<T, D>(a, b, h, row0 + row, c, x);
     }
@@ -451,13 +451,13 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) attend_few_kernel(const Att
   if (CLUSTER) {
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     cluster.sync();
-    for (int i = sp * 32 * FEW_WARPS + threadIdx.x; i < rows * (D / 4); i += a.splits * 32 * FEW_WARPS) {
+    for (int i = sp % a.cluster * 32 * FEW_WARPS + threadIdx.x; i < rows * (D / 4); i += a.cluster * 32 * FEW_WARPS) {
       const int row = i / (D / 4), c = i % (D / 4);
       float top = -INFINITY, sum = 0.f;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < a.splits; ++r) top = fmaxf(top, *cluster.map_shared_rank(&tl[row], r));
+      for (int r = 0; r < a.cluster; ++r) top = fmaxf(top, *cluster.map_shared_rank(&tl[row], r));
       const float ref = top == -INFINITY ? 0.f : top;
-      for (int r = 0; r < a.splits; ++r) {
+      for (int r = 0; r < a.cluster; ++r) {
         const float f = ex2(*cluster.map_shared_rank(&tl[row], r) - ref);
         const float4 y = *cluster.map_shared_rank(&reinterpret_cast<float4*>(to)[i], r);
         sum += f;
@@ -465,52 +465,59 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, 2) attend_few_kernel(const Att
       }
       const float inverse = sum == 0.f ? 0.f : 1.f / sum;
       x.x *= inverse, x.y *= inverse, x.z *= inverse, x.w *= inverse;
-      store_out<T, D>(a, b, h, row0 + row, c, x);
+      if (a.splits > a.cluster) {
+        store_part<D>(a, sp / a.cluster, b, h, row0 + row, c, x, sum == 0.f ? -INFINITY : top + __log2f(sum));
+      } else {
+        store_out<T, D>(a, b, h, row0 + row, c, x);
+      }
     }
     cluster.sync();                                   // a block's shared memory is read until here
   }
 }
 
-// Joins the ranges of keys: one warp per row, in the order of the ranges.
+// Joins what clusters have written, in their order: one block per row, a thread for four numbers of every second (fourth) part.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_join_kernel(const AttendArgs a) {
+__global__ void __launch_bounds__(64) attend_join_kernel(const AttendArgs a) {
+  constexpr int C = D / 4, SIDES = 64 / C;
+  __shared__ float4 other[SIDES][C];
+  __shared__ float others[SIDES];
   follow_grid();
-  const int group = a.heads / a.kv_heads, lane = threadIdx.x & 31;
-  const long long rows = (long long)a.batch * a.kv_heads * a.fresh * group, at = (long long)blockIdx.x * 4 + threadIdx.x / 32;
-  if (at >= rows) return;
-  float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 32) top = fmaxf(top, a.part_w[s * rows + at]);
-#pragma unroll
-  for (int w = 16; w; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  const int group = a.heads / a.kv_heads, c = threadIdx.x % C, side = threadIdx.x / C, parts = a.splits / a.cluster;
+  const long long rows = (long long)a.batch * a.kv_heads * a.fresh * group, at = blockIdx.x;
+  float top = -INFINITY, sum = 0.f;
+  for (int s = 0; s < parts; ++s) top = fmaxf(top, a.part_w[s * rows + at]);
   const float ref = top == -INFINITY ? 0.f : top;
-  constexpr int C = D / 4, LANES = C < 32 ? 32 / C : 1;      // ranges that a warp reads at once
-  float sum = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int s = lane / C; s < a.splits; s += LANES) {
-    const float w = a.part_w[s * rows + at];
-    const float4 y = reinterpret_cast<const float4*>(a.part_o)[(s * rows + at) * C + lane % C];
-    const float f = ex2(w - ref);
+#pragma unroll 8
+  for (int s = side; s < parts; s += SIDES) {
+    const float f = ex2(a.part_w[s * rows + at] - ref);
+    const float4 y = reinterpret_cast<const float4*>(a.part_o)[(s * rows + at) * C + c];
     sum += f;
     x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
   }
-  if (LANES == 2) {
-    sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-    x.x += __shfl_xor_sync(0xffffffffu, x.x, 16), x.y += __shfl_xor_sync(0xffffffffu, x.y, 16);
-    x.z += __shfl_xor_sync(0xffffffffu, x.z, 16), x.w += __shfl_xor_sync(0xffffffffu, x.w, 16);
+  other[side][c] = x;
+  if (c == 0) others[side] = sum;
+  __syncthreads();
+  if (side > 0) return;
+#pragma unroll
+  for (int s = 1; s < SIDES; ++s) {
+    const float4 y = other[s][c];
+    sum += others[s];
+    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
   }
   const float inverse = sum == 0.f ? 0.f : 1.f / sum;
   x.x *= inverse, x.y *= inverse, x.z *= inverse, x.w *= inverse;
   const int r = static_cast<int>(at % (a.fresh * group)), h = static_cast<int>(at / (a.fresh * group) % a.kv_heads),
             b = static_cast<int>(at / (a.fresh * group) / a.kv_heads);
-  if (lane < C) store_out<T, D>(a, b, h, r, lane, x);
+  store_out<T, D>(a, b, h, r, c, x);
 }
 
-
-// Ranges of keys for each (sequence, head, 16 rows), by sizes alone. A cluster of up to 8 blocks joins its ranges in distributed shared memory; more
+// Ranges of keys for each (sequence, head, tile of rows), by sizes alone. A cluster of up to 8 blocks joins its ranges in distributed shared memory; more
 // go through memory and a second kernel.
+static int few_rows(int rows) { return rows <= 8 ? 8 : 16; }
 static int few_splits(int batch, int fresh, int heads, int kv_heads, long long room) {
-  const long long units = (long long)batch * kv_heads * ((fresh * (heads / kv_heads) + FEW_ROWS - 1) / FEW_ROWS);
+  const int rows = fresh * (heads / kv_heads), tile = few_rows(rows);
+  const long long units = (long long)batch * kv_heads * ((rows + tile - 1) / tile);
   const long long most = (room + FEW_WARPS * STEP - 1) / (FEW_WARPS * STEP);           // a step for each warp at least
   long long want = (296 + units - 1) / units;
   if (want <= 8) want = 8;
@@ -518,42 +525,46 @@ static int few_splits(int batch, int fresh, int heads, int kv_heads, long long r
   if (units * want > 4 * 296) want = 2;
   if (units * want > 4 * 296) want = 1;
   if (want > most) want = most;
-  if (want < 8) want = want >= 4 ? 4 : want >= 2 ? 2 : 1;
-  return static_cast<int>(want < 1 ? 1 : want > 128 ? 128 : want);
+  want = want >= 8 ? want / 8 * 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
+  return static_cast<int>(want > 128 ? 128 : want);
 }
 
-template <typename T, int D>
+template <typename T, int D, int RT>
 static cudaError_t launch_few(const AttendArgs& a, cudaStream_t stream) {
-  const bool cluster = a.splits > 1 && a.splits <= 8;
-  const auto kernel = cluster ? attend_few_kernel<T, D, true> : attend_few_kernel<T, D, false>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Few<D>::SMEM);
-  if (e != cudaSuccess) return e;
-  const long long grid = (long long)a.splits * a.kv_heads * a.batch * ((a.fresh * (a.heads / a.kv_heads) + FEW_ROWS - 1) / FEW_ROWS);
+  const bool cluster = a.cluster > 1;
+  const auto kernel = cluster ? attend_few_kernel<T, D, RT, true> : attend_few_kernel<T, D, RT, false>;
+  const long long grid = (long long)a.splits * a.kv_heads * a.batch * ((a.fresh * (a.heads / a.kv_heads) + 8 * RT - 1) / (8 * RT));
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  static_assert(Few<D, RT>::SMEM <= 48 * 1024, "no more than a kernel has without asking");
+  cudaError_t e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(32 * FEW_WARPS);
-  cfg.dynamicSmemBytes = Few<D>::SMEM;
+  cfg.dynamicSmemBytes = Few<D, RT>::SMEM;
   cfg.stream = stream;
   cfg.attrs = attr;
   if (cluster) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(a.splits);
+    attr[0].val.clusterDim.x = static_cast<unsigned>(a.cluster);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
   }
   nb::set_following(cfg);
   e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess || cluster || a.splits == 1) return e;
-  const long long rows = (long long)a.batch * a.fresh * a.heads;
-  return launch_following(attend_join_kernel<T, D>, dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(128), 0, stream, a);
+  if (e != cudaSuccess || a.splits == a.cluster) return e;
+  return launch_following(attend_join_kernel<T, D>, dim3(static_cast<unsigned>((long long)a.batch * a.fresh * a.heads)), dim3(64), 0, stream, a);
+}
+
+template <typename T, int D>
+static cudaError_t launch_attend(const AttendArgs& a, cudaStream_t stream) {
+  return few_rows(a.fresh * (a.heads / a.kv_heads)) == 8 ? launch_few<T, D, 1>(a, stream) : launch_few<T, D, 2>(a, stream);
 }
 
 }  // namespace nbc
 
-// Ranges of keys that nb_cached_attention is to be called with for these sizes. From 9 on it needs scratch: splits * batch * new * heads * (head_dim + 1)
-// floats.
+// Ranges of keys that nb_cached_attention is to be called with for these sizes. Above 8 it needs scratch: splits / 8 * batch * new * heads *
+// (head_dim + 1) floats.
 extern "C" int nb_cached_attention_splits(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int columns, int fp32) {
   return nbc::few_splits(batch, fresh, heads, kv_heads, (long long)columns * block);
 }
@@ -574,11 +585,13 @@ extern "C" int nb_cached_attention(const void* q, const void* k_codes, const voi
   a.batch = batch, a.fresh = fresh, a.heads = heads, a.kv_heads = kv_heads, a.causal = causal;
   a.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : -1;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.splits = splits, a.part_o = scratch, a.part_w = scratch + (long long)splits * batch * fresh * heads * head_dim;
+  a.splits = splits, a.cluster = splits < 8 ? splits : 8;
+  if (splits != 1 && splits != 2 && splits != 4 && splits % 8 != 0) return -1;
+  a.part_o = scratch, a.part_w = scratch + (long long)(splits / a.cluster) * batch * fresh * heads * head_dim;
   if (a.block_log < 0 || (head_dim != 64 && head_dim != 128)) return -1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (fp32) return head_dim == 64 ? launch_few<float, 64>(a, s) : launch_few<float, 128>(a, s);
-  return head_dim == 64 ? launch_few<__nv_bfloat16, 64>(a, s) : launch_few<__nv_bfloat16, 128>(a, s);
+  if (fp32) return head_dim == 64 ? launch_attend<float, 64>(a, s) : launch_attend<float, 128>(a, s);
+  return head_dim == 64 ? launch_attend<__nv_bfloat16, 64>(a, s) : launch_attend<__nv_bfloat16, 128>(a, s);
 }
 
 NB_DEBUG_DEFINE(cached_attention)

@@ -93,8 +93,8 @@ def cached_attention(q, k_codes, k_scale, v_codes, v_scale, table, past, count, 
     out = torch.empty((b, t, hq, d), dtype=q.dtype, device=q.device)
     fp32 = int(q.dtype == torch.float32)
     splits = _splits(b, t, hq, h, d, n, table.shape[1], fp32)
-    # fp32 results of the ranges: outputs and the logarithms of their weights; a cluster of up to 8 blocks needs none
-    part = torch.empty(splits * b * t * hq * (d + 1), dtype=torch.float32, device=q.device) if splits > 8 else None
+    # fp32 results of clusters of 8 blocks: outputs and the logarithms of their weights; a single cluster needs none
+    part = torch.empty(splits // 8 * b * t * hq * (d + 1), dtype=torch.float32, device=q.device) if splits > 8 else None
     _ok(_L().nb_cached_attention(ptr(q), ptr(k_codes), ptr(k_scale), ptr(v_codes), ptr(v_scale), ptr(out), ptr(table), ptr(past), ptr(count),
                                  _wide(table, past, count), b, t, hq, h, d, n, blocks, table.shape[1], *q.stride()[:3], float(scale), int(causal),
                                  splits, ptr(part), fp32, stream_ptr()), "cached_attention", 2 if splits > 8 else 1)
