@@ -35,7 +35,7 @@ TARGETS: dict[str, tuple[list[str], list[str]]] = {
     "libnb_gemm.so": (["gemm_tcgen05.cu"], []),
     "libnb_kernels.so": (["fused_kernels.cu", "elementwise_kernels.cu"], []),
     "libnb_attention.so": (["attention_tcgen05.cu"], []),
-    "libnb_serving.so": (["kv_cache.cu", "cached_attention.cu", "logits.cu"], []),
+    "libnb_serving.so": (["kv_cache.cu", "cached_attention.cu", "cached_attention_tcgen05.cu", "logits.cu"], []),
     "libnb_comm.so": (["peer_collectives.cu"], []),
     "libnb_runtime.so": (["plan_runtime.cpp"], []),
     "libnb_noalloc.so": (["no_alloc_entry.cu"], []),

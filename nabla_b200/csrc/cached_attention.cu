@@ -6,74 +6,12 @@
 // `count` on, and rows that see no key, are zero. `group` query heads share a head of the cache.
 #include <cooperative_groups.h>
 
-#include "kv_cache.cuh"
+#include "cached_attention.cuh"
 
 namespace nbc {
 using nb::follow_grid;
 using nb::launch_following;
 
-struct AttendArgs {
-  const void* q;                 // [batch][new][heads][D]
-  long long q_sb, q_st, q_sh;        // its strides in elements
-  const int8_t* codes[2];        // keys, values
-  const float* scales[2];
-  Table table;
-  Whole past, count;             // count.p null: all of them
-  void* out;                     // [batch][new][heads][D], dense
-  int batch, fresh, heads, kv_heads, block_log, causal;
-  float scale_log2;              // softmax scale * log2(e)
-  int splits, cluster;           // ranges of keys, one block each; blocks of a cluster, which join theirs
-  float *part_o, *part_w;        // where there are several clusters: [splits / cluster][batch][kv_heads][new * group] output over their ranges, and
-                                 // log2 of the sum of its weights
-};
-
-// Four neighbouring numbers of row r (token r / group, head r % group) of cache head h.
-template <typename T, int D>
-__device__ __forceinline__ void store_out(const AttendArgs& a, int b, int h, int r, int c, float4 x) {
-  const int group = a.heads / a.kv_heads;
-  T* p = static_cast<T*>(a.out) + (((long long)b * a.fresh + r / group) * a.heads + h * group + r % group) * D + 4 * c;
-  if constexpr (sizeof(T) == 4) {
-    *reinterpret_cast<float4*>(p) = x;
-  } else {
-    __nv_bfloat162 u = __floats2bfloat162_rn(x.x, x.y), w = __floats2bfloat162_rn(x.z, x.w);
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&u), *reinterpret_cast<uint32_t*>(&w));
-  }
-}
-
-template <int D>
-__device__ __forceinline__ void store_part(const AttendArgs& a, int part, int b, int h, int r, int c, float4 x, float weight) {
-  const long long at = (((long long)part * a.batch + b) * a.kv_heads + h) * a.fresh * (a.heads / a.kv_heads) + r;
-  reinterpret_cast<float4*>(a.part_o)[at * (D / 4) + c] = x;
-  if (c == 0) a.part_w[at] = weight;
-}
-
-// ---------------------------------------------------------------- matrix instructions on codes
-// A code c becomes the 16-bit float 1024 + (c + 128) by placing its byte under the exponent of 1024; less 1152 that is c, exactly. So
-// keys and values go into products of 16-bit floats (fp32 sums) without a rounding. What is rounded is the other operand:
-//  - queries, to 11 bits after a power of two that brings a row's largest to [2^8, 2^9); bf16 has 8 bits, so those are exact (down to 2^-23 of the largest),
-//  - weights, to 11 bits. fp32 calls carry queries and weights as two such parts (22 bits) and take two products.
-// Scales never meet a rounding: a key's goes into its score, and a value's into the exponent of its weight. With
-//     t_j = scale * log2(e) * s_k(j) * (q . k_j) + log2 s_v(j),   m = max t_j,   P_j = 2^(t_j - m)
-// the output is sum P_j v_j / sum (P_j / s_v(j)), and the largest P is 1 however the scales differ. Where they differ so much that a P which counts in
-// the lower sum falls out of the range of fp32, P_j / s_v(j) is taken as an exponential of its own.
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t half2_minus(uint32_t x, uint32_t y) {
-  uint32_t d;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
-  return d;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
-  uint32_t d;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
-  return d;
-}
-// 1024 + 128 + codes 0, 1 (sel 0x4140) or 2, 3 (sel 0x4342) of a word of biased codes
-__device__ __forceinline__ uint32_t widen(uint32_t biased, uint32_t sel) { return __byte_perm(biased, 0x64646464u, sel); }
-constexpr uint32_t BIAS2 = 0x64806480u;      // 1152 twice
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -85,18 +23,6 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-// Codes are read once by a block, past L1. (The address comes from the table, so these cannot move ahead of the wait for the grid ahead.)
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 v;
-  asm("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-  uint2 v;
-  asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
 // ---------------------------------------------------------------- few rows
 // Up to 8 * RT rows (tokens times heads of a group) of one sequence and cache head, over one of `splits` ranges of its keys. The codes are the
 // large operand of the products: S^T = K Q^T (16 keys by 8 rows) and O^T = V^T P^T (16 dims by 8 rows), so no part of a product is padding when
@@ -512,12 +438,20 @@ __global__ void __launch_bounds__(64) attend_join_kernel(const AttendArgs a) {
   store_out<T, D>(a, b, h, r, c, x);
 }
 
+// Above this many rows of a sequence and cache head, bf16 goes to tiles of 128 rows (cached_attention_tcgen05.cu).
+constexpr int MANY = 32;
+static bool many(int rows, int fp32) { return !fp32 && rows > MANY; }
+
 // Ranges of keys for each (sequence, head, tile of rows), by sizes alone. A cluster of up to 8 blocks joins its ranges in distributed shared memory; more
 // go through memory and a second kernel.
 static int few_rows(int rows) { return rows <= 8 ? 8 : 16; }
-static int few_splits(int batch, int fresh, int heads, int kv_heads, long long room) {
-  const int rows = fresh * (heads / kv_heads), tile = few_rows(rows);
+static int splits_for(int batch, int rows, int kv_heads, long long room, int fp32) {
+  const int tile = many(rows, fp32) ? 128 : few_rows(rows);
   const long long units = (long long)batch * kv_heads * ((rows + tile - 1) / tile);
+  if (many(rows, fp32)) {
+    const long long most = (room + 511) / 512, want = 148 / units;           // four tiles of keys at least
+    return static_cast<int>(want < 2 || most < 2 ? 1 : want < most ? want : most);
+  }
   const long long most = (room + FEW_WARPS * STEP - 1) / (FEW_WARPS * STEP);           // a step for each warp at least
   long long want = (296 + units - 1) / units;
   if (want <= 8) want = 8;
@@ -527,6 +461,12 @@ static int few_splits(int batch, int fresh, int heads, int kv_heads, long long r
   if (want > most) want = most;
   want = want >= 8 ? want / 8 * 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
   return static_cast<int>(want > 128 ? 128 : want);
+}
+
+template <typename T, int D>
+static cudaError_t join(const AttendArgs& a, cudaStream_t stream) {
+  if (a.splits == a.cluster) return cudaSuccess;
+  return launch_following(attend_join_kernel<T, D>, dim3(static_cast<unsigned>((long long)a.batch * a.fresh * a.heads)), dim3(64), 0, stream, a);
 }
 
 template <typename T, int D, int RT>
@@ -552,27 +492,33 @@ static cudaError_t launch_few(const AttendArgs& a, cudaStream_t stream) {
   }
   nb::set_following(cfg);
   e = cudaLaunchKernelEx(&cfg, kernel, a);
-  if (e != cudaSuccess || a.splits == a.cluster) return e;
-  return launch_following(attend_join_kernel<T, D>, dim3(static_cast<unsigned>((long long)a.batch * a.fresh * a.heads)), dim3(64), 0, stream, a);
+  return e != cudaSuccess ? e : join<T, D>(a, stream);
 }
 
 template <typename T, int D>
-static cudaError_t launch_attend(const AttendArgs& a, cudaStream_t stream) {
-  return few_rows(a.fresh * (a.heads / a.kv_heads)) == 8 ? launch_few<T, D, 1>(a, stream) : launch_few<T, D, 2>(a, stream);
+static cudaError_t launch_attend(const AttendArgs& a, int* status, cudaStream_t stream) {
+  const int rows = a.fresh * (a.heads / a.kv_heads);
+  if (many(rows, sizeof(T) == 4)) {
+    if (a.cluster != 1) return cudaErrorInvalidValue;       // its ranges are not joined in clusters
+    const cudaError_t e = launch_many<D>(a, status, stream);
+    return e != cudaSuccess ? e : join<T, D>(a, stream);
+  }
+  return few_rows(rows) == 8 ? launch_few<T, D, 1>(a, stream) : launch_few<T, D, 2>(a, stream);
 }
 
 }  // namespace nbc
 
-// Ranges of keys that nb_cached_attention is to be called with for these sizes. Above 8 it needs scratch: splits / 8 * batch * new * heads *
-// (head_dim + 1) floats.
+// Ranges of keys that nb_cached_attention is to be called with for these sizes (positive), and blocks of a cluster that join theirs (in bits 16 and up). Where
+// the two differ it needs scratch: ranges / cluster * batch * new * heads * (head_dim + 1) floats.
 extern "C" int nb_cached_attention_splits(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int columns, int fp32) {
-  return nbc::few_splits(batch, fresh, heads, kv_heads, (long long)columns * block);
+  const int rows = fresh * (heads / kv_heads), s = nbc::splits_for(batch, rows, kv_heads, (long long)columns * block, fp32);
+  return s | (nbc::many(rows, fp32) ? 1 : s < 8 ? s : 8) << 16;
 }
 
 extern "C" int nb_cached_attention(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, void* out,
                                    const void* table, const void* past, const void* count, int wide, int batch, int fresh, int heads, int kv_heads,
                                    int head_dim, int block, int blocks, int columns, long long q_sb, long long q_st, long long q_sh, float scale,
-                                   int causal, int splits, float* scratch, int fp32, void* stream) {
+                                   int causal, int splits, float* scratch, int fp32, int* status, void* stream) {
   using namespace nbc;
   AttendArgs a = {};
   a.q = q, a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh;
@@ -585,13 +531,13 @@ extern "C" int nb_cached_attention(const void* q, const void* k_codes, const voi
   a.batch = batch, a.fresh = fresh, a.heads = heads, a.kv_heads = kv_heads, a.causal = causal;
   a.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : -1;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.splits = splits, a.cluster = splits < 8 ? splits : 8;
-  if (splits != 1 && splits != 2 && splits != 4 && splits % 8 != 0) return -1;
-  a.part_o = scratch, a.part_w = scratch + (long long)(splits / a.cluster) * batch * fresh * heads * head_dim;
+  a.splits = splits & 0xffff, a.cluster = splits >> 16;
+  if (a.cluster < 1 || a.cluster > 8 || a.splits < a.cluster || a.splits % a.cluster != 0 || (a.splits > a.cluster && scratch == nullptr)) return -1;
+  a.part_o = scratch, a.part_w = scratch + (long long)(a.splits / a.cluster) * batch * fresh * heads * head_dim;
   if (a.block_log < 0 || (head_dim != 64 && head_dim != 128)) return -1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (fp32) return head_dim == 64 ? launch_attend<float, 64>(a, s) : launch_attend<float, 128>(a, s);
-  return head_dim == 64 ? launch_attend<__nv_bfloat16, 64>(a, s) : launch_attend<__nv_bfloat16, 128>(a, s);
+  if (fp32) return head_dim == 64 ? launch_attend<float, 64>(a, status, s) : launch_attend<float, 128>(a, status, s);
+  return head_dim == 64 ? launch_attend<__nv_bfloat16, 64>(a, status, s) : launch_attend<__nv_bfloat16, 128>(a, status, s);
 }
 
 NB_DEBUG_DEFINE(cached_attention)

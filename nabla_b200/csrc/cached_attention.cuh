@@ -1,0 +1,85 @@
+// What the kernels of attention over a key / value cache in 8 bits share (the operation: cached_attention.cu).
+#pragma once
+#include "kv_cache.cuh"
+
+namespace nbc {
+
+struct AttendArgs {
+  const void* q;                 // [batch][new][heads][D]
+  long long q_sb, q_st, q_sh;        // its strides in elements
+  const int8_t* codes[2];        // keys, values
+  const float* scales[2];
+  Table table;
+  Whole past, count;             // count.p null: all of them
+  void* out;                     // [batch][new][heads][D], dense
+  int batch, fresh, heads, kv_heads, block_log, causal;
+  float scale_log2;              // softmax scale * log2(e)
+  int splits, cluster;           // ranges of keys, one block each; blocks of a cluster, which join theirs
+  float *part_o, *part_w;        // where there are several clusters: [splits / cluster][batch][kv_heads][new * group] output over their ranges, and
+                                 // log2 of the sum of its weights
+};
+
+// Four neighbouring numbers of row r (token r / group, head r % group) of cache head h.
+template <typename T, int D>
+__device__ __forceinline__ void store_out(const AttendArgs& a, int b, int h, int r, int c, float4 x) {
+  const int group = a.heads / a.kv_heads;
+  T* p = static_cast<T*>(a.out) + (((long long)b * a.fresh + r / group) * a.heads + h * group + r % group) * D + 4 * c;
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4*>(p) = x;
+  } else {
+    __nv_bfloat162 u = __floats2bfloat162_rn(x.x, x.y), w = __floats2bfloat162_rn(x.z, x.w);
+    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&u), *reinterpret_cast<uint32_t*>(&w));
+  }
+}
+
+template <int D>
+__device__ __forceinline__ void store_part(const AttendArgs& a, int part, int b, int h, int r, int c, float4 x, float weight) {
+  const long long at = (((long long)part * a.batch + b) * a.kv_heads + h) * a.fresh * (a.heads / a.kv_heads) + r;
+  reinterpret_cast<float4*>(a.part_o)[at * (D / 4) + c] = x;
+  if (c == 0) a.part_w[at] = weight;
+}
+
+// ---------------------------------------------------------------- matrix instructions on codes
+// A code c becomes the 16-bit float 1024 + (c + 128) by placing its byte under the exponent of 1024; less 1152 that is c, exactly. So
+// keys and values go into products of 16-bit floats (fp32 sums) without a rounding. What is rounded is the other operand:
+//  - queries, to 11 bits after a power of two that brings a row's largest to [2^8, 2^9); bf16 has 8 bits, so those are exact (down to 2^-23 of the largest),
+//  - weights, to 11 bits. fp32 calls carry queries and weights as two such parts (22 bits) and take two products.
+// Scales never meet a rounding: a key's goes into its score, and a value's into the exponent of its weight. With
+//     t_j = scale * log2(e) * s_k(j) * (q . k_j) + log2 s_v(j),   m = max t_j,   P_j = 2^(t_j - m)
+// the output is sum P_j v_j / sum (P_j / s_v(j)), and the largest P is 1 however the scales differ. Where they differ so much that a P which counts in
+// the lower sum falls out of the range of fp32, P_j / s_v(j) is taken as an exponential of its own.
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_minus(uint32_t x, uint32_t y) {
+  uint32_t d;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(x), "r"(y));
+  return d;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  uint32_t d;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+// 1024 + 128 + codes 0, 1 (sel 0x4140) or 2, 3 (sel 0x4342) of a word of biased codes
+__device__ __forceinline__ uint32_t widen(uint32_t biased, uint32_t sel) { return __byte_perm(biased, 0x64646464u, sel); }
+constexpr uint32_t BIAS2 = 0x64806480u;      // 1152 twice
+// Codes are read once by a block, past L1. (The address comes from the table, so these cannot move ahead of the wait for the grid ahead.)
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 v;
+  asm("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  uint2 v;
+  asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// Many rows: tiles of 128 rows on the tensor cores (cached_attention_tcgen05.cu), bf16 only.
+template <int D>
+cudaError_t launch_many(const AttendArgs& a, int* status, cudaStream_t stream);
+
+}  // namespace nbc

@@ -22,7 +22,7 @@ _status: dict[int, torch.Tensor] = {}
 _debug_rec: dict[int, torch.Tensor] = {}
 # translation units of each library (each has its own nb_debug_bind_<tu> / nb_debug_enabled_<tu>)
 _DEBUG_UNITS = {"libnb_gemm.so": ("gemm",), "libnb_kernels.so": ("fused", "elementwise"),
-                "libnb_attention.so": ("attention",), "libnb_serving.so": ("kv_cache", "cached_attention", "logits"),
+                "libnb_attention.so": ("attention",), "libnb_serving.so": ("kv_cache", "cached_attention", "cached_attention_tcgen05", "logits"),
                 "libnb_comm.so": ("comm",)}
 
 

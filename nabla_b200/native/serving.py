@@ -10,7 +10,7 @@ import functools
 
 import torch
 
-from . import load, ptr, recorder, stream_ptr
+from . import load, ptr, recorder, status_word, stream_ptr
 
 _lib = None
 launch_count = 0
@@ -24,7 +24,7 @@ def _L():
         sig = {
             "nb_kv_write": [c_vp] * 9 + [c_int] * 8 + [c_ll] * 6 + [c_int, c_vp],
             "nb_kv_read": [c_vp] * 9 + [c_int] * 9 + [c_vp],
-            "nb_cached_attention": [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_int, c_vp, c_int, c_vp],
+            "nb_cached_attention": [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_int, c_vp, c_int, c_vp, c_vp],
             "nb_cached_attention_splits": [c_int] * 8,
             "nb_adjust_logits": [c_vp] * 9 + [c_ll, c_vp] + [c_int] * 6 + [c_vp],
         }
@@ -93,11 +93,12 @@ def cached_attention(q, k_codes, k_scale, v_codes, v_scale, table, past, count, 
     out = torch.empty((b, t, hq, d), dtype=q.dtype, device=q.device)
     fp32 = int(q.dtype == torch.float32)
     splits = _splits(b, t, hq, h, d, n, table.shape[1], fp32)
-    # fp32 results of clusters of 8 blocks: outputs and the logarithms of their weights; a single cluster needs none
-    part = torch.empty(splits // 8 * b * t * hq * (d + 1), dtype=torch.float32, device=q.device) if splits > 8 else None
+    # fp32 results of ranges of keys: outputs and the logarithms of their weights; those of one cluster of blocks need none
+    parts = (splits & 0xffff) // (splits >> 16)
+    part = torch.empty(parts * b * t * hq * (d + 1), dtype=torch.float32, device=q.device) if parts > 1 else None
     _ok(_L().nb_cached_attention(ptr(q), ptr(k_codes), ptr(k_scale), ptr(v_codes), ptr(v_scale), ptr(out), ptr(table), ptr(past), ptr(count),
                                  _wide(table, past, count), b, t, hq, h, d, n, blocks, table.shape[1], *q.stride()[:3], float(scale), int(causal),
-                                 splits, ptr(part), fp32, stream_ptr()), "cached_attention", 2 if splits > 8 else 1)
+                                 splits, ptr(part), fp32, ptr(status_word(q.device)), stream_ptr()), "cached_attention", 2 if parts > 1 else 1)
     return out
 
 
