@@ -394,6 +394,27 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           tmem_st_32x32(t_o + c * 32, o);
         }
       }
+      // weights that are lost in fp32 may count once their value's scale is taken out: exponentials of their own (rare)
+      uint32_t small = 0;
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) small |= (gt[k] < base - 100.f && gt[k] > -INFINITY ? 1u : 0u) << k;
+      if (__any_sync(0xffffffffu, small != 0)) {
+#pragma unroll 1
+        for (int k = 0; k < GROUPS; ++k) {
+          uint32_t x[16];
+          tmem_ld_32x16(t_s + 16 * k, x);
+          tmem_ld_wait();
+          float f = sc[k] * row_mul;
+          f = f < 1e-37f ? 1e-37f : f;
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            asm volatile("" : "+r"(x[i]));
+            sum += ex2(fmaf(__uint_as_float(x[i]), f, fmaf(-offset, f, sc[GROUPS + k])) - base - sc[GROUPS + k]);
+          }
+          if (small >> k & 1) l += sum;
+        }
+      }
       // pass 2: weights over the first 64 columns of the scores
 #pragma unroll
       for (int c = 0; c < BT / 32; ++c) {
@@ -411,19 +432,15 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           const float lg = sc[GROUPS + gi], add = fmaf(-offset, f, lg);
           const float2 f2 = make_float2(f, f), a2 = make_float2(add, add), b2 = make_float2(-base, -base);
           float2 acc = make_float2(0.f, 0.f);
-          float apart = 0.f;
-          const bool small = gt[gi] < base - 100.f && gt[gi] > -INFINITY;      // weights that are lost in fp32 may count without their value's scale
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float2 x = __fadd2_rn(__ffma2_rn(two(v[16 * k + 2 * i], v[16 * k + 2 * i + 1]), f2, a2), b2);
             const float2 p = make_float2(ex2(x.x), ex2(x.y));
             acc = __fadd2_rn(acc, p);
-            if (small) apart += ex2(x.x - lg) + ex2(x.y - lg);
             pk[8 * k + i] = pack_half2(p.x, p.y);
           }
           const float sum = acc.x + acc.y;
-          if (small) l += apart;
-          else if (sum != 0.f) l = fmaf(sum, sc[2 * GROUPS + gi], l);           // a row that sees none of these keys does not see their scale either
+          if (sum != 0.f && !(small >> gi & 1)) l = fmaf(sum, sc[2 * GROUPS + gi], l);       // a row that sees none of these keys does not see their scale either
         }
         st_tmem16(t_s + c * 16, pk);
       }
