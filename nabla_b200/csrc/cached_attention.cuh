@@ -66,18 +66,6 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 // 1024 + 128 + codes 0, 1 (sel 0x4140) or 2, 3 (sel 0x4342) of a word of biased codes
 __device__ __forceinline__ uint32_t widen(uint32_t biased, uint32_t sel) { return __byte_perm(biased, 0x64646464u, sel); }
 constexpr uint32_t BIAS2 = 0x64806480u;      // 1152 twice
-// Codes are read once by a block, past L1. (The address comes from the table, so these cannot move ahead of the wait for the grid ahead.)
-__device__ __forceinline__ uint4 ldg16(const void* p) {
-  uint4 v;
-  asm("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 ldg8(const void* p) {
-  uint2 v;
-  asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
 // Many rows: tiles of 128 rows on the tensor cores (cached_attention_tcgen05.cu), bf16 only.
 template <int D>
 cudaError_t launch_many(const AttendArgs& a, int* status, cudaStream_t stream);

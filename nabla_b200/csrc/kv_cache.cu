@@ -25,9 +25,21 @@ struct WriteArgs {
   int batch, fresh, heads, block_log, columns;     // fresh: new tokens, columns: table columns that a sequence may touch
 };
 
-__device__ __forceinline__ float scale_for(float top) {      // top: the largest magnitude, NaN kept
-  const float s = top * (1.0f / 127.0f);
-  return s < INFINITY ? fmaxf(s, LEAST_SCALE) : __int_as_float(0x7fc00000);
+__device__ __forceinline__ float scale_for(uint32_t top) {      // bits of the largest magnitude; those of infinities and NaN are the largest
+  return top < 0x7f800000u ? fmaxf(__uint_as_float(top) * (1.0f / 127.0f), LEAST_SCALE) : __int_as_float(0x7fc00000);
+}
+// Codes of four numbers. The product with 1 / scale is at most 127.00002 in magnitude; with 1.5 * 2^23 added its nearest whole number stands in
+// the low byte.
+__device__ __forceinline__ uint32_t codes4(float2 a, float2 b, float2 inverse) {
+  const float2 magic = make_float2(12582912.f, 12582912.f);
+  a = __fadd2_rn(__fmul2_rn(a, inverse), magic);
+  b = __fadd2_rn(__fmul2_rn(b, inverse), magic);
+  return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040),
+                     0x5410);
+}
+// Code i of a word, exactly: its byte, with 128 added, under the exponent of 2^23.
+__device__ __forceinline__ float code_value(uint32_t biased, int i) {
+  return __uint_as_float(__byte_perm(biased, 0x4b000000u, 0x7440 | i)) - 8388736.f;
 }
 
 template <typename T, int D, int THREADS, int VECS>
@@ -41,79 +53,59 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(const WriteArgs a) {
   id /= a.heads;
   const int j = id % a.columns, b = id / a.columns;
   const int n = 1 << a.block_log;
-  const long long room = (long long)a.table.columns << a.block_log;
+  const int room = a.table.columns << a.block_log;
   const int past = clamp_tokens(a.past.at(b), room);
   const int count = clamp_tokens(a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
   const int column = (past >> a.block_log) + j;
-  const long long first = (long long)column << a.block_log;       // position of the block's first row
-  const int f = static_cast<int>(max(past - first, 0ll));                  // rows [f, e) are new
-  const int e = static_cast<int>(min((long long)n, past + (long long)count - first));
-  if (e <= f) return;
+  const int first = column << a.block_log;              // position of the block's first row
+  const int f = max(past - first, 0), e = min(n, past + count - first);       // rows [f, e) are new
+  if (e <= f || column >= a.table.columns) return;
   const int block = a.table.block(b, column);
-  if (block < 0) return;
-  const long long unit = (long long)block * a.heads + h;
-  int8_t* codes = a.codes[which] + unit * n * D;
-  float* scale = a.scales[which] + unit;
-  const float before = f > 0 ? *scale : 0.f;
 
-  const T* in = static_cast<const T*>(a.in[which]) + b * a.sb[which] + h * a.sh[which];
-  float x[VECS][8];
-  float top = 0.f;
-  bool odd = false;              // something that is not finite
+  const T* in = static_cast<const T*>((which ? a.in[1] : a.in[0])) + b * (which ? a.sb[1] : a.sb[0]) + h * (which ? a.sh[1] : a.sh[0]);
+  Eight<T> x[VECS];
+  uint32_t top = 0;
 #pragma unroll
   for (int u = 0; u < VECS; ++u) {
     const int i = u * THREADS + threadIdx.x, r = i / PER_ROW, c = i % PER_ROW;
-    if (r >= f && r < e) {
-      load8(in + (first + r - past) * a.st[which] + c * 8, x[u]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[u][k] = 0.f;
-    }
+    if (r >= f && r < e) x[u].load(in + (first + r - past) * (which ? a.st[1] : a.st[0]) + c * 8); else x[u].clear();
   }
+  if (block < 0) return;
+  const long long unit = (long long)block * a.heads + h;
+  int8_t* codes = (which ? a.codes[1] : a.codes[0]) + unit * n * D;
+  float* scale = (which ? a.scales[1] : a.scales[0]) + unit;
+  const float before = f > 0 ? scale_at(scale, 0) : 0.f;
 #pragma unroll
-  for (int u = 0; u < VECS; ++u)
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      top = fmaxf(top, fabsf(x[u][k]));
-      odd |= !(fabsf(x[u][k]) < INFINITY);
-    }
-  top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(odd ? INFINITY : top)));     // magnitudes order as their bits do
-  __shared__ float tops[THREADS / 32];
+  for (int u = 0; u < VECS; ++u) top = max(top, x[u].top());
+  top = __reduce_max_sync(0xffffffffu, top);
+  __shared__ uint32_t tops[THREADS / 32];
   if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) top = fmaxf(top, tops[w]);
+  for (int w = 0; w < THREADS / 32; ++w) top = max(top, tops[w]);
   float now = scale_for(top);
   now = before > now || before != before ? before : now;
   const float inverse = 1.0f / now;
   if (threadIdx.x == 0) *scale = now;
   const bool known = now == now;
+  const float2 inverse2 = make_float2(inverse, inverse);
 #pragma unroll
   for (int u = 0; u < VECS; ++u) {
-    const int i = u * THREADS + threadIdx.x, r = i / PER_ROW, c = i % PER_ROW;
+    const int i = u * THREADS + threadIdx.x, r = i / PER_ROW;
     if (r < f || r >= e) continue;
-    uint32_t w[2] = {0u, 0u};
-    if (known) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int q = max(-127, min(127, __float2int_rn(x[u][k] * inverse)));
-        w[k / 4] |= (static_cast<uint32_t>(q) & 0xffu) << (8 * (k & 3));
-      }
-    }
-    *reinterpret_cast<uint2*>(codes + r * D + c * 8) = make_uint2(w[0], w[1]);
+    uint2 w = make_uint2(codes4(x[u].pair(0), x[u].pair(1), inverse2), codes4(x[u].pair(2), x[u].pair(3), inverse2));
+    if (!known) w = make_uint2(0, 0);
+    *reinterpret_cast<uint2*>(codes + i * 8) = w;
   }
   if (f == 0 || now == before || !known) return;
   const float ratio = before * inverse;
+  const float2 ratio2 = make_float2(ratio, ratio);
   for (int i = threadIdx.x; i < f * PER_ROW; i += THREADS) {
-    uint2 v = *reinterpret_cast<const uint2*>(codes + i * 8);
-    uint32_t w[2] = {v.x, v.y}, o[2] = {0u, 0u};
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int q = static_cast<int8_t>(w[k / 4] >> (8 * (k & 3)));
-      const int t = max(-127, min(127, __float2int_rn(static_cast<float>(q) * ratio)));
-      o[k / 4] |= (static_cast<uint32_t>(t) & 0xffu) << (8 * (k & 3));
-    }
-    *reinterpret_cast<uint2*>(codes + i * 8) = make_uint2(o[0], o[1]);
+    const uint2 v = *reinterpret_cast<const uint2*>(codes + i * 8);
+    const uint32_t p = v.x ^ 0x80808080u, q = v.y ^ 0x80808080u;
+    *reinterpret_cast<uint2*>(codes + i * 8) =
+        make_uint2(codes4(make_float2(code_value(p, 0), code_value(p, 1)), make_float2(code_value(p, 2), code_value(p, 3)), ratio2),
+                   codes4(make_float2(code_value(q, 0), code_value(q, 1)), make_float2(code_value(q, 2), code_value(q, 3)), ratio2));
   }
 }
 
@@ -125,46 +117,70 @@ struct ReadArgs {
   Table table;
   Whole start, count;
   int batch, most, heads, block_log, columns;      // columns: table columns that the rows of a sequence may touch
-  long long vectors;             // of 16 codes, of one of keys and values: batch * columns * heads * N * D / 16
 };
 
+// Sixteen codes times a scale: each product is rounded once to fp32, as a code is exact there, and to bf16 where that is asked for.
+__device__ __forceinline__ float2 two_values(uint32_t biased, int i, float2 s) {
+  return __fmul2_rn(make_float2(code_value(biased, i), code_value(biased, i + 1)), s);
+}
+template <typename T>
+__device__ __forceinline__ void put16(T* p, uint4 v, float s) {
+  const uint32_t w[4] = {v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u};
+  const float2 s2 = make_float2(s, s);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 x = two_values(w[k], 0, s2), y = two_values(w[k], 2, s2);
+      reinterpret_cast<float4*>(p)[k] = make_float4(x.x, x.y, y.x, y.y);
+    }
+  } else {
+    uint32_t o[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const float2 x = two_values(w[k / 2], 2 * (k & 1), s2);
+      const __nv_bfloat162 y = __floats2bfloat162_rn(x.x, x.y);
+      o[k] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    reinterpret_cast<uint4*>(p)[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    reinterpret_cast<uint4*>(p)[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  }
+}
+
+// One block of threads takes one cache block and head, keys or values.
+constexpr int READ_THREADS = 128;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_read_kernel(const ReadArgs a) {
+__global__ void __launch_bounds__(READ_THREADS) kv_read_kernel(const ReadArgs a) {
   constexpr int PER_ROW = D / 16;
   follow_grid();
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (at >= a.vectors) return;
-  const int which = blockIdx.y;
+  int id = blockIdx.x;
+  const int which = id & 1;
+  id >>= 1;
+  const int h = id % a.heads;
+  id /= a.heads;
+  const int j = id % a.columns, b = id / a.columns;
   const int n = 1 << a.block_log;
-  const int c = static_cast<int>(at % PER_ROW);
-  long long rest = at / PER_ROW;
-  const int r = static_cast<int>(rest & (n - 1));
-  rest >>= a.block_log;
-  const int h = static_cast<int>(rest % a.heads);
-  rest /= a.heads;
-  const int j = static_cast<int>(rest % a.columns), b = static_cast<int>(rest / a.columns);
-  const long long room = (long long)a.table.columns << a.block_log;
-  const int start = clamp_tokens(a.start.at(b), room);
-  const int count = clamp_tokens(a.count.at(b), a.most);
-  const int column = (start >> a.block_log) + j;
-  const long long i = ((long long)column << a.block_log) + r - start;        // row of the result
-  if (i < 0 || i >= a.most) return;
-  T o[16];
-  const int block = i < count ? a.table.block(b, column) : -1;
-  if (block >= 0) {
-    const long long unit = (long long)block * a.heads + h;
-    const int4 v = *reinterpret_cast<const int4*>(a.codes[which] + (unit * n + r) * D + c * 16);
-    const float s = a.scales[which][unit];
-    const int w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int k = 0; k < 16; ++k) o[k] = round_to<T>(static_cast<float>(static_cast<int8_t>(w[k / 4] >> (8 * (k & 3)))) * s);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 16; ++k) o[k] = round_to<T>(0.f);
+  const int room = a.table.columns << a.block_log;
+  const int start = clamp_tokens(a.start.at(b), room), count = clamp_tokens(a.count.at(b), a.most);
+  const int column = (start >> a.block_log) + j, first = (column << a.block_log) - start;       // the block's first row in the result
+  // rows [from, to) of the block lie in the result, those from `end` on are zero
+  const int from = max(-first, 0), to = static_cast<int>(min((long long)n, (long long)a.most - first));
+  const int block = first + from < count ? a.table.block(b, column) : -1;
+  const int end = block < 0 ? 0 : static_cast<int>(min((long long)to, (long long)count - first));
+  const long long unit = (long long)max(block, 0) * a.heads + h;
+  const int8_t* codes = (which ? a.codes[1] : a.codes[0]) + unit * n * D;
+  const float s = block < 0 ? 0.f : scale_at((which ? a.scales[1] : a.scales[0]), unit);
+  T* out = static_cast<T*>((which ? a.out[1] : a.out[0])) + (((long long)b * a.most + first) * a.heads + h) * D;
+  const long long row = (long long)a.heads * D;
+  for (int i0 = from * PER_ROW + threadIdx.x; i0 < to * PER_ROW; i0 += READ_THREADS * 4) {
+    // four vectors under way at once
+    const int i1 = i0 + READ_THREADS, i2 = i1 + READ_THREADS, i3 = i2 + READ_THREADS;
+    const uint4 none = make_uint4(0, 0, 0, 0), v0 = i0 < end * PER_ROW ? ldg16(codes + i0 * 16) : none, v1 = i1 < end * PER_ROW ? ldg16(codes + i1 * 16) : none,
+                v2 = i2 < end * PER_ROW ? ldg16(codes + i2 * 16) : none, v3 = i3 < end * PER_ROW ? ldg16(codes + i3 * 16) : none;
+    auto put = [&](int i, uint4 v) {
+      if (i < to * PER_ROW) put16<T>(out + (i / PER_ROW) * row + (i % PER_ROW) * 16, v, i < end * PER_ROW ? s : 0.f);
+    };
+    put(i0, v0), put(i1, v1), put(i2, v2), put(i3, v3);
   }
-  T* out = static_cast<T*>(a.out[which]) + (((long long)b * a.most + i) * a.heads + h) * D + c * 16;
-#pragma unroll
-  for (int k = 0; k < static_cast<int>(sizeof(o) / 16); ++k) reinterpret_cast<uint4*>(out)[k] = reinterpret_cast<const uint4*>(o)[k];
 }
 
 template <typename T, int D>
@@ -184,9 +200,9 @@ static cudaError_t launch_write(const WriteArgs& a, cudaStream_t stream) {
 
 template <typename T, int D>
 static cudaError_t launch_read(const ReadArgs& a, cudaStream_t stream) {
-  const long long grid = (a.vectors + 255) / 256;
+  const long long grid = 2ll * a.heads * a.columns * a.batch;
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  return launch_following(kv_read_kernel<T, D>, dim3(static_cast<unsigned>(grid), 2), dim3(256), 0, stream, a);
+  return launch_following(kv_read_kernel<T, D>, dim3(static_cast<unsigned>(grid)), dim3(READ_THREADS), 0, stream, a);
 }
 
 static int block_log(int n) { return n == 16 ? 4 : n == 32 ? 5 : n == 64 ? 6 : n == 128 ? 7 : -1; }
@@ -230,7 +246,6 @@ extern "C" int nb_kv_read(const void* k_codes, const void* k_scales, const void*
   a.batch = batch, a.most = most, a.heads = heads, a.block_log = block_log(block);
   if (a.block_log < 0 || (head_dim != 64 && head_dim != 128)) return -1;
   a.columns = (most + block - 2) / block + 1;
-  a.vectors = (long long)batch * a.columns * heads * block * (head_dim / 16);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (fp32) return head_dim == 64 ? launch_read<float, 64>(a, s) : launch_read<float, 128>(a, s);
   return head_dim == 64 ? launch_read<__nv_bfloat16, 64>(a, s) : launch_read<__nv_bfloat16, 128>(a, s);

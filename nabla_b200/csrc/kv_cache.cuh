@@ -22,9 +22,41 @@ struct Whole {
   const void* p;
   int wide;
   __device__ __forceinline__ long long at(long long i) const {
-    return wide ? static_cast<const long long*>(p)[i] : static_cast<long long>(static_cast<const int*>(p)[i]);
+    long long v;
+    int w;
+    if (wide) {
+      asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(static_cast<const long long*>(p) + i));      // volatile: behind the wait for the grid ahead
+      return v;
+    }
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(w) : "l"(static_cast<const int*>(p) + i));
+    return w;
   }
 };
+// Numbers i, i + step ... below `end` at once, -1 for the others and for what no int holds.
+template <int N>
+__device__ __forceinline__ void several(const Whole& w, long long base, int i, int step, int end, int (&out)[N]) {
+  if (w.wide) {
+    long long v[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v[k] = -1;
+      if (i + k * step < end) asm volatile("ld.global.s64 %0, [%1];" : "=l"(v[k]) : "l"(static_cast<const long long*>(w.p) + base + i + k * step));
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) out[k] = v[k] >= 0 && v[k] <= 0x7fffffff ? static_cast<int>(v[k]) : -1;
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      out[k] = -1;
+      if (i + k * step < end) asm volatile("ld.global.s32 %0, [%1];" : "=r"(out[k]) : "l"(static_cast<const int*>(w.p) + base + i + k * step));
+    }
+  }
+}
+__device__ __forceinline__ float scale_at(const float* p, long long i) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p + i));
+  return v;
+}
 
 struct Table {
   Whole ids;          // [batch][columns]
@@ -57,6 +89,49 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
+// Codes are read once by a block, past L1. (The address comes from the table, so these cannot move ahead of the wait for the grid ahead.)
+__device__ __forceinline__ uint4 ldg16(const void* p) {
+  uint4 v;
+  asm("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg8(const void* p) {
+  uint2 v;
+  asm("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
+// Eight numbers as they lie in memory.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<__nv_bfloat16> {
+  uint4 w;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void clear() { w = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t top() const {              // of the magnitudes, which order as their bits do
+    const uint32_t m = 0x7fff7fffu, x = __vmaxu2(__vmaxu2(w.x & m, w.y & m), __vmaxu2(w.z & m, w.w & m));
+    return max(x & 0xffff0000u, x << 16);
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    const uint32_t x = i == 0 ? w.x : i == 1 ? w.y : i == 2 ? w.z : w.w;
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  }
+};
+template <>
+struct Eight<float> {
+  uint4 w, v;
+  __device__ __forceinline__ void load(const float* p) { w = reinterpret_cast<const uint4*>(p)[0], v = reinterpret_cast<const uint4*>(p)[1]; }
+  __device__ __forceinline__ void clear() { w = v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint32_t top() const {
+    const uint32_t m = 0x7fffffffu;
+    return max(max(max(w.x & m, w.y & m), max(w.z & m, w.w & m)), max(max(v.x & m, v.y & m), max(v.z & m, v.w & m)));
+  }
+  __device__ __forceinline__ float2 pair(int i) const {
+    return i == 0 ? make_float2(__uint_as_float(w.x), __uint_as_float(w.y)) : i == 1 ? make_float2(__uint_as_float(w.z), __uint_as_float(w.w))
+         : i == 2 ? make_float2(__uint_as_float(v.x), __uint_as_float(v.y)) : make_float2(__uint_as_float(v.z), __uint_as_float(v.w));
+  }
+};
 template <typename T>
 __device__ __forceinline__ T round_to(float x);
 template <>
