@@ -41,7 +41,43 @@ struct Few {
   static constexpr int SMEM = (FEW_WARPS * ROWS * (D + 2) + ROWS * (D + 1)) * 4;
 };
 
-template <typename T, int D, int RT, bool CLUSTER>
+// How the keys are shared out:
+//  ONE      a block for all keys of a sequence, head and tile of rows
+//  CLUSTER  a cluster of blocks for them, which joins its ranges in distributed shared memory (few sequences and heads: no second launch)
+//  FLAT     all keys of all sequences and heads in one line, of which every block takes the same length, whatever the lengths of the sequences; a block
+//           writes what it has for the (at most two) lines it does not hold whole, and attend_join_kernel joins them
+enum Share { ONE, CLUSTER, FLAT };
+constexpr int UNIT = FEW_WARPS * STEP, FLAT_BATCH = 1024;      // keys that a line is cut in multiples of; sequences that FLAT takes
+
+// lines[b] = units of sequences in front of b, for b up to the batch, in shared memory. All threads.
+__device__ __forceinline__ void number_lines(const AttendArgs& a, int tiles, int* lines) {
+  __shared__ int sums[FEW_WARPS];
+  const int each = (a.batch + 32 * FEW_WARPS - 1) / (32 * FEW_WARPS), b0 = min(a.batch, static_cast<int>(threadIdx.x) * each), b1 = min(a.batch, b0 + each);
+  const int room = a.table.columns << a.block_log;
+  int own = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int count = clamp_tokens(a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
+    const int keys = count == 0 ? 0 : min(room, clamp_tokens(a.past.at(b), room) + count);
+    const int units = (keys + UNIT - 1) / UNIT * a.kv_heads * tiles;
+    lines[b + 1] = units;
+    own += units;
+  }
+  int sum = own;                 // of the threads up to this one
+#pragma unroll
+  for (int w = 1; w < 32; w <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, sum, w);
+    if ((threadIdx.x & 31) >= w) sum += x;
+  }
+  if ((threadIdx.x & 31) == 31) sums[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  for (int w = 0; w < static_cast<int>(threadIdx.x >> 5); ++w) sum += sums[w];
+  sum -= own;
+  for (int b = b0; b < b1; ++b) sum += lines[b + 1], lines[b + 1] = sum;
+  if (threadIdx.x == 0) lines[0] = 0;
+  __syncthreads();
+}
+
+template <typename T, int D, int RT, Share SHARE>
 __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_kernel(const AttendArgs a) {
   constexpr bool EXACT = sizeof(T) == 4;              // fp32: two parts, codes less their offset before the product
   constexpr int PARTS = EXACT ? 2 : 1, KSTEPS = D / 16, PIECES = D / 64, MT = D / 16, ROWS = 8 * RT;
@@ -49,16 +85,43 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   follow_grid();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int group = a.heads / a.kv_heads, tiles = (a.fresh * group + ROWS - 1) / ROWS;
-  const int sp = blockIdx.x % a.splits, h = blockIdx.x / a.splits % a.kv_heads, tile = blockIdx.x / a.splits / a.kv_heads % tiles,
-            b = blockIdx.x / a.splits / a.kv_heads / tiles;
+  int sp = 0, h = 0, tile = 0, b = 0, line_from = 0, line_to = 0, line = 0;
+  int* lines = reinterpret_cast<int*>(smem) + Few<D, RT>::SMEM / 4;
+  if (SHARE == FLAT) {
+    number_lines(a, tiles, lines);
+    const int all = lines[a.batch];
+    line_from = static_cast<int>((long long)blockIdx.x * all / gridDim.x), line_to = static_cast<int>((long long)(blockIdx.x + 1) * all / gridDim.x);
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= a.batch; i += 32 * FEW_WARPS) a.lines[i] = lines[i];
+  } else {
+    sp = blockIdx.x % a.splits, h = blockIdx.x / a.splits % a.kv_heads, tile = blockIdx.x / a.splits / a.kv_heads % tiles,
+    b = blockIdx.x / a.splits / a.kv_heads / tiles;
+  }
+  for (line = line_from; SHARE != FLAT || line < line_to;) {
+  int piece = 0, slot = 0;             // FLAT: units of this piece, where it goes (-1: it is whole)
+  int unit0 = 0;
+  if (SHARE == FLAT) {
+    int lo = 0, hi = a.batch;          // lines[lo] <= line < lines[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (lines[mid] <= line) lo = mid; else hi = mid;
+    }
+    b = lo;
+    const int units = (lines[b + 1] - lines[b]) / (a.kv_heads * tiles), at = line - lines[b], pair = at / units;
+    h = pair % a.kv_heads, tile = pair / a.kv_heads;
+    unit0 = at - pair * units;
+    piece = min(line_to - line, units - unit0);
+    slot = piece == units ? -1 : 2 * static_cast<int>(blockIdx.x) + (unit0 == 0 ? 1 : 0);
+    line += piece;
+  }
   const int room = a.table.columns << a.block_log, past = clamp_tokens(a.past.at(b), room);
   const int count = clamp_tokens(a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
   const int row0 = tile * ROWS, rows = min(ROWS, a.fresh * group - row0);       // row r: token r / group, head r % group
   const int live = min(rows, count * group - row0);                             // rows from here on are zero
   // keys that the last row sees
   const int keys = live <= 0 ? 0 : static_cast<int>(min((long long)room, (long long)past + (a.causal ? (row0 + live - 1) / group + 1 : count)));
-  const int per = (keys + a.splits * STEP - 1) / (a.splits * STEP) * STEP;
-  const int k0 = min(keys, sp * per), k1 = min(keys, k0 + per);
+  const int per = SHARE == FLAT ? piece * UNIT : (keys + a.splits * STEP - 1) / (a.splits * STEP) * STEP;
+  const int k0 = min(keys, SHARE == FLAT ? unit0 * UNIT : sp * per), k1 = min(keys, k0 + per);
   const int steps = (k1 - k0 + STEP - 1) / STEP, mine = (steps - warp + FEW_WARPS - 1) / FEW_WARPS;
   const int all_see = a.causal ? min(keys - 1, past + row0 / group) : keys - 1;     // keys up to here are seen by every row
   const int n = 1 << a.block_log;
@@ -184,15 +247,18 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   for (int step = 0; step < mine; ++step) {
     float s[RT][2][4];                                // [16 keys each][key g: rows 2t, 2t + 1; key g + 8: the same]
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int u = 0; u < RT; ++u)
 #pragma unroll
-      for (int u = 0; u < RT; ++u) s[u][i][0] = s[u][i][1] = s[u][i][2] = s[u][i][3] = 0.f;
+      for (int i = 0; i < 2; ++i) s[u][i][0] = s[u][i][1] = s[u][i][2] = s[u][i][3] = 0.f;
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) {
-        const uint32_t w[2][4] = {{kr[i][0][p].x, kr[i][0][p].y, kr[i][0][p].z, kr[i][0][p].w}, {kr[i][1][p].x, kr[i][1][p].y, kr[i][1][p].z, kr[i][1][p].w}};
+    for (int p = 0; p < PIECES; ++p) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t x = w[0][k] ^ 0x80808080u, y = w[1][k] ^ 0x80808080u;
+      for (int k = 0; k < 4; ++k) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {                 // (two chains of products, in turn)
+          const uint4 &kx = kr[i][0][p], &ky = kr[i][1][p];
+          const uint32_t x = (k == 0 ? kx.x : k == 1 ? kx.y : k == 2 ? kx.z : kx.w) ^ 0x80808080u,
+                         y = (k == 0 ? ky.x : k == 1 ? ky.y : k == 2 ? ky.z : ky.w) ^ 0x80808080u;
           uint32_t c[4] = {widen(x, 0x4140), widen(y, 0x4140), widen(x, 0x4342), widen(y, 0x4342)};
           if (EXACT)
 #pragma unroll
@@ -365,25 +431,26 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
     const float inverse = sum == 0.f ? 0.f : 1.f / sum;       // NaN stays
     x.x *= inverse, x.y *= inverse, x.z *= inverse, x.w *= inverse;
     const float weight = sum == 0.f ? -INFINITY : top + __log2f(sum);
-    if (CLUSTER) {
+    if (SHARE == CLUSTER) {
       reinterpret_cast<float4*>(to)[i] = x;
       if (c == 0) tl[row] = weight;
-    } else if (a.splits > 1) {
-      store_part<D>(a, sp, b, h, row0 + row, c, x, weight);
+    } else if (SHARE == FLAT && slot >= 0) {
+      reinterpret_cast<float4*>(a.part_o)[((long long)slot * ROWS + row) * (D / 4) + c] = x;
+      if (c == 0) a.part_w[slot * ROWS + row] = weight;
     } else {
       store_out<T, D>(a, b, h, row0 + row, c, x);
     }
   }
-  if (CLUSTER) {
+  if (SHARE == CLUSTER) {
     cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
     cluster.sync();
-    for (int i = sp % a.cluster * 32 * FEW_WARPS + threadIdx.x; i < rows * (D / 4); i += a.cluster * 32 * FEW_WARPS) {
+    for (int i = sp % a.splits * 32 * FEW_WARPS + threadIdx.x; i < rows * (D / 4); i += a.splits * 32 * FEW_WARPS) {
       const int row = i / (D / 4), c = i % (D / 4);
       float top = -INFINITY, sum = 0.f;
       float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int r = 0; r < a.cluster; ++r) top = fmaxf(top, *cluster.map_shared_rank(&tl[row], r));
+      for (int r = 0; r < a.splits; ++r) top = fmaxf(top, *cluster.map_shared_rank(&tl[row], r));
       const float ref = top == -INFINITY ? 0.f : top;
-      for (int r = 0; r < a.cluster; ++r) {
+      for (int r = 0; r < a.splits; ++r) {
         const float f = ex2(*cluster.map_shared_rank(&tl[row], r) - ref);
         const float4 y = *cluster.map_shared_rank(&reinterpret_cast<float4*>(to)[i], r);
         sum += f;
@@ -391,50 +458,91 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
       }
       const float inverse = sum == 0.f ? 0.f : 1.f / sum;
       x.x *= inverse, x.y *= inverse, x.z *= inverse, x.w *= inverse;
-      if (a.splits > a.cluster) {
-        store_part<D>(a, sp / a.cluster, b, h, row0 + row, c, x, sum == 0.f ? -INFINITY : top + __log2f(sum));
-      } else {
-        store_out<T, D>(a, b, h, row0 + row, c, x);
-      }
+      store_out<T, D>(a, b, h, row0 + row, c, x);
     }
     cluster.sync();                                   // a block's shared memory is read until here
   }
+  if (SHARE != FLAT) break;
+  __syncthreads();                                    // before the next piece's results
+  }
 }
 
-// Joins what clusters have written, in their order: one block per row, a thread for four numbers of every second (fourth) part.
-template <typename T, int D>
-__global__ void __launch_bounds__(64) attend_join_kernel(const AttendArgs a) {
-  constexpr int C = D / 4, SIDES = 64 / C;
+// Joins the parts of each row in their order: those of ranges of keys (tiles of 128 rows), or of the pieces of a line (FLAT). One block per row; side s of its
+// threads takes every SIDES-th part.
+constexpr int JOIN_THREADS = 256;
+template <typename T, int D, bool LINES>
+__global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const AttendArgs a) {
+  constexpr int C = D / 4, SIDES = JOIN_THREADS / C;
   __shared__ float4 other[SIDES][C];
-  __shared__ float others[SIDES];
+  __shared__ float others[SIDES], tops[SIDES];
   follow_grid();
-  const int group = a.heads / a.kv_heads, c = threadIdx.x % C, side = threadIdx.x / C, parts = a.splits / a.cluster;
-  const long long rows = (long long)a.batch * a.kv_heads * a.fresh * group, at = blockIdx.x;
+  const int group = a.heads / a.kv_heads, c = threadIdx.x % C, side = threadIdx.x / C;
+  const long long at = blockIdx.x;
+  const int r = static_cast<int>(at % (a.fresh * group)), h = static_cast<int>(at / (a.fresh * group) % a.kv_heads),
+            b = static_cast<int>(at / (a.fresh * group) / a.kv_heads);
+  // part s of this row is number first + s * stride of the rows of parts; FLAT: behind the first, which ends its block's share, those that begin one
+  long long first = at, stride = (long long)a.batch * a.kv_heads * a.fresh * group;
+  int parts = a.splits;
+  bool begins = false;
+  if (LINES) {
+    const int tile = r / a.tile_rows, tiles = (a.fresh * group + a.tile_rows - 1) / a.tile_rows, all = a.lines[a.batch];
+    const int units = (a.lines[b + 1] - a.lines[b]) / (a.kv_heads * tiles), from = a.lines[b] + (tile * a.kv_heads + h) * units, to = from + units - 1;
+    if (units == 0) {                                  // no keys: nobody has written it
+      if (side == 0) store_out<T, D>(a, b, h, r, c, make_float4(0.f, 0.f, 0.f, 0.f));
+      return;
+    }
+    const long long n = a.splits;                      // blocks
+    const int c0 = static_cast<int>(((from + 1ll) * n - 1) / all), c1 = static_cast<int>(((to + 1ll) * n - 1) / all);
+    if (c0 == c1) return;                              // one block had it whole
+    parts = c1 - c0 + 1;
+    begins = true;
+    first = 2ll * c0 * a.tile_rows + r - tile * a.tile_rows;
+    stride = 2ll * a.tile_rows;
+  }
+  auto place = [&](int s) { return first + s * stride + (begins && s == 0 ? a.tile_rows : 0); };
+  // each side over its parts, eight under way at once, against the largest weight of the eights so far
+  constexpr int AHEAD = 8;
   float top = -INFINITY, sum = 0.f;
-  for (int s = 0; s < parts; ++s) top = fmaxf(top, a.part_w[s * rows + at]);
-  const float ref = top == -INFINITY ? 0.f : top;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int s = side; s < parts; s += SIDES) {
-    const float f = ex2(a.part_w[s * rows + at] - ref);
-    const float4 y = reinterpret_cast<const float4*>(a.part_o)[(s * rows + at) * C + c];
-    sum += f;
-    x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+  for (int s0 = side; s0 < parts; s0 += SIDES * AHEAD) {
+    float w[AHEAD];
+    float4 y[AHEAD];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int s = s0 + k * SIDES;
+      w[k] = -INFINITY, y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (s < parts) w[k] = a.part_w[place(s)], y[k] = reinterpret_cast<const float4*>(a.part_o)[place(s) * C + c];
+    }
+    float now = top;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) now = fmaxf(now, w[k]);
+    const float ref = now == -INFINITY ? 0.f : now, f = ex2(top - ref);
+    top = now;
+    sum *= f, x.x *= f, x.y *= f, x.z *= f, x.w *= f;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const float e = ex2(w[k] - ref);
+      sum += e;
+      x.x = fmaf(e, y[k].x, x.x), x.y = fmaf(e, y[k].y, x.y), x.z = fmaf(e, y[k].z, x.z), x.w = fmaf(e, y[k].w, x.w);
+    }
   }
   other[side][c] = x;
-  if (c == 0) others[side] = sum;
+  if (c == 0) others[side] = sum, tops[side] = top;
   __syncthreads();
   if (side > 0) return;
 #pragma unroll
-  for (int s = 1; s < SIDES; ++s) {
+  for (int s = 0; s < SIDES; ++s) top = fmaxf(top, tops[s]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  x = make_float4(0.f, 0.f, 0.f, 0.f), sum = 0.f;
+#pragma unroll
+  for (int s = 0; s < SIDES; ++s) {
     const float4 y = other[s][c];
-    sum += others[s];
-    x.x += y.x, x.y += y.y, x.z += y.z, x.w += y.w;
+    const float f = ex2(tops[s] - ref);
+    sum = fmaf(f, others[s], sum);
+    x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
   }
   const float inverse = sum == 0.f ? 0.f : 1.f / sum;
   x.x *= inverse, x.y *= inverse, x.z *= inverse, x.w *= inverse;
-  const int r = static_cast<int>(at % (a.fresh * group)), h = static_cast<int>(at / (a.fresh * group) % a.kv_heads),
-            b = static_cast<int>(at / (a.fresh * group) / a.kv_heads);
   store_out<T, D>(a, b, h, r, c, x);
 }
 
@@ -442,83 +550,86 @@ __global__ void __launch_bounds__(64) attend_join_kernel(const AttendArgs a) {
 constexpr int MANY = 32;
 static bool many(int rows, int fp32) { return !fp32 && rows > MANY; }
 
-// Ranges of keys for each (sequence, head, tile of rows), by sizes alone. A cluster of up to 8 blocks joins its ranges in distributed shared memory; more
-// go through memory and a second kernel.
+// How a call is cut, by its sizes alone.
+struct Cut {
+  Share share;
+  int splits;                    // ranges of keys (tiles of 128 rows, CLUSTER), blocks (FLAT)
+  int rows;                      // of a tile
+  long long scratch;             // floats
+};
 static int few_rows(int rows) { return rows <= 8 ? 8 : 16; }
-static int splits_for(int batch, int rows, int kv_heads, long long room, int fp32) {
-  const int tile = many(rows, fp32) ? 128 : few_rows(rows);
-  const long long units = (long long)batch * kv_heads * ((rows + tile - 1) / tile);
+static Cut cut(int batch, int rows, int heads_rows, int kv_heads, int head_dim, long long room, int fp32) {
+  Cut c = {ONE, 1, many(rows, fp32) ? 128 : few_rows(rows), 0};
+  const long long units = (long long)batch * kv_heads * ((rows + c.rows - 1) / c.rows);
   if (many(rows, fp32)) {
     const long long most = (room + 511) / 512, want = 148 / units;           // four tiles of keys at least
-    return static_cast<int>(want < 2 || most < 2 ? 1 : want < most ? want : most);
+    c.splits = static_cast<int>(want < 2 || most < 2 ? 1 : want < most ? want : most);
+    if (c.splits > 1) c.scratch = (long long)c.splits * heads_rows * (head_dim + 1);
+    return c;
   }
-  const long long most = (room + FEW_WARPS * STEP - 1) / (FEW_WARPS * STEP);           // a step for each warp at least
-  long long want = (296 + units - 1) / units;
-  if (want <= 8) want = 8;
-  if (units * want > 4 * 296) want = 4;
-  if (units * want > 4 * 296) want = 2;
-  if (units * want > 4 * 296) want = 1;
-  if (want > most) want = most;
-  want = want >= 8 ? want / 8 * 8 : want >= 4 ? 4 : want >= 2 ? 2 : 1;
-  return static_cast<int>(want > 128 ? 128 : want);
+  const long long most = (room + UNIT - 1) / UNIT;
+  if (most < 2) return c;                                                    // a step for each warp
+  if (units * 8 <= 296 && room <= 8192) {
+    c.share = CLUSTER;
+    c.splits = room >= 512 ? 8 : room >= 256 ? 4 : 2;
+  } else if (rows <= 32 && batch <= FLAT_BATCH && units * most < (1ll << 31)) {
+    c.share = FLAT;
+    const long long blocks = 148 * (c.rows == 8 ? 3 : 2);
+    c.splits = static_cast<int>(blocks < units * most ? blocks : units * most);
+    c.scratch = 2ll * c.splits * c.rows * (head_dim + 1) + batch + 1;
+  }
+  return c;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool LINES>
 static cudaError_t join(const AttendArgs& a, cudaStream_t stream) {
-  if (a.splits == a.cluster) return cudaSuccess;
-  return launch_following(attend_join_kernel<T, D>, dim3(static_cast<unsigned>((long long)a.batch * a.fresh * a.heads)), dim3(64), 0, stream, a);
+  return launch_following(attend_join_kernel<T, D, LINES>, dim3(static_cast<unsigned>((long long)a.batch * a.fresh * a.heads)), dim3(JOIN_THREADS), 0, stream, a);
 }
 
 template <typename T, int D, int RT>
-static cudaError_t launch_few(const AttendArgs& a, cudaStream_t stream) {
-  const bool cluster = a.cluster > 1;
-  const auto kernel = cluster ? attend_few_kernel<T, D, RT, true> : attend_few_kernel<T, D, RT, false>;
-  const long long grid = (long long)a.splits * a.kv_heads * a.batch * ((a.fresh * (a.heads / a.kv_heads) + 8 * RT - 1) / (8 * RT));
+static cudaError_t launch_few(const AttendArgs& a, const Cut& c, cudaStream_t stream) {
+  const auto kernel = c.share == CLUSTER ? attend_few_kernel<T, D, RT, CLUSTER> : c.share == FLAT ? attend_few_kernel<T, D, RT, FLAT> : attend_few_kernel<T, D, RT, ONE>;
+  const long long grid = c.share == FLAT ? c.splits : (long long)c.splits * a.kv_heads * a.batch * ((a.fresh * (a.heads / a.kv_heads) + 8 * RT - 1) / (8 * RT));
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  static_assert(Few<D, RT>::SMEM <= 48 * 1024, "no more than a kernel has without asking");
-  cudaError_t e;
+  static_assert(Few<D, RT>::SMEM + (FLAT_BATCH + 1) * 4 <= 48 * 1024, "no more than a kernel has without asking");
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(32 * FEW_WARPS);
-  cfg.dynamicSmemBytes = Few<D, RT>::SMEM;
+  cfg.dynamicSmemBytes = Few<D, RT>::SMEM + (c.share == FLAT ? (a.batch + 1) * 4 : 0);
   cfg.stream = stream;
   cfg.attrs = attr;
-  if (cluster) {
+  if (c.share == CLUSTER) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(a.cluster);
+    attr[0].val.clusterDim.x = static_cast<unsigned>(c.splits);
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.numAttrs = 1;
   }
   nb::set_following(cfg);
-  e = cudaLaunchKernelEx(&cfg, kernel, a);
-  return e != cudaSuccess ? e : join<T, D>(a, stream);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  return e != cudaSuccess || c.share != FLAT ? e : join<T, D, true>(a, stream);
 }
 
 template <typename T, int D>
-static cudaError_t launch_attend(const AttendArgs& a, int* status, cudaStream_t stream) {
-  const int rows = a.fresh * (a.heads / a.kv_heads);
-  if (many(rows, sizeof(T) == 4)) {
-    if (a.cluster != 1) return cudaErrorInvalidValue;       // its ranges are not joined in clusters
+static cudaError_t launch_attend(const AttendArgs& a, const Cut& c, int* status, cudaStream_t stream) {
+  if (c.rows == 128) {
     const cudaError_t e = launch_many<D>(a, status, stream);
-    return e != cudaSuccess ? e : join<T, D>(a, stream);
+    return e != cudaSuccess || c.splits == 1 ? e : join<T, D, false>(a, stream);
   }
-  return few_rows(rows) == 8 ? launch_few<T, D, 1>(a, stream) : launch_few<T, D, 2>(a, stream);
+  return c.rows == 8 ? launch_few<T, D, 1>(a, c, stream) : launch_few<T, D, 2>(a, c, stream);
 }
 
 }  // namespace nbc
 
-// Ranges of keys that nb_cached_attention is to be called with for these sizes (positive), and blocks of a cluster that join theirs (in bits 16 and up). Where
-// the two differ it needs scratch: ranges / cluster * batch * new * heads * (head_dim + 1) floats.
-extern "C" int nb_cached_attention_splits(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int columns, int fp32) {
-  const int rows = fresh * (heads / kv_heads), s = nbc::splits_for(batch, rows, kv_heads, (long long)columns * block, fp32);
-  return s | (nbc::many(rows, fp32) ? 1 : s < 8 ? s : 8) << 16;
+// Scratch of a call with these sizes, in floats.
+extern "C" long long nb_cached_attention_scratch(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int columns, int fp32) {
+  return nbc::cut(batch, fresh * (heads / kv_heads), batch * fresh * heads, kv_heads, head_dim, (long long)columns * block, fp32).scratch;
 }
 
 extern "C" int nb_cached_attention(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, void* out,
                                    const void* table, const void* past, const void* count, int wide, int batch, int fresh, int heads, int kv_heads,
                                    int head_dim, int block, int blocks, int columns, long long q_sb, long long q_st, long long q_sh, float scale,
-                                   int causal, int splits, float* scratch, int fp32, int* status, void* stream) {
+                                   int causal, float* scratch, int fp32, int* status, void* stream) {
   using namespace nbc;
   AttendArgs a = {};
   a.q = q, a.q_sb = q_sb, a.q_st = q_st, a.q_sh = q_sh;
@@ -531,13 +642,19 @@ extern "C" int nb_cached_attention(const void* q, const void* k_codes, const voi
   a.batch = batch, a.fresh = fresh, a.heads = heads, a.kv_heads = kv_heads, a.causal = causal;
   a.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : -1;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.splits = splits & 0xffff, a.cluster = splits >> 16;
-  if (a.cluster < 1 || a.cluster > 8 || a.splits < a.cluster || a.splits % a.cluster != 0 || (a.splits > a.cluster && scratch == nullptr)) return -1;
-  a.part_o = scratch, a.part_w = scratch + (long long)(a.splits / a.cluster) * batch * fresh * heads * head_dim;
   if (a.block_log < 0 || (head_dim != 64 && head_dim != 128)) return -1;
+  const Cut c = cut(batch, fresh * (heads / kv_heads), batch * fresh * heads, kv_heads, head_dim, (long long)columns * block, fp32);
+  if (c.scratch > 0 && scratch == nullptr) return -1;
+  a.splits = c.splits, a.tile_rows = c.rows;
+  a.part_o = scratch;
+  a.part_w = scratch + c.scratch / (head_dim + 1) * head_dim;
+  if (c.share == FLAT) {
+    a.part_w = scratch + 2ll * c.splits * c.rows * head_dim;
+    a.lines = reinterpret_cast<int*>(a.part_w + 2ll * c.splits * c.rows);
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (fp32) return head_dim == 64 ? launch_attend<float, 64>(a, status, s) : launch_attend<float, 128>(a, status, s);
-  return head_dim == 64 ? launch_attend<__nv_bfloat16, 64>(a, status, s) : launch_attend<__nv_bfloat16, 128>(a, status, s);
+  if (fp32) return head_dim == 64 ? launch_attend<float, 64>(a, c, status, s) : launch_attend<float, 128>(a, c, status, s);
+  return head_dim == 64 ? launch_attend<__nv_bfloat16, 64>(a, c, status, s) : launch_attend<__nv_bfloat16, 128>(a, c, status, s);
 }
 
 NB_DEBUG_DEFINE(cached_attention)

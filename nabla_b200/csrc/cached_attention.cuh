@@ -14,9 +14,11 @@ struct AttendArgs {
   void* out;                     // [batch][new][heads][D], dense
   int batch, fresh, heads, kv_heads, block_log, causal;
   float scale_log2;              // softmax scale * log2(e)
-  int splits, cluster;           // ranges of keys, one block each; blocks of a cluster, which join theirs
-  float *part_o, *part_w;        // where there are several clusters: [splits / cluster][batch][kv_heads][new * group] output over their ranges, and
-                                 // log2 of the sum of its weights
+  int splits;                    // ranges of keys, one block each; or blocks that share all keys
+  int tile_rows;
+  // fp32 results of parts, and log2 of the sum of their weights: [splits][batch][kv_heads][new * group] rows, or two tiles of rows for each block
+  float *part_o, *part_w;
+  int* lines;                    // see attend_few_kernel
 };
 
 // Four neighbouring numbers of row r (token r / group, head r % group) of cache head h.

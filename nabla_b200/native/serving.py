@@ -24,14 +24,15 @@ def _L():
         sig = {
             "nb_kv_write": [c_vp] * 9 + [c_int] * 8 + [c_ll] * 6 + [c_int, c_vp],
             "nb_kv_read": [c_vp] * 9 + [c_int] * 9 + [c_vp],
-            "nb_cached_attention": [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_int, c_vp, c_int, c_vp, c_vp],
-            "nb_cached_attention_splits": [c_int] * 8,
+            "nb_cached_attention": [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_vp, c_int, c_vp, c_vp],
             "nb_adjust_logits": [c_vp] * 9 + [c_ll, c_vp] + [c_int] * 6 + [c_vp],
         }
         for name, args in sig.items():
             fn = getattr(lib, name)
             fn.argtypes = args
             fn.restype = c_int
+        lib.nb_cached_attention_scratch.argtypes = [c_int] * 8
+        lib.nb_cached_attention_scratch.restype = c_ll
         _lib = lib
     r = recorder()
     return _lib if r is None else r.library(_lib)
@@ -92,20 +93,18 @@ def cached_attention(q, k_codes, k_scale, v_codes, v_scale, table, past, count, 
     blocks, h, n, _ = k_codes.shape
     out = torch.empty((b, t, hq, d), dtype=q.dtype, device=q.device)
     fp32 = int(q.dtype == torch.float32)
-    splits = _splits(b, t, hq, h, d, n, table.shape[1], fp32)
-    # fp32 results of ranges of keys: outputs and the logarithms of their weights; those of one cluster of blocks need none
-    parts = (splits & 0xffff) // (splits >> 16)
-    part = torch.empty(parts * b * t * hq * (d + 1), dtype=torch.float32, device=q.device) if parts > 1 else None
+    floats = _scratch(b, t, hq, h, d, n, table.shape[1], fp32)      # of parts that a second kernel joins
+    part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     _ok(_L().nb_cached_attention(ptr(q), ptr(k_codes), ptr(k_scale), ptr(v_codes), ptr(v_scale), ptr(out), ptr(table), ptr(past), ptr(count),
                                  _wide(table, past, count), b, t, hq, h, d, n, blocks, table.shape[1], *q.stride()[:3], float(scale), int(causal),
-                                 splits, ptr(part), fp32, ptr(status_word(q.device)), stream_ptr()), "cached_attention", 2 if parts > 1 else 1)
+                                 ptr(part), fp32, ptr(status_word(q.device)), stream_ptr()), "cached_attention", 2 if floats else 1)
     return out
 
 
 @functools.lru_cache(1024)
-def _splits(*sizes: int) -> int:
+def _scratch(*sizes: int) -> int:
     """A function of the sizes alone."""
-    return _L().nb_cached_attention_splits(*sizes)
+    return _L().nb_cached_attention_scratch(*sizes)
 
 
 def adjust_logits(logits, history, length, prompt, repetition, presence, frequency, bias, allowed):

@@ -28,7 +28,7 @@ LAUNCHES = frozenset("""nb_gemm_bf16 nb_gemm_dual_bf16 nb_attn_fwd nb_attn_bwd n
     nb_adjust_logits""".split())
 # functions of sizes alone
 QUERIES = frozenset("""nb_layernorm_bwd_nblocks nb_colsum_nparts nb_conv2d_wgrad_slices nb_sgemm_slices nb_reduce_splits
-    nb_embedding_scatter_work nb_cached_attention_splits""".split())
+    nb_embedding_scatter_work nb_cached_attention_scratch""".split())
 # switches that the wrappers read on every call
 ENVIRONMENT = ("NABLA_B200_DISABLE_NATIVE", "NABLA_B200_ATTENTION", "NABLA_B200_ATTENTION_BWD", "NABLA_B200_ELEMENTWISE", "NABLA_B200_LN_BWD",
                "NABLA_B200_OPTIMIZER_STREAM", "NABLA_B200_TAPE")
