@@ -124,48 +124,38 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   const int k0 = min(keys, SHARE == FLAT ? unit0 * UNIT : sp * per), k1 = min(keys, k0 + per);
   const int steps = (k1 - k0 + STEP - 1) / STEP, mine = (steps - warp + FEW_WARPS - 1) / FEW_WARPS;
   const int all_see = a.causal ? min(keys - 1, past + row0 / group) : keys - 1;     // keys up to here are seen by every row
-  const int n = 1 << a.block_log;
+  const int n = 1 << a.block_log, last_key = max(k1 - 1, 0);
 
   // ---- where a step's codes lie
-  struct Place { int id[2]; };
+  // (of no block: the cache's first, so that loads need no condition: behind one they would be waited for where the paths meet. The step
+  // behind the last is the last again.)
+  struct Place { int id[2], there; };
   auto find = [&](int step) {
-    Place p = {{-1, -1}};
-    const int at = k0 + (step * FEW_WARPS + warp) * STEP;
-    if (step < mine) {
-      p.id[0] = a.table.block(b, at >> a.block_log);
-      if (at + 16 < k1) p.id[1] = n == 16 ? a.table.block(b, (at + 16) >> a.block_log) : p.id[0];
-    }
+    const int at = k0 + (max(min(step, mine - 1), 0) * FEW_WARPS + warp) * STEP;
+    const int x = a.table.block(b, min(at, last_key) >> a.block_log), y = n == 16 ? a.table.block(b, min(at + 16, last_key) >> a.block_log) : x;
+    const Place p = {{max(x, 0), max(y, 0)}, (x >= 0 ? 1 : 0) | (y >= 0 && at + 16 < k1 ? 2 : 0)};
     return p;
   };
   auto unit = [&](const Place& p, int i) { return (long long)p.id[i] * a.kv_heads + h; };
   auto from = [&](const Place& p, int i, int step) {
-    return ((unit(p, i) << a.block_log) + ((k0 + (step * FEW_WARPS + warp) * STEP + 16 * i) & (n - 1))) * D;
+    return ((unit(p, i) << a.block_log) + ((k0 + (max(min(step, mine - 1), 0) * FEW_WARPS + warp) * STEP + 16 * i) & (n - 1))) * D;
   };
   uint4 kr[2][2][PIECES], vr[2][4];                   // [16 keys each][keys g and g + 8], [keys 2t, 2t + 1, 2t + 8, 2t + 9]
   float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-#pragma unroll
-    for (int p = 0; p < 2 * PIECES; ++p) kr[i][p / PIECES][p % PIECES] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) vr[i][r] = make_uint4(0, 0, 0, 0);
-  }
   auto get_keys = [&](const Place& p, int step) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (p.id[i] >= 0) {
+    for (int i = 0; i < 2; ++i) {
         const int8_t* at = a.codes[0] + from(p, i, step) + g * D + t * 16;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int c = 0; c < PIECES; ++c) kr[i][u][c] = ldg16(at + u * 8 * D + c * 64);
-        ks[i] = a.scales[0][unit(p, i)];
+        ks[i] = scale_at(a.scales[0], unit(p, i));
       }
   };
   auto get_values = [&](const Place& p, int step) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (p.id[i] >= 0) {
+    for (int i = 0; i < 2; ++i) {
         const int8_t* at = a.codes[1] + from(p, i, step) + 2 * t * D + g * (D / 8);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -184,7 +174,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   get_values(now, 0);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    if (now.id[i] >= 0) vs[i] = a.scales[1][unit(now, i)];
+    vs[i] = scale_at(a.scales[1], unit(now, i));
   Place next = find(1);
 
   // ---- queries as the small operand: lane (g, t) holds dims 16 (t + 4 p) + 4 s + {0, 1} and {2, 3} of row g for k-step 4 p + s
@@ -278,7 +268,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
     bool grow = false, small = false;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const bool is = now.id[i] >= 0;
+      const bool is = now.there >> i & 1;
       const float sv = vs[i] < LEAST_SCALE ? LEAST_SCALE : vs[i];
       lg[i] = __log2f(sv);
       per_value[i] = __fdividef(1.f, sv);
@@ -379,7 +369,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
     get_values(next, step + 1);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      if (next.id[i] >= 0) vs[i] = a.scales[1][unit(next, i)];
+      vs[i] = scale_at(a.scales[1], unit(next, i));
     now = next;
     next = find(step + 2);
   }
