@@ -28,12 +28,17 @@ struct WriteArgs {
 __device__ __forceinline__ float scale_for(uint32_t top) {      // bits of the largest magnitude; those of infinities and NaN are the largest
   return top < 0x7f800000u ? fmaxf(__uint_as_float(top) * (1.0f / 127.0f), LEAST_SCALE) : __int_as_float(0x7fc00000);
 }
+// x * y, rounded, and z added to that, rounded again. Not by the two-wide functions: their pair was made one operation with one rounding here, and codes
+// halfway between two differed from what the definition's two operations give.
+__device__ __forceinline__ float2 multiply_then_add(float2 x, float2 y, float2 z) {
+  return make_float2(__fadd_rn(__fmul_rn(x.x, y.x), z.x), __fadd_rn(__fmul_rn(x.y, y.y), z.y));
+}
 // Codes of four numbers. The product with 1 / scale is at most 127.00002 in magnitude; with 1.5 * 2^23 added its nearest whole number stands in
 // the low byte.
 __device__ __forceinline__ uint32_t codes4(float2 a, float2 b, float2 inverse) {
   const float2 magic = make_float2(12582912.f, 12582912.f);
-  a = __fadd2_rn(__fmul2_rn(a, inverse), magic);
-  b = __fadd2_rn(__fmul2_rn(b, inverse), magic);
+  a = multiply_then_add(a, inverse, magic);
+  b = multiply_then_add(b, inverse, magic);
   return __byte_perm(__byte_perm(__float_as_uint(a.x), __float_as_uint(a.y), 0x0040), __byte_perm(__float_as_uint(b.x), __float_as_uint(b.y), 0x0040),
                      0x5410);
 }

@@ -327,6 +327,22 @@ def check_written(cache, before, want, name):
     assert torch.equal(cache[name][others], before[name][others])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_codes_are_those_of_the_definition_bit_for_bit(dtype):
+    """1 / scale rounded, the product rounded, the nearest whole number: quotients halfway between two are many in bf16, and kernels and torch agree."""
+    g = gen("cuda", 19)
+    b, t, h, d, n = 4, 300, 4, 128, 64
+    cache = new_cache(g, "cuda", b * 8, h, n, d)
+    table = new_table(g, "cuda", b, 8, b * 8)
+    past, count = torch.tensor([0, 10, 63, 130], device="cuda", dtype=torch.int32), torch.tensor([300, 299, 0, 64], device="cuda", dtype=torch.int32)
+    k, v = ((torch.randn((b, t, h, d), generator=g, device="cuda") * 3).to(dtype) for _ in range(2))
+    host = F.kv_cache_write({name: T(x.cpu()) for name, x in cache.items()}, T(k.cpu()), T(v.cpu()), T(table.cpu()), T(past.cpu()), T(count.cpu()))
+    F.kv_cache_write(wrap(cache), T(k), T(v), T(table), T(past), T(count))
+    for name in cache:
+        assert torch.equal(cache[name].cpu(), host[name].to_torch())
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_writing_what_is_not_finite_or_zero_and_writing_past_the_end(device):
     h, d, n = 2, 64, 16
