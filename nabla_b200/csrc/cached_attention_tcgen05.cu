@@ -1,10 +1,10 @@
 // Attention over a key / value cache in 8 bits for many rows (the operation and its terms: cached_attention.cu, cached_attention.cuh).
 //
 // A block of threads takes two tiles of 128 rows (tokens times the heads of a group, so that all heads that share a cache head share its
-// codes) and walks over tiles of 128 keys. 13 warps:
-//   warps 0-3   make 16-bit floats of codes: 16 bytes at a time from global memory, a tile ahead in registers, into the swizzled operand tiles
+// codes) and walks over tiles of 128 keys. 12 warps:
+//   warps 0-2   make 16-bit floats of codes: 16 bytes at a time from global memory, a tile ahead in registers, into the swizzled operand tiles
 //   warps 4-11  two groups of 128 threads, one per row tile, thread r owns row r (lane r of tensor memory): queries, softmax, output
-//   warp 12     allocates tensor memory and issues the products (one elected thread)
+//   warp 3      allocates tensor memory and issues the products (one elected thread)
 // Scores S (fp32) of row tile t are in columns t * 128 ..., the weights (16-bit floats, two in a column) take the place of the scores just read and
 // feed the second product from there, the outputs are in columns 256 + t * D.
 //
@@ -18,7 +18,7 @@
 namespace nbc {
 using namespace nb;
 
-constexpr int BT = 128, MANY_THREADS = 416, CONVERT = 128, GROUPS = BT / 16;
+constexpr int BT = 128, MANY_THREADS = 384, CONVERT = 96, ISSUER = 3, GROUPS = BT / 16;
 
 struct ManyArgs {
   AttendArgs a;
@@ -93,9 +93,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
   float* scales = reinterpret_cast<float*>(smem + L::SCALES);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BARS);
   uint64_t* q_full = bars + 0;     // [2] per row tile (128 arrivals)
-  uint64_t* k_full = bars + 2;     // [2] (128 arrivals)
+  uint64_t* k_full = bars + 2;     // [2] (96 arrivals)
   uint64_t* k_empty = bars + 4;    // [2]
-  uint64_t* v_full = bars + 6;     // [2] (128 arrivals)
+  uint64_t* v_full = bars + 6;     // [2] (96 arrivals)
   uint64_t* v_empty = bars + 8;    // [2]
   uint64_t* s_full = bars + 10;    // [2] per row tile: the scores of the next key tile are there, and the last product of weights has retired
   uint64_t* p_full = bars + 12;    // [2] per row tile: the weights are there (128 arrivals)
@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
     fence_mbar_init();
     fence_proxy_async_smem();
   }
-  if (warp == 12) {
+  if (warp == ISSUER) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -153,63 +153,46 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
   n_t[1] = min(max(n_t[1] - kt0, 0), per);
   const int n_max = max(n_t[0], n_t[1]);
 
-  if (warp < 4) {
-    // ---- codes: lane takes piece (lane & 3) + 4 u of key 32 i + 8 warp + lane / 4, so that 8 lanes write two keys' pieces to all banks
-    constexpr int PIECES = D / 64;
-    const int key = 8 * warp + (lane >> 2), c = lane & 3, n = 1 << a.block_log;
-    auto find = [&](int j, int (&id)[4]) {
+  if (warp < ISSUER) {
+    // ---- codes: a unit is 8 keys by 64 codes, lane takes piece (lane & 3) of key lane / 4, so that 8 lanes write two keys' pieces to all banks. The warps take
+    // units in turn
+    constexpr int PER_KEYS = D / 64, UNITS = BT / 8 * PER_KEYS, MINE = (UNITS + ISSUER - 1) / ISSUER;
+    const int key = lane >> 2, c = lane & 3, n = 1 << a.block_log;
+    // lane i < 8 knows where the i-th 16 keys of a tile lie (those of no block: the cache's first, so that loads need no condition: behind one they
+    // would be waited for where the paths meet)
+    struct Place { long long codes, unit; bool there; };
+    auto find = [&](int j) {
+      const int at = (kt0 + j) * BT + 16 * (lane & 7);
+      const int id = j < n_max && at < all_keys ? a.table.block(b, at >> a.block_log) : -1;
+      const long long unit = (long long)max(id, 0) * a.kv_heads + h;
+      return Place{((unit << a.block_log) + (at & (n - 1))) * D, unit, id >= 0};
+    };
+    auto get = [&](int which, const Place& place, uint4 (&x)[MINE]) {
+      const int8_t* codes = which ? a.codes[1] : a.codes[0];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int at = (kt0 + j) * BT + 32 * i + 16 * (warp >> 1);
-        id[i] = j < n_max && at < all_keys ? a.table.block(b, at >> a.block_log) : -1;
+      for (int i = 0; i < MINE; ++i) {
+        const int u = min(warp + i * ISSUER, UNITS - 1), k = u / PER_KEYS;
+        x[i] = ldg16(codes + __shfl_sync(0xffffffffu, place.codes, k >> 1) + ((k & 1) * 8 + key) * D + (u % PER_KEYS) * 64 + c * 16);
       }
     };
-    auto get = [&](int which, int j, const int (&id)[4], uint4 (&x)[4][PIECES]) {
+    auto put = [&](uint32_t tile, const uint4 (&x)[MINE], bool offset) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (id[i] < 0) continue;
-        const int at = (kt0 + j) * BT + 32 * i + key;
-        const int8_t* p = a.codes[which] + ((((long long)id[i] * a.kv_heads + h) << a.block_log) + (at & (n - 1))) * D + c * 16;
-#pragma unroll
-        for (int u = 0; u < PIECES; ++u) x[i][u] = ldg16(p + u * 64);
-      }
-    };
-    auto put = [&](uint32_t tile, const uint4 (&x)[4][PIECES], bool offset) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int u = 0; u < PIECES; ++u) {
-          uint4 lo, hi;
-          widen16(x[i][u], offset, lo, hi);
-          const uint32_t row = tile + u * (BT * 128) + (32 * i + key) * 128;
-          sts16(row + (((2 * c) ^ (key & 7)) << 4), lo);
-          sts16(row + (((2 * c + 1) ^ (key & 7)) << 4), hi);
+      for (int i = 0; i < MINE; ++i) {
+        const int u = warp + i * ISSUER, k = u / PER_KEYS;
+        uint4 lo, hi;
+        widen16(x[i], offset, lo, hi);
+        const uint32_t row = tile + (u % PER_KEYS) * (BT * 128) + (k * 8 + key) * 128;
+        if (u < UNITS) {
+          sts16(row + (((2 * c) ^ key) << 4), lo);
+          sts16(row + (((2 * c + 1) ^ key) << 4), hi);
         }
+      }
     };
-    uint4 kr[4][PIECES], vr[4][PIECES];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int u = 0; u < PIECES; ++u) kr[i][u] = vr[i][u] = make_uint4(0, 0, 0, 0);
-    // threads 0 to 7 bring the scales of 16 keys each
-    const int sg = threadIdx.x;
-    auto scale_block = [&](int j) {
-      const int at = (kt0 + j) * BT + 16 * sg;
-      return sg < GROUPS && j < n_max && at < all_keys ? a.table.block(b, at >> a.block_log) : -1;
-    };
-    auto get_scales = [&](int id, float& k, float& v) {
-      if (id < 0) return;
-      const long long unit = (long long)id * a.kv_heads + h;
-      k = a.scales[0][unit], v = a.scales[1][unit];
-    };
-    int id[4];
-    find(0, id);
-    get(0, 0, id, kr);
-    get(1, 0, id, vr);
-    find(1, id);
-    int sid = scale_block(0), sid_next = scale_block(1);
-    float sk = 0.f, sv = 0.f;
-    get_scales(sid, sk, sv);
+    uint4 kr[MINE], vr[MINE];
+    Place now = find(0), next = find(1);
+    get(0, now, kr);
+    get(1, now, vr);
+    float sk = scale_at(a.scales[0], now.unit), sv = scale_at(a.scales[1], now.unit);
     bool ok = true;
     for (int j = 0; j < n_max; ++j) {
       const int st = j & 1;
@@ -217,30 +200,29 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
       ok = mbar_wait(&k_empty[st], ph);
       if (!ok) break;
       put(smem_u32(smem + L::K + st * L::TILE), kr, true);
-      if (sg < GROUPS) {
+      if (threadIdx.x < GROUPS) {
         // (the softmax of the tile three ahead has let this one's place go)
-        float* s = scales + (j & 3) * 3 * GROUPS + sg;
+        float* s = scales + (j & 3) * 3 * GROUPS + threadIdx.x;
         const float v = sv < LEAST_SCALE ? LEAST_SCALE : sv;
-        s[0] = sid < 0 ? 1.f : sk < LEAST_SCALE ? LEAST_SCALE : sk;
-        s[GROUPS] = sid < 0 ? -INFINITY : __log2f(v);
-        s[2 * GROUPS] = sid < 0 ? 0.f : __fdividef(1.f, v);
+        s[0] = !now.there ? 1.f : sk < LEAST_SCALE ? LEAST_SCALE : sk;
+        s[GROUPS] = !now.there ? -INFINITY : __log2f(v);
+        s[2 * GROUPS] = !now.there ? 0.f : __fdividef(1.f, v);
       }
       fence_proxy_async_smem();
       mbar_arrive(&k_full[st]);
-      get(0, j + 1, id, kr);
+      get(0, next, kr);
       ok = mbar_wait(&v_empty[st], ph);
       if (!ok) break;
       put(smem_u32(smem + L::V + st * L::TILE), vr, false);
       fence_proxy_async_smem();
       mbar_arrive(&v_full[st]);
-      get(1, j + 1, id, vr);
-      find(j + 2, id);
-      sid = sid_next;
-      get_scales(sid, sk, sv);
-      sid_next = scale_block(j + 2);
+      get(1, next, vr);
+      sk = scale_at(a.scales[0], next.unit), sv = scale_at(a.scales[1], next.unit);
+      now = next;
+      next = find(j + 2);
     }
     if (!ok) atomicExch(args.status, NB_ERR_TIMEOUT_PRODUCER);
-  } else if (warp == 12) {
+  } else if (warp == ISSUER) {
     if (n_max > 0 && elect_one()) {
       const uint32_t q = smem_u32(smem + L::Q), k = smem_u32(smem + L::K), v = smem_u32(smem + L::V);
       bool ok = true;
@@ -349,7 +331,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
       }
       // pass 1: the maximum of each 16 scores, then with their scales. The next 32 columns are under way while these are worked on
       const float* sc = scales + (j & 3) * 3 * GROUPS;
-      float gt[GROUPS];                    // of 16 keys: the largest exponent
+      float gt[GROUPS], fs[GROUPS], adds[GROUPS];      // of 16 keys: the largest exponent; an exponent is a score times fs plus adds
       tmem_ld_32x32(t_s, va);
 #pragma unroll
       for (int c = 0; c < BT / 32; ++c) {
@@ -364,9 +346,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           for (int i = 2; i < 16; i += 4) x = top3(x, __uint_as_float(v[16 * k + i]), __uint_as_float(v[16 * k + i + 1]));
 #pragma unroll
           for (int i = 4; i < 16; i += 4) y = top3(y, __uint_as_float(v[16 * k + i]), __uint_as_float(v[16 * k + i + 1]));
-          float f = sc[2 * c + k] * row_mul;
-          f = f < 1e-37f ? 1e-37f : f;     // so that what is out of sight stays there
-          gt[2 * c + k] = fmaf(fmaxf(x, y), f, fmaf(-offset, f, sc[GROUPS + 2 * c + k]));
+          const float f = sc[2 * c + k] * row_mul;
+          fs[2 * c + k] = f < 1e-37f ? 1e-37f : f;     // so that what is out of sight stays there
+          adds[2 * c + k] = fmaf(-offset, fs[2 * c + k], sc[GROUPS + 2 * c + k]);
+          gt[2 * c + k] = fmaf(fmaxf(x, y), fs[2 * c + k], adds[2 * c + k]);
         }
       }
       const float mx = fmaxf(fmaxf(fmaxf(gt[0], gt[1]), fmaxf(gt[2], gt[3])), fmaxf(fmaxf(gt[4], gt[5]), fmaxf(gt[6], gt[7])));
@@ -426,11 +409,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int gi = 2 * c + k;
-          float f = sc[gi] * row_mul;
-          f = f < 1e-37f ? 1e-37f : f;
           // the exponent is rounded as that of the maximum was, and less that then: the largest weight is 1 however far the scores are from 0
-          const float lg = sc[GROUPS + gi], add = fmaf(-offset, f, lg);
-          const float2 f2 = make_float2(f, f), a2 = make_float2(add, add), b2 = make_float2(-base, -base);
+          const float2 f2 = make_float2(fs[gi], fs[gi]), a2 = make_float2(adds[gi], adds[gi]), b2 = make_float2(-base, -base);
           float2 acc = make_float2(0.f, 0.f);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
@@ -440,7 +420,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
             pk[8 * k + i] = pack_half2(p.x, p.y);
           }
           const float sum = acc.x + acc.y;
-          if (sum != 0.f && !(small >> gi & 1)) l = fmaf(sum, sc[2 * GROUPS + gi], l);       // a row that sees none of these keys does not see their scale either
+          l = fmaf(sum, sum != 0.f && !(small >> gi & 1) ? sc[2 * GROUPS + gi] : 0.f, l);      // a row that sees none of these keys does not see their scale either
         }
         st_tmem16(t_s + c * 16, pk);
       }
@@ -486,7 +466,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == ISSUER) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
