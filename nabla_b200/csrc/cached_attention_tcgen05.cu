@@ -398,6 +398,31 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           if (small >> k & 1) l += sum;
         }
       }
+      // Scores far from 0: an exponent is rounded as that of the maximum was, and less that then, so that the largest weight is 1 however far they are. It
+      // takes the score's place (rare). Near 0 the rounding of the sum of the two constants does not count (2^-15 at 512)
+      float far = fabsf(base);
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) far = fmaxf(far, adds[k] > -INFINITY ? fabsf(adds[k]) : 0.f);
+      if (__any_sync(0xffffffffu, !(far < 512.f))) {
+        tmem_ld_wait_regs(va);
+#pragma unroll
+        for (int c = 0; c < BT / 32; ++c) {
+          if (c > 0) {
+            tmem_ld_32x32(t_s + c * 32, va);
+            tmem_ld_wait_regs(va);
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) va[i] = __float_as_uint(fmaf(__uint_as_float(va[i]), fs[2 * c + i / 16], adds[2 * c + i / 16]) - base);
+          tmem_st_32x32(t_s + c * 32, va);
+        }
+        tmem_st_wait();
+        tmem_ld_32x32(t_s, va);
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) fs[k] = 1.f, adds[k] = 0.f;
+      } else {
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) adds[k] -= base;
+      }
       // pass 2: weights over the first 64 columns of the scores
 #pragma unroll
       for (int c = 0; c < BT / 32; ++c) {
@@ -406,20 +431,21 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
         tmem_ld_wait_regs(v);
         if (c + 1 < BT / 32) tmem_ld_32x32(t_s + (c + 1) * 32, nx);
         uint32_t pk[16];
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {    // two groups of 16 in turn
+            const int gi = 2 * c + k;
+            const float2 x = __ffma2_rn(two(v[16 * k + 2 * i], v[16 * k + 2 * i + 1]), make_float2(fs[gi], fs[gi]), make_float2(adds[gi], adds[gi]));
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            acc[k] = __fadd2_rn(acc[k], p);
+            pk[8 * k + i] = pack_half2(p.x, p.y);
+          }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const int gi = 2 * c + k;
-          // the exponent is rounded as that of the maximum was, and less that then: the largest weight is 1 however far the scores are from 0
-          const float2 f2 = make_float2(fs[gi], fs[gi]), a2 = make_float2(adds[gi], adds[gi]), b2 = make_float2(-base, -base);
-          float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float2 x = __fadd2_rn(__ffma2_rn(two(v[16 * k + 2 * i], v[16 * k + 2 * i + 1]), f2, a2), b2);
-            const float2 p = make_float2(ex2(x.x), ex2(x.y));
-            acc = __fadd2_rn(acc, p);
-            pk[8 * k + i] = pack_half2(p.x, p.y);
-          }
-          const float sum = acc.x + acc.y;
+          const float sum = acc[k].x + acc[k].y;
           l = fmaf(sum, sum != 0.f && !(small >> gi & 1) ? sc[2 * GROUPS + gi] : 0.f, l);      // a row that sees none of these keys does not see their scale either
         }
         st_tmem16(t_s + c * 16, pk);
