@@ -8,7 +8,7 @@
 // Scores S (fp32) of row tile t are in columns t * 128 ..., the weights (16-bit floats, two in a column) take the place of the scores just read and
 // feed the second product from there, the outputs are in columns 256 + t * D.
 //
-// Scales are one per 16 keys or more, so a row's 128 scores have 8 of them.
+// Scales are one per 16 keys or more, so a row's 128 scores have 8 of them: the maximum is taken over each 16 scores first, then with the scales.
 // Keys keep the offset of their codes (1152 each), and the product's part of it, 1152 times the sum of the query's numbers, is taken from the
 // scores; values do not, their offset would cancel against far smaller sums.
 #include "sm100_ptx.cuh"
@@ -82,24 +82,6 @@ __device__ __forceinline__ float top3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-
-// A row's outputs so far times root * root. The second product is not writing them: s_full also tracks the one before.
-template <int D>
-__device__ __noinline__ void scale_outputs(uint32_t t_o, float root) {
-#pragma unroll 1
-  for (int c = 0; c < D / 16; ++c) {
-    uint32_t o[16];
-    tmem_ld_32x16(t_o + c * 16, o);
-    tmem_ld_wait();
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      asm volatile("" : "+r"(o[i]));
-      o[i] = __float_as_uint(__uint_as_float(o[i]) * root * root);
-    }
-    st_tmem16(t_o + c * 16, o);
-  }
-  tmem_st_wait();
 }
 
 template <int D>
@@ -347,73 +329,101 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
         }
         tmem_st_wait();
       }
-      // an exponent is a score times fs plus adds, for each 16 keys
+      // pass 1: the maximum of each 16 scores, then with their scales. The next 32 columns are under way while these are worked on
       const float* sc = scales + (j & 3) * 3 * GROUPS;
-      float fs[GROUPS], adds[GROUPS];
+      float gt[GROUPS], fs[GROUPS], adds[GROUPS];      // of 16 keys: the largest exponent; an exponent is a score times fs plus adds
       tmem_ld_32x32(t_s, va);
-      float far = fabsf(m);                // of -inf too: there is no reference yet
 #pragma unroll
-      for (int k = 0; k < GROUPS; ++k) {
-        const float f = sc[k] * row_mul;
-        fs[k] = f < 1e-37f ? 1e-37f : f;   // so that what is out of sight stays there
-        const float x = -offset * fs[k];
-        far = fmaxf(far, fabsf(x));
-        adds[k] = sc[GROUPS + k] + (x - m);
+      for (int c = 0; c < BT / 32; ++c) {
+        uint32_t (&v)[32] = (c & 1) ? vb : va;
+        uint32_t (&nx)[32] = (c & 1) ? va : vb;
+        tmem_ld_wait_regs(v);
+        tmem_ld_32x32(t_s + ((c + 1) & 3) * 32, nx);       // after the last: the first again, for pass 2
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float x = __uint_as_float(v[16 * k]), y = __uint_as_float(v[16 * k + 1]);
+#pragma unroll
+          for (int i = 2; i < 16; i += 4) x = top3(x, __uint_as_float(v[16 * k + i]), __uint_as_float(v[16 * k + i + 1]));
+#pragma unroll
+          for (int i = 4; i < 16; i += 4) y = top3(y, __uint_as_float(v[16 * k + i]), __uint_as_float(v[16 * k + i + 1]));
+          const float f = sc[2 * c + k] * row_mul;
+          fs[2 * c + k] = f < 1e-37f ? 1e-37f : f;     // so that what is out of sight stays there
+          adds[2 * c + k] = fmaf(-offset, fs[2 * c + k], sc[GROUPS + 2 * c + k]);
+          gt[2 * c + k] = fmaf(fmaxf(x, y), fs[2 * c + k], adds[2 * c + k]);
+        }
       }
-      if (__any_sync(0xffffffffu, !(far < 512.f))) {
-        // The first tile, or scores far from 0 (rare): the maximum first. An exponent is rounded as that of the maximum was, and less that then, so that the
-        // largest weight is 1 however far they are. It takes the score's place
-        float mx = -INFINITY;
-        tmem_ld_wait_regs(va);
+      const float mx = fmaxf(fmaxf(fmaxf(gt[0], gt[1]), fmaxf(gt[2], gt[3])), fmaxf(fmaxf(gt[4], gt[5]), fmaxf(gt[6], gt[7])));
+      // the reference follows the maximum only when that has grown by 2^8: weights stay below 2^8
+      float half = 1.f;                    // the root of what the sums so far are multiplied by (the factor may fall out of the range of fp32)
+      bool grow = false;
+      if (m == -INFINITY) {
+        m = mx;                            // may stay: every key so far is hidden from this row
+      } else if (mx > m + 8.f) {
+        half = ex2(0.5f * (m - mx));
+        m = mx;
+        grow = true;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      if (__any_sync(0xffffffffu, grow)) {
+        // the output is not being written now: s_full also tracks the product of the weights before
+        l = l * half * half;
 #pragma unroll 1
-        for (int c = 0; c < BT / 16; ++c) {
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32(t_o + c * 32, o);
+          tmem_ld_wait_regs(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * half * half);
+          tmem_st_32x32(t_o + c * 32, o);
+        }
+      }
+      // weights that are lost in fp32 may count once their value's scale is taken out: exponentials of their own (rare)
+      uint32_t small = 0;
+#pragma unroll
+      for (int k = 0; k < GROUPS; ++k) small |= (gt[k] < base - 100.f && gt[k] > -INFINITY ? 1u : 0u) << k;
+      if (__any_sync(0xffffffffu, small != 0)) {
+#pragma unroll 1
+        for (int k = 0; k < GROUPS; ++k) {
           uint32_t x[16];
-          tmem_ld_32x16(t_s + 16 * c, x);
+          tmem_ld_32x16(t_s + 16 * k, x);
           tmem_ld_wait();
-          float f = sc[c] * row_mul;
+          float f = sc[k] * row_mul;
           f = f < 1e-37f ? 1e-37f : f;
-          const float add = fmaf(-offset, f, sc[GROUPS + c]);
+          float sum = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             asm volatile("" : "+r"(x[i]));
-            const float e = fmaf(__uint_as_float(x[i]), f, add);
-            mx = fmaxf(mx, e);
-            x[i] = __float_as_uint(e);
+            sum += ex2(fmaf(__uint_as_float(x[i]), f, fmaf(-offset, f, sc[GROUPS + k])) - base - sc[GROUPS + k]);
           }
-          st_tmem16(t_s + 16 * c, x);
+          if (small >> k & 1) l += sum;
         }
-        tmem_st_wait();
-        float root = 1.f;                  // of what the sums so far are multiplied by (the factor may fall out of the range of fp32)
-        bool grow = false;
-        if (m == -INFINITY) {
-          m = mx;                          // may stay: every key so far is hidden from this row
-        } else if (mx > m + 8.f) {
-          root = ex2(0.5f * (m - mx));
-          m = mx;
-          grow = true;
-        }
-        l = l * root * root;
-        if (__any_sync(0xffffffffu, grow)) scale_outputs<D>(t_o, root);
-        const float base = m == -INFINITY ? 0.f : m;
-#pragma unroll 1
-        for (int c = 0; c < BT / 16; ++c) {
-          uint32_t x[16];
-          tmem_ld_32x16(t_s + 16 * c, x);
-          tmem_ld_wait();
+      }
+      // Scores far from 0: an exponent is rounded as that of the maximum was, and less that then, so that the largest weight is 1 however far they are. It
+      // takes the score's place (rare). Near 0 the rounding of the sum of the two constants does not count (2^-15 at 512)
+      float far = fabsf(base);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            asm volatile("" : "+r"(x[i]));
-            x[i] = __float_as_uint(__uint_as_float(x[i]) - base);
+      for (int k = 0; k < GROUPS; ++k) far = fmaxf(far, adds[k] > -INFINITY ? fabsf(adds[k]) : 0.f);
+      if (__any_sync(0xffffffffu, !(far < 512.f))) {
+        tmem_ld_wait_regs(va);
+#pragma unroll
+        for (int c = 0; c < BT / 32; ++c) {
+          if (c > 0) {
+            tmem_ld_32x32(t_s + c * 32, va);
+            tmem_ld_wait_regs(va);
           }
-          st_tmem16(t_s + 16 * c, x);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) va[i] = __float_as_uint(fmaf(__uint_as_float(va[i]), fs[2 * c + i / 16], adds[2 * c + i / 16]) - base);
+          tmem_st_32x32(t_s + c * 32, va);
         }
         tmem_st_wait();
         tmem_ld_32x32(t_s, va);
 #pragma unroll
         for (int k = 0; k < GROUPS; ++k) fs[k] = 1.f, adds[k] = 0.f;
+      } else {
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k) adds[k] -= base;
       }
-      // Weights, over the first 64 columns of the scores, against the reference as it is: they stay below 2^14, or it is moved. So the maximum of a tile need
-      // not be known before its weights. The next 32 columns are under way while these are worked on
+      // pass 2: weights over the first 64 columns of the scores
 #pragma unroll
       for (int c = 0; c < BT / 32; ++c) {
         uint32_t (&v)[32] = (c & 1) ? vb : va;
@@ -421,62 +431,22 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
         tmem_ld_wait_regs(v);
         if (c + 1 < BT / 32) tmem_ld_32x32(t_s + (c + 1) * 32, nx);
         uint32_t pk[16];
-        float sum[2];
-        while (true) {
-          float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {  // two groups of 16 in turn
-              const int gi = 2 * c + k;
-              const float2 x = __ffma2_rn(two(v[16 * k + 2 * i], v[16 * k + 2 * i + 1]), make_float2(fs[gi], fs[gi]), make_float2(adds[gi], adds[gi]));
-              const float2 p = make_float2(ex2(x.x), ex2(x.y));
-              acc[k] = __fadd2_rn(acc[k], p);
-              pk[8 * k + i] = pack_half2(p.x, p.y);
-            }
-          sum[0] = acc[0].x + acc[0].y, sum[1] = acc[1].x + acc[1].y;
-          if (!__any_sync(0xffffffffu, fmaxf(sum[0], sum[1]) >= 16384.f)) break;
-          // the reference moves up by a whole number of powers of two, to this chunk's maximum (rare)
-          float mx = 0.f;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaf(__uint_as_float(v[i]), fs[2 * c + i / 16], adds[2 * c + i / 16]));
-          const float d = mx > 8.f ? ceilf(mx) : 0.f, root = ex2(-0.5f * d);
-          m += d;
-          l = l * root * root;
-#pragma unroll
-          for (int k = 0; k < GROUPS; ++k) adds[k] -= d;
-          scale_outputs<D>(t_o, root);
-          const uint32_t f2 = pack_half2(root * root, root * root);
-#pragma unroll 1
-          for (int e = 0; e < c; ++e) {    // weights of this tile that are there already
-            uint32_t x[16];
-            tmem_ld_32x16(t_s + 16 * e, x);
-            tmem_ld_wait();
-#pragma unroll
-            for (int i = 0; i < 16; ++i) asm volatile("mul.rn.f16x2 %0, %0, %1;" : "+r"(x[i]) : "r"(f2));
-            st_tmem16(t_s + 16 * e, x);
-          }
-        }
-        if (__any_sync(0xffffffffu, fminf(sum[0], sum[1]) < 1e-30f)) {
-          // weights that are lost in fp32 may count once their value's scale is taken out: exponentials of their own (hidden keys come here too)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
+          for (int k = 0; k < 2; ++k) {    // two groups of 16 in turn
             const int gi = 2 * c + k;
-            float more = 0.f;
-            if (sum[k] < 1e-30f) {
-#pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float x = fmaf(__uint_as_float(v[16 * k + i]), fs[gi], adds[gi]);
-                more += x == -INFINITY ? 0.f : ex2(x - sc[GROUPS + gi]);
-              }
-              l += more;
-            } else {
-              l = fmaf(sum[k], sc[2 * GROUPS + gi], l);
-            }
+            const float2 x = __ffma2_rn(two(v[16 * k + 2 * i], v[16 * k + 2 * i + 1]), make_float2(fs[gi], fs[gi]), make_float2(adds[gi], adds[gi]));
+            const float2 p = make_float2(ex2(x.x), ex2(x.y));
+            acc[k] = __fadd2_rn(acc[k], p);
+            pk[8 * k + i] = pack_half2(p.x, p.y);
           }
-        } else {
-          l = fmaf(sum[0], sc[2 * GROUPS + 2 * c], l);
-          l = fmaf(sum[1], sc[2 * GROUPS + 2 * c + 1], l);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int gi = 2 * c + k;
+          const float sum = acc[k].x + acc[k].y;
+          l = fmaf(sum, sum != 0.f && !(small >> gi & 1) ? sc[2 * GROUPS + gi] : 0.f, l);      // a row that sees none of these keys does not see their scale either
         }
         st_tmem16(t_s + c * 16, pk);
       }
