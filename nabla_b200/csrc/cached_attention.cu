@@ -31,6 +31,7 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
 // its 16 bytes of four values are rows of eight output tiles. Each of the four warps takes every fourth step of 32 keys and keeps its own
 // reference, sum and output until the end; keys of the next step are on their way from when this step's are used up, so are values.
 constexpr int FEW_WARPS = 4, STEP = 32;
+constexpr float ROOM = 7.f;      // see the weights
 // Four-float piece c of a row of outputs in shared memory: pieces are turned so that the 8 lanes that an access serves at once meet different banks
 // (lane (g, t) writes pieces g * D / 32 ... of rows 2t and 2t + 1).
 template <int D>
@@ -90,7 +91,9 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   if (SHARE == FLAT) {
     number_lines(a, tiles, lines);
     const int all = lines[a.batch];
-    line_from = static_cast<int>((long long)blockIdx.x * all / gridDim.x), line_to = static_cast<int>((long long)(blockIdx.x + 1) * all / gridDim.x);
+    // no more blocks than units, so that each has one: the joining kernel reads what every block between a line's first and last has written
+    const int blocks = min(static_cast<int>(gridDim.x), all), c = blockIdx.x;
+    if (c < blocks) line_from = static_cast<int>((long long)c * all / blocks), line_to = static_cast<int>((c + 1ll) * all / blocks);
     if (blockIdx.x == 0)
       for (int i = threadIdx.x; i <= a.batch; i += 32 * FEW_WARPS) a.lines[i] = lines[i];
   } else {
@@ -290,7 +293,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
           for (int e = 0; e < 4; ++e)
             if (key0 + 16 * i + 8 * (e >> 1) + g > lim[u][e & 1]) s[u][i][e] = -INFINITY;
     }
-    // the reference that weights are taken against follows the maximum only when that has grown by 2^8: weights stay below 2^8
+    // the reference that weights are taken against follows the maximum only when that has grown by 2^8. They are taken 2^7 larger, so that they stay
+    // below 2^15 and small ones, and the second parts of those of fp32 calls, keep their bits (16-bit floats have none below 2^-24)
 #pragma unroll
     for (int u = 0; u < RT; ++u)
 #pragma unroll
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
     const bool apart = __any_sync(0xffffffffu, small);
 #pragma unroll
     for (int u = 0; u < RT; ++u) {
-      const float base[2] = {m[u][0] == -INFINITY ? 0.f : m[u][0], m[u][1] == -INFINITY ? 0.f : m[u][1]};
+      const float base[2] = {m[u][0] == -INFINITY ? 0.f : m[u][0] - ROOM, m[u][1] == -INFINITY ? 0.f : m[u][1] - ROOM};
       if (apart) {                                    // weights that are lost in fp32 may count once their value's scale is taken out
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -388,7 +392,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
       for (int w = 4; w < 32; w <<= 1) l[u][r] += __shfl_xor_sync(0xffffffffu, l[u][r], w);
       const int row = 8 * u + 2 * t + r;
       if (g == 0) {
-        sm[warp * ROWS + row] = l[u][r] == 0.f ? -INFINITY : m[u][r] + __log2f(l[u][r]);
+        sm[warp * ROWS + row] = l[u][r] == 0.f ? -INFINITY : m[u][r] - ROOM + __log2f(l[u][r]);
         sl[warp * ROWS + row] = l[u][r] == 0.f ? 0.f : 1.f / l[u][r];
       }
       if (row < live)
@@ -481,7 +485,7 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const AttendA
       if (side == 0) store_out<T, D>(a, b, h, r, c, make_float4(0.f, 0.f, 0.f, 0.f));
       return;
     }
-    const long long n = a.splits;                      // blocks
+    const long long n = min(a.splits, all);            // blocks that have a share
     const int c0 = static_cast<int>(((from + 1ll) * n - 1) / all), c1 = static_cast<int>(((to + 1ll) * n - 1) / all);
     if (c0 == c1) return;                              // one block had it whole
     parts = c1 - c0 + 1;
@@ -548,13 +552,13 @@ struct Cut {
   long long scratch;             // floats
 };
 static int few_rows(int rows) { return rows <= 8 ? 8 : 16; }
-static Cut cut(int batch, int rows, int heads_rows, int kv_heads, int head_dim, long long room, int fp32) {
+static Cut cut(int batch, int rows, long long heads_rows, int kv_heads, int head_dim, long long room, int fp32) {
   Cut c = {ONE, 1, many(rows, fp32) ? 128 : few_rows(rows), 0};
   const long long units = (long long)batch * kv_heads * ((rows + c.rows - 1) / c.rows);
   if (many(rows, fp32)) {
     const long long most = (room + 511) / 512, want = 148 / units;           // four tiles of keys at least
     c.splits = static_cast<int>(want < 2 || most < 2 ? 1 : want < most ? want : most);
-    if (c.splits > 1) c.scratch = (long long)c.splits * heads_rows * (head_dim + 1);
+    if (c.splits > 1) c.scratch = c.splits * heads_rows * (head_dim + 1);
     return c;
   }
   const long long most = (room + UNIT - 1) / UNIT;
@@ -613,7 +617,7 @@ static cudaError_t launch_attend(const AttendArgs& a, const Cut& c, int* status,
 
 // Scratch of a call with these sizes, in floats.
 extern "C" long long nb_cached_attention_scratch(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int columns, int fp32) {
-  return nbc::cut(batch, fresh * (heads / kv_heads), batch * fresh * heads, kv_heads, head_dim, (long long)columns * block, fp32).scratch;
+  return nbc::cut(batch, fresh * (heads / kv_heads), (long long)batch * fresh * heads, kv_heads, head_dim, (long long)columns * block, fp32).scratch;
 }
 
 extern "C" int nb_cached_attention(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, void* out,
@@ -633,7 +637,7 @@ extern "C" int nb_cached_attention(const void* q, const void* k_codes, const voi
   a.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : -1;
   a.scale_log2 = scale * 1.4426950408889634f;
   if (a.block_log < 0 || (head_dim != 64 && head_dim != 128)) return -1;
-  const Cut c = cut(batch, fresh * (heads / kv_heads), batch * fresh * heads, kv_heads, head_dim, (long long)columns * block, fp32);
+  const Cut c = cut(batch, fresh * (heads / kv_heads), (long long)batch * fresh * heads, kv_heads, head_dim, (long long)columns * block, fp32);
   if (c.scratch > 0 && scratch == nullptr) return -1;
   a.splits = c.splits, a.tile_rows = c.rows;
   a.part_o = scratch;

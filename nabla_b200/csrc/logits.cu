@@ -7,6 +7,9 @@
 // Bound by memory: logits are read and written once, 8 at a time and asked for before the history is gone over. A row is cut into slices, one block of
 // threads each; the counts of a slice's tokens are in shared memory, and every block of a row goes over its whole history. Counts are sums of
 // whole numbers: their order does not matter.
+// 256 rows of 32001 in bf16 with histories of up to 2001, an odd row length, a bias and a grammar: 19.3 us; 5.6 without any of the three (6.1
+// TB/s), 9.5 with histories of one token (the counts' zeros and two barriers), 12.1 with the histories, 4.3 more for the bias, whose rows start off
+// boundaries. One row of 32000 with 300 tokens: 2.8 us. Blocks of 512 threads, 4096 tokens, and five or six resident blocks were slower (20 to 24 us).
 #include "kv_cache.cuh"
 
 namespace nbc {
@@ -53,7 +56,7 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
   for (int u = 0; u < PER; ++u) {
     const int v = token(u);
     raw[u].clear();
-    if (v >= 0 && v + 8 <= a.vocab) raw[u].load(in + v);
+    if (v >= 0 && v + 8 <= a.vocab && NB_IN_BOUNDS(NB_SITE_LOGITS_TOKEN, v + 7, a.vocab)) raw[u].load(in + v);
   }
   const bool counted = a.history.p != nullptr;
   if (counted) {

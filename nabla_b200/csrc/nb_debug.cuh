@@ -42,6 +42,9 @@ enum NbSite : int {
   NB_SITE_COMM_PEER_RANK = 18,   // peer collectives: peer rank vs world size
   NB_SITE_COMM_OFFSET = 19,      // peer collectives: element offset vs buffer length
   NB_SITE_COMM_FLAG = 20,        // peer collectives: flag slot vs flag pad
+  NB_SITE_CACHE_CODE = 21,       // key / value cache: code vs codes of the cache
+  NB_SITE_CACHE_ROW = 22,        // key / value cache: row of new, read or attended tokens vs their number
+  NB_SITE_LOGITS_TOKEN = 23,     // logits: token vs vocabulary
 };
 
 #ifdef NB_DEBUG_CHECKS

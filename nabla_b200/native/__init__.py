@@ -87,6 +87,7 @@ _DEBUG_SITES = {
     13: "fused GEMM + collective: peer rank", 14: "fused GEMM + collective: block offset",
     15: "attention: TMA tile coordinate", 16: "attention: row-statistics index", 17: "attention: output row",
     18: "peer collectives: rank / world size", 19: "peer collectives: element offset", 20: "peer collectives: flag slot",
+    21: "key / value cache: code", 22: "key / value cache: row of tokens", 23: "logits: token",
 }
 
 

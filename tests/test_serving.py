@@ -175,6 +175,33 @@ def test_attention_where_blocks_are_missing_and_scales_differ_widely(device, new
     check_attention(got, want, bound, cache)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("b,hq,h,columns,longest,dtype", [
+    (39, 16, 4, 11, 649, "bf16"),         # more units of keys than blocks share them, fewer, and far fewer than the table has room for
+    (3, 4, 1, 400, 11990, "bf16"), (3, 4, 1, 400, 300, "bf16"), (2, 8, 1, 4000, 129, "fp32"), (16, 32, 8, 40, 209, "bf16"), (5, 12, 2, 300, 9000, "fp32"),
+    (200, 8, 8, 8, 200, "bf16"), (1024, 4, 2, 4, 90, "bf16"), (1025, 4, 2, 4, 90, "bf16"), (7, 32, 2, 500, 4000, "bf16"),
+])
+def test_ragged_batches_share_the_chip(b, hq, h, columns, longest, dtype, d):
+    """Sequences of lengths from nothing to the longest, idle ones among them; scratch that holds garbage."""
+    g = gen("cuda", 41)
+    n, dtype = 64, torch.bfloat16 if dtype == "bf16" else torch.float32
+    blocks = -(-longest // n) * b + 1
+    cache = new_cache(g, "cuda", blocks, h, n, d)
+    table = torch.full((b, columns), -1, device="cuda", dtype=torch.int32)
+    used = -(-longest // n)
+    table[:, :used] = new_table(g, "cuda", b, used, blocks)
+    past = torch.randint(0, longest, (b,), generator=g, device="cuda", dtype=torch.int32)
+    past[0], past[-1] = longest - 1, 0
+    count = (torch.rand((b,), generator=g, device="cuda") < 0.7).to(torch.int32)
+    q = torch.randn((b, 1, hq, d), generator=g, device="cuda").to(dtype)
+    garbage = torch.full((64 << 20,), math.nan, device="cuda")       # what freed memory holds
+    del garbage
+    got = F.cached_attention(T(q), wrap(cache), T(table), T(past), T(count)).to_torch()
+    want, bound = attend64(q, cache, table, past.tolist(), count.tolist(), True, d ** -0.5)
+    check_attention(got, want, bound, cache)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("new", [1, 150])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
