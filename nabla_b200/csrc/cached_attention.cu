@@ -29,7 +29,14 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
 // there are 8 rows, and what is made of a code serves all rows. Fragments are read from global memory as the instruction wants them, whole
 // sectors at a time; a product's reduction may run in any order, so a lane's 16 bytes of a key are the four dims each of four k-steps, and
 // its 16 bytes of four values are rows of eight output tiles. Each of the four warps takes every fourth step of 32 keys and keeps its own
-// reference, sum and output until the end; keys of the next step are on their way from when this step's are used up, so are values.
+// reference, sum and output until the end; keys of the next step are on their way from when this step's are used up, so are values. No load
+// stands behind a condition: it would be waited for where the paths meet.
+//
+// What bounds it: latency, then instructions. 2 x 120001 tokens, 16 heads over 2 of 128: 29.6 us for 123 MB, 4.15 TB/s, 64 % of a plain copy's rate; some 800
+// instructions for 32 tokens, of which 320 make 16-bit floats of codes, at 12 warps an SM. 32 sequences of 200 to 4001, 16 heads over 4: 25 us
+// for 69 MB, of which 8 are starts, the joining kernel and the way from the table to the first code. One sequence of 700 with 16 heads: 6 us.
+// Slower were copies through shared memory (37 us for the first), and products of whole numbers with the weights in fixed point, which need no 16-bit floats
+// but the maximum first and then more registers (35 to 43 us).
 constexpr int FEW_WARPS = 4, STEP = 32;
 constexpr float ROOM = 7.f;      // see the weights
 // Four-float piece c of a row of outputs in shared memory: pieces are turned so that the 8 lanes that an access serves at once meet different banks
@@ -540,9 +547,11 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const AttendA
   store_out<T, D>(a, b, h, r, c, x);
 }
 
-// Above this many rows of a sequence and cache head, bf16 goes to tiles of 128 rows (cached_attention_tcgen05.cu).
-constexpr int MANY = 32;
-static bool many(int rows, int fp32) { return !fp32 && rows > MANY; }
+// bf16 calls of more than 32 rows of a sequence and cache head go to tiles of 128 rows (cached_attention_tcgen05.cu), up to 128 rows where they are more than
+// 32 tiles of 16 in all: for few tiles of 16 the pass over the codes of each is quicker than the longer start. us, tiles of 16 and of 128, 4 heads of 128: one
+// sequence of 1000 with 48, 64, 128 rows 9.0 and 18.5, 9.8 and 18.7, 11.2 and 20.0, of 8000 17.0 and 20.2, 19.9 and 20.7, 20.9 and 23.5; eight of 1000 and 8000
+// with 32 rows 22.5 and 22.1, 43.9 and 50.4, with 48 26.5 and 23.9, 57.7 and 52.5.
+static bool many(int rows, int fp32, long long pairs) { return !fp32 && rows > 32 && (rows > 128 || pairs * ((rows + 15) / 16) > 32); }
 
 // How a call is cut, by its sizes alone.
 struct Cut {
@@ -553,9 +562,10 @@ struct Cut {
 };
 static int few_rows(int rows) { return rows <= 8 ? 8 : 16; }
 static Cut cut(int batch, int rows, long long heads_rows, int kv_heads, int head_dim, long long room, int fp32) {
-  Cut c = {ONE, 1, many(rows, fp32) ? 128 : few_rows(rows), 0};
+  const bool wide = many(rows, fp32, (long long)batch * kv_heads);
+  Cut c = {ONE, 1, wide ? 128 : few_rows(rows), 0};
   const long long units = (long long)batch * kv_heads * ((rows + c.rows - 1) / c.rows);
-  if (many(rows, fp32)) {
+  if (wide) {
     const long long most = (room + 511) / 512, want = 148 / units;           // four tiles of keys at least
     c.splits = static_cast<int>(want < 2 || most < 2 ? 1 : want < most ? want : most);
     if (c.splits > 1) c.scratch = c.splits * heads_rows * (head_dim + 1);
@@ -563,10 +573,12 @@ static Cut cut(int batch, int rows, long long heads_rows, int kv_heads, int head
   }
   const long long most = (room + UNIT - 1) / UNIT;
   if (most < 2) return c;                                                    // a step for each warp
-  if (units * 8 <= 296 && room <= 8192) {
+  // us, a cluster of 8 and a line for 4 query heads to each of 1, 8, 16, 32, 64 pairs: 2000 tokens 7.0 and 8.1, 7.7 and 9.2, 8.4 and 9.8, 11.3 and 16.2, 21.2 and
+  // 20.7; 8000 tokens 12.7 and 8.9, 16.0 and 13.0, 18.4 and 18.0, 23.1 and 24.4, 42.5 and 34.1
+  if (units * 8 <= 296 && room <= 4096 + 256 * units) {
     c.share = CLUSTER;
     c.splits = room >= 512 ? 8 : room >= 256 ? 4 : 2;
-  } else if (rows <= 32 && batch <= FLAT_BATCH && units * most < (1ll << 31)) {
+  } else if (rows <= 128 && batch <= FLAT_BATCH && units * most < (1ll << 31)) {
     c.share = FLAT;
     const long long blocks = 148 * (c.rows == 8 ? 3 : 2);
     c.splits = static_cast<int>(blocks < units * most ? blocks : units * most);
