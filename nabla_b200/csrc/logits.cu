@@ -7,9 +7,10 @@
 // Bound by memory: logits are read and written once, 8 at a time and asked for before the history is gone over. A row is cut into slices, one block of
 // threads each; the counts of a slice's tokens are in shared memory, and every block of a row goes over its whole history. Counts are sums of
 // whole numbers: their order does not matter.
-// 256 rows of 32001 in bf16 with histories of up to 2001, an odd row length, a bias and a grammar: 19.3 us; 5.6 without any of the three (6.1
-// TB/s), 9.5 with histories of one token (the counts' zeros and two barriers), 12.1 with the histories, 4.3 more for the bias, whose rows start off
-// boundaries. One row of 32000 with 300 tokens: 2.8 us. Blocks of 512 threads, 4096 tokens, and five or six resident blocks were slower (20 to 24 us).
+// 256 rows of 32001 with histories of up to 2001, an odd row length, a bias and a grammar: 18.5 us in bf16, 21.6 in fp32; 13.9 and 17.5 without the bias, whose
+// rows start off boundaries, 10.9 and 14.7 without the histories, 5.6 in bf16 without any of the three (6.1 TB/s). One row of 32000 with 300 tokens: 2.8.
+// What bounds it are loads that wait for loads (10 of 17 stalled cycles) and going over the history for each slice. Blocks of 512 threads, and five or
+// six resident blocks were slower (20 to 24 us in bf16).
 #include "kv_cache.cuh"
 
 namespace nbc {
@@ -33,7 +34,7 @@ constexpr int THREADS = 256;
 
 // PER: groups of 8 tokens of a thread. A slice takes every 2^slice_log-th run of 32 groups: the tokens that stand in a history most often have ids close to
 // each other, and so fall to all slices alike.
-template <typename T, int PER>
+template <typename T, int PER, bool GRAMMAR>
 __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
   constexpr int SLICE = THREADS * PER * 8;
   extern __shared__ __align__(16) uint32_t times[];        // per token of the slice: how often in the prompt, how often behind it
@@ -58,6 +59,17 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
     raw[u].clear();
     if (v >= 0 && v + 8 <= a.vocab && NB_IN_BOUNDS(NB_SITE_LOGITS_TOKEN, v + 7, a.vocab)) raw[u].load(in + v);
   }
+  // the grammar's words are read ahead of the history; biases are not: registers for them cost blocks (21 to 23 us)
+  uint32_t bits[GRAMMAR ? PER : 1];
+  if (GRAMMAR)
+#pragma unroll
+    for (int u = 0; u < PER; ++u) {
+      const int v = token(u), w = v < 0 ? 0 : v >> 5;
+      const uint32_t* allowed = a.allowed + (long long)b * a.words;
+      uint32_t lo = 0u, hi = 0u;
+      if (v < a.vocab) lo = allowed[w], hi = allowed[w + 1 < a.words ? w + 1 : w];
+      bits[u] = v < 0 ? lo << -v : __funnelshift_r(lo, hi, v & 31);
+    }
   const bool counted = a.history.p != nullptr;
   if (counted) {
     constexpr int AHEAD = 8;               // ids under way at once; the first of them before it is known how many count
@@ -84,7 +96,6 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
   const float r = a.repetition == nullptr ? 1.f : a.repetition[b], over = 1.f / r, presence = a.presence == nullptr ? 0.f : a.presence[b],
               frequency = a.frequency == nullptr ? 0.f : a.frequency[b];
   const float* bias = a.bias == nullptr ? nullptr : a.bias + b * a.bias_sb;
-  const uint32_t* allowed = a.allowed == nullptr ? nullptr : a.allowed + (long long)b * a.words;
 #pragma unroll
   for (int u = 0; u < PER; ++u) {
     const int at = (u * THREADS + threadIdx.x) * 8, v = token(u);
@@ -125,14 +136,10 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
           if (v + e >= 0 && v + e < a.vocab) z[e] += p[e];
       }
     }
-    if (allowed != nullptr) {
-      const int w = v < 0 ? 0 : v >> 5;
-      const uint32_t lo = allowed[w], hi = w + 1 < a.words ? allowed[w + 1] : 0u;
-      const uint32_t bits = v < 0 ? lo << -v : __funnelshift_r(lo, hi, v & 31);
+    if (GRAMMAR)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (!(bits >> e & 1u)) z[e] = -INFINITY;
-    }
+        if (!(bits[u] >> e & 1u)) z[e] = -INFINITY;
     T o[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) o[e] = round_to<T>(z[e]);
@@ -154,13 +161,14 @@ static cudaError_t launch_adjust(LogitsArgs a, cudaStream_t stream) {
   while (tokens > (long long)SLICE << a.slice_log) ++a.slice_log;
   const long long grid = (long long)a.batch << a.slice_log;
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  return launch_following(adjust_kernel<T, PER>, dim3(static_cast<unsigned>(grid)), dim3(THREADS), a.history.p == nullptr ? 0 : SLICE * sizeof(uint32_t),
+  return launch_following(a.allowed == nullptr ? adjust_kernel<T, PER, false> : adjust_kernel<T, PER, true>, dim3(static_cast<unsigned>(grid)), dim3(THREADS), a.history.p == nullptr ? 0 : SLICE * sizeof(uint32_t),
                           stream, a);
 }
-// Slices of 8192 tokens go over a row's history fewer times; where they are fewer than two for each SM, of 2048.
+// Slices of 8192 tokens go over a row's history fewer times; where they are fewer than two for each SM, of 2048. fp32 rows are twice as long: slices of 4096
+// have more loads under way (256 x 32001 with a history of 2001: 21.6 us, 22.9 in slices of 8192; bf16 19.7 and 18.5).
 template <typename T>
 static cudaError_t launch_adjust(const LogitsArgs& a, cudaStream_t stream) {
-  return (long long)a.batch * ((a.vocab + 8191) / 8192) >= 296 ? launch_adjust<T, 4>(a, stream) : launch_adjust<T, 1>(a, stream);
+  return (long long)a.batch * ((a.vocab + 8191) / 8192) >= 296 ? launch_adjust<T, sizeof(T) == 4 ? 2 : 4>(a, stream) : launch_adjust<T, 1>(a, stream);
 }
 
 }  // namespace nbc
