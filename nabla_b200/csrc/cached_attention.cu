@@ -547,11 +547,14 @@ __global__ void __launch_bounds__(JOIN_THREADS) attend_join_kernel(const AttendA
   store_out<T, D>(a, b, h, r, c, x);
 }
 
-// bf16 calls of more than 32 rows of a sequence and cache head go to tiles of 128 rows (cached_attention_tcgen05.cu), up to 128 rows where they are more than
-// 32 tiles of 16 in all: for few tiles of 16 the pass over the codes of each is quicker than the longer start. us, tiles of 16 and of 128, 4 heads of 128: one
-// sequence of 1000 with 48, 64, 128 rows 9.0 and 18.5, 9.8 and 18.7, 11.2 and 20.0, of 8000 17.0 and 20.2, 19.9 and 20.7, 20.9 and 23.5; eight of 1000 and 8000
-// with 32 rows 22.5 and 22.1, 43.9 and 50.4, with 48 26.5 and 23.9, 57.7 and 52.5.
-static bool many(int rows, int fp32, long long pairs) { return !fp32 && rows > 32 && (rows > 128 || pairs * ((rows + 15) / 16) > 32); }
+// bf16 calls of more than 32 rows of a sequence and cache head go to tiles of 128 rows (cached_attention_tcgen05.cu), up to 128 rows where they are more tiles of
+// 16 than 32, or than run at once where keys are few: the pass over the codes for each tile of 16 is then quicker than the longer start. us, tiles of 16 and of
+// 128, 4 heads of 128: 4 pairs of sequence and head with 48 to 128 rows 9 to 11 and 18 to 20 for 1000 tokens, 20 to 21 and 20 to 24 for 8000; 32 pairs
+// with 64 rows 15.5 and 26.1 for 1000, 27.4 and 27.5 for 2000, 69 and 55 for 8000; 64 pairs with 64 rows 32 and 43 for 2000, 131 and 97 for 8000, with 96
+// rows (384 tiles) 59 and 50 for 2000; 128 pairs with 48 rows 36 and 29 for 1000.
+static bool many(int rows, int fp32, long long pairs, long long room) {
+  return !fp32 && rows > 32 && (rows > 128 || pairs * ((rows + 15) / 16) > (room <= 2048 ? 296 : 32));
+}
 
 // How a call is cut, by its sizes alone.
 struct Cut {
@@ -562,7 +565,7 @@ struct Cut {
 };
 static int few_rows(int rows) { return rows <= 8 ? 8 : 16; }
 static Cut cut(int batch, int rows, long long heads_rows, int kv_heads, int head_dim, long long room, int fp32) {
-  const bool wide = many(rows, fp32, (long long)batch * kv_heads);
+  const bool wide = many(rows, fp32, (long long)batch * kv_heads, room);
   Cut c = {ONE, 1, wide ? 128 : few_rows(rows), 0};
   const long long units = (long long)batch * kv_heads * ((rows + c.rows - 1) / c.rows);
   if (wide) {
@@ -573,12 +576,17 @@ static Cut cut(int batch, int rows, long long heads_rows, int kv_heads, int head
   }
   const long long most = (room + UNIT - 1) / UNIT;
   if (most < 2) return c;                                                    // a step for each warp
+  // Lines that are short or many are not shared: a block that ends and begins within lines of 500 tokens has more to join than to read. us, shared and whole, with
+  // 4 rows: 64 lines of 500 12.2 and 7.9, of 62 to 938 12.8 and 12.1, of 2000 20.6 and 23.8, of 250 to 3750 20.5 and 36.8; 256 of 500 22.5 and 13.9, of 2000
+  // 36.8 and 35.4, of 250 to 3750 40.7 and 51.5; 1024 of 250 to 3750 127 and 111. With 16 rows: 64 lines of 500 15.4 and 11.0, of 2000 27.0 and 28.1; 256 of
+  // 2000 57.8 and 35.2, of 250 to 3750 68.9 and 53.3, of 8000 131 and 114, of 1000 to 15000 143 and 191.
+  const bool whole = room <= (c.rows == 16 && 24 * units > 1024 ? 24 * units : units < 1024 ? 1024 : 4 * units);
   // us, a cluster of 8 and a line for 4 query heads to each of 1, 8, 16, 32, 64 pairs: 2000 tokens 7.0 and 8.1, 7.7 and 9.2, 8.4 and 9.8, 11.3 and 16.2, 21.2 and
   // 20.7; 8000 tokens 12.7 and 8.9, 16.0 and 13.0, 18.4 and 18.0, 23.1 and 24.4, 42.5 and 34.1
   if (units * 8 <= 296 && room <= 4096 + 256 * units) {
     c.share = CLUSTER;
     c.splits = room >= 512 ? 8 : room >= 256 ? 4 : 2;
-  } else if (rows <= 128 && batch <= FLAT_BATCH && units * most < (1ll << 31)) {
+  } else if (!whole && rows <= 128 && batch <= FLAT_BATCH && units * most < (1ll << 31)) {
     c.share = FLAT;
     const long long blocks = 148 * (c.rows == 8 ? 3 : 2);
     c.splits = static_cast<int>(blocks < units * most ? blocks : units * most);

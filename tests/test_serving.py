@@ -176,6 +176,30 @@ def test_attention_where_blocks_are_missing_and_scales_differ_widely(device, new
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("b,new,hq,h,longest", [
+    (1, 12, 16, 4, 700), (2, 16, 16, 4, 5000), (9, 32, 8, 4, 1000), (4, 16, 32, 8, 1900), (4, 16, 32, 8, 2300), (16, 24, 32, 8, 300), (3, 33, 16, 4, 1500),
+    (1, 9, 4, 1, 2080),
+])
+def test_attention_of_some_tens_of_rows(b, new, hq, h, longest, dtype):
+    """Between single tokens and prompts: rows of one to several tiles, on both sides of where another form is taken."""
+    g = gen("cuda", 43)
+    n, d, dtype = 64, 128, torch.bfloat16 if dtype == "bf16" else torch.float32
+    columns = -(-(longest + new) // n)
+    cache = new_cache(g, "cuda", b * columns + 1, h, n, d)
+    table = new_table(g, "cuda", b, columns, b * columns + 1)
+    past = torch.randint(0, longest + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
+    past[-1] = 0
+    past[0] = longest
+    count = torch.randint(0, new + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
+    count[0] = new
+    q = torch.randn((b, new, hq, d), generator=g, device="cuda").to(dtype)
+    got = F.cached_attention(T(q), wrap(cache), T(table), T(past), T(count)).to_torch()
+    want, bound = attend64(q, cache, table, past.tolist(), count.tolist(), True, d ** -0.5)
+    check_attention(got, want, bound, cache)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("b,hq,h,columns,longest,dtype", [
     (39, 16, 4, 11, 649, "bf16"),         # more units of keys than blocks share them, fewer, and far fewer than the table has room for
