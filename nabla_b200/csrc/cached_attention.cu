@@ -37,7 +37,6 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
 // for 69 MB, of which 8 are starts, the joining kernel and the way from the table to the first code. One sequence of 700 with 16 heads: 6 us.
 // Slower were copies through shared memory (37 us for the first), and products of whole numbers with the weights in fixed point, which need no 16-bit floats
 // but the maximum first and then more registers (35 to 43 us).
-constexpr int FEW_WARPS = 4, STEP = 32;
 constexpr float ROOM = 7.f;      // see the weights
 // Four-float piece c of a row of outputs in shared memory: pieces are turned so that the 8 lanes that an access serves at once meet different banks
 // (lane (g, t) writes pieces g * D / 32 ... of rows 2t and 2t + 1).
@@ -131,8 +130,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   // keys that the last row sees
   const int keys = live <= 0 ? 0 : static_cast<int>(min((long long)room, (long long)past + (a.causal ? (row0 + live - 1) / group + 1 : count)));
   const int per = SHARE == FLAT ? piece * UNIT : (keys + a.splits * STEP - 1) / (a.splits * STEP) * STEP;
-  const int k0 = min(keys, SHARE == FLAT ? unit0 * UNIT : sp * per), k1 = min(keys, k0 + per);
-  const int steps = (k1 - k0 + STEP - 1) / STEP, mine = (steps - warp + FEW_WARPS - 1) / FEW_WARPS;
+  const Keys range = keys_of(keys, SHARE == FLAT ? unit0 * UNIT : sp * per, per);
+  const int k0 = range.k0, k1 = range.k1, mine = steps_of(range, warp);
   const int all_see = a.causal ? min(keys - 1, past + row0 / group) : keys - 1;     // keys up to here are seen by every row
   const int n = 1 << a.block_log, last_key = max(k1 - 1, 0);
 
@@ -141,43 +140,44 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   // behind the last is the last again.)
   struct Place { int id[2], there; };
   auto find = [&](int step) {
-    const int at = k0 + (max(min(step, mine - 1), 0) * FEW_WARPS + warp) * STEP;
+    const int at = key_of(range, warp, mine, step);
     const int x = a.table.block(b, min(at, last_key) >> a.block_log), y = n == 16 ? a.table.block(b, min(at + 16, last_key) >> a.block_log) : x;
     const Place p = {{max(x, 0), max(y, 0)}, (x >= 0 ? 1 : 0) | (y >= 0 && at + 16 < k1 ? 2 : 0)};
     return p;
   };
   auto unit = [&](const Place& p, int i) { return (long long)p.id[i] * a.kv_heads + h; };
-  auto from = [&](const Place& p, int i, int step) {
-    return ((unit(p, i) << a.block_log) + ((k0 + (max(min(step, mine - 1), 0) * FEW_WARPS + warp) * STEP + 16 * i) & (n - 1))) * D;
-  };
+  auto row = [&](int i, int step) { return row_of(key_of(range, warp, mine, step), i, n); };
+  auto from = [&](const Place& p, int i, int step) { return ((unit(p, i) << a.block_log) + row(i, step)) * D; };
   uint4 kr[2][2][PIECES], vr[2][4];                   // [16 keys each][keys g and g + 8], [keys 2t, 2t + 1, 2t + 8, 2t + 9]
   float ks[2] = {0.f, 0.f}, vs[2] = {0.f, 0.f};
   auto get_keys = [&](const Place& p, int step) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int8_t* at = a.codes[0] + from(p, i, step) + g * D + t * 16;
+      if (!holds_keys(a, unit(p, i), row(i, step))) continue;
+      const int8_t* at = a.codes[0] + from(p, i, step) + g * D + t * 16;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u)
 #pragma unroll
-          for (int c = 0; c < PIECES; ++c) kr[i][u][c] = ldg16(at + u * 8 * D + c * 64);
-        ks[i] = scale_at(a.scales[0], unit(p, i));
-      }
+        for (int c = 0; c < PIECES; ++c) kr[i][u][c] = ldg16(at + u * 8 * D + c * 64);
+      ks[i] = scale_at(a.scales[0], unit(p, i));
+    }
   };
   auto get_values = [&](const Place& p, int step) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int8_t* at = a.codes[1] + from(p, i, step) + 2 * t * D + g * (D / 8);
+      if (!holds_keys(a, unit(p, i), row(i, step))) continue;
+      const int8_t* at = a.codes[1] + from(p, i, step) + 2 * t * D + g * (D / 8);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int8_t* row = at + ((r & 1) + 8 * (r >> 1)) * D;
-          if (D == 128) {
-            vr[i][r] = ldg16(row);
-          } else {
-            const uint2 x = ldg8(row);
-            vr[i][r].x = x.x, vr[i][r].y = x.y;
-          }
+      for (int r = 0; r < 4; ++r) {
+        const int8_t* codes = at + ((r & 1) + 8 * (r >> 1)) * D;
+        if (D == 128) {
+          vr[i][r] = ldg16(codes);
+        } else {
+          const uint2 x = ldg8(codes);
+          vr[i][r].x = x.x, vr[i][r].y = x.y;
         }
       }
+    }
   };
   Place now = find(0);
   get_keys(now, 0);
@@ -634,6 +634,20 @@ static cudaError_t launch_attend(const AttendArgs& a, const Cut& c, int* status,
 }
 
 }  // namespace nbc
+
+// The last row of a block of `block` tokens that the few-row kernel's loads touch for the range [from, from + length) of a sequence's keys.
+extern "C" int nb_cached_attention_last_row(int keys, int from, int length, int block) {
+  using namespace nbc;
+  const Keys k = keys_of(keys, from, length);
+  int last = 0;
+  for (int warp = 0; warp < FEW_WARPS; ++warp)
+    for (int mine = steps_of(k, warp), step = 0; step < (mine > 0 ? mine : 0) + 2; ++step)
+      for (int i = 0; i < 2; ++i) {
+        const int row = row_of(key_of(k, warp, mine, step), i, block) + 15;
+        last = row > last ? row : last;
+      }
+  return last;
+}
 
 // Scratch of a call with these sizes, in floats.
 extern "C" long long nb_cached_attention_scratch(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int columns, int fp32) {

@@ -21,6 +21,30 @@ struct AttendArgs {
   int* lines;                    // see attend_few_kernel
 };
 
+// Few rows: a block's warps take steps of STEP keys of its range in turn. The keys of a range, and the row of its block at which the loads of 16 keys start,
+// half i of a step. Loads have no condition, so every row that comes out of this lies in the block, with the 15 behind it: also those of a warp that
+// has no step (`mine` up to 0).
+constexpr int FEW_WARPS = 4, STEP = 32;
+struct Keys {
+  int k0, k1;
+};
+__host__ __device__ __forceinline__ Keys keys_of(int keys, int from, int length) {
+  Keys k = {0, 0};                                    // empty: at the first key, where 16 keys start (at the last one, they do not)
+  if (from < keys) k.k0 = from, k.k1 = keys - from < length ? keys : from + length;
+  return k;
+}
+__host__ __device__ __forceinline__ int steps_of(const Keys& k, int warp) { return ((k.k1 - k.k0 + STEP - 1) / STEP - warp + FEW_WARPS - 1) / FEW_WARPS; }
+__host__ __device__ __forceinline__ int key_of(const Keys& k, int warp, int mine, int step) {
+  const int last = step < mine - 1 ? step : mine - 1;
+  return k.k0 + ((last > 0 ? last : 0) * FEW_WARPS + warp) * STEP;
+}
+__host__ __device__ __forceinline__ int row_of(int key, int i, int block) { return (key + 16 * i) & (block - 1); }
+
+// Checked build: do the 16 keys from row `row` of a block and head lie in that block, and it in the cache?
+__device__ __forceinline__ bool holds_keys(const AttendArgs& a, long long unit, int row) {
+  return NB_IN_BOUNDS(NB_SITE_CACHE_CODE, unit, (long long)a.table.blocks * a.kv_heads) && NB_IN_BOUNDS(NB_SITE_CACHE_ROW, row, (1 << a.block_log) - 15);
+}
+
 // Four neighbouring numbers of row r (token r / group, head r % group) of cache head h.
 template <typename T, int D>
 __device__ __forceinline__ void store_out(const AttendArgs& a, int b, int h, int r, int c, float4 x) {

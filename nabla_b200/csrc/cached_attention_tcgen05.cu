@@ -165,19 +165,23 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
     const int key = lane >> 2, c = lane & 3, n = 1 << a.block_log;
     // lane i < 8 knows where the i-th 16 keys of a tile lie (those of no block: the cache's first, so that loads need no condition: behind one they
     // would be waited for where the paths meet)
-    struct Place { long long codes, unit; bool there; };
+    struct Place { long long codes, unit; bool there, in; };
     auto find = [&](int j) {
       const int at = (kt0 + j) * BT + 16 * (lane & 7);
       const int id = j < n_max && at < all_keys ? a.table.block(b, at >> a.block_log) : -1;
       const long long unit = (long long)max(id, 0) * a.kv_heads + h;
-      return Place{((unit << a.block_log) + (at & (n - 1))) * D, unit, id >= 0};
+      return Place{((unit << a.block_log) + (at & (n - 1))) * D, unit, id >= 0, holds_keys(a, unit, at & (n - 1))};
     };
     auto get = [&](int which, const Place& place, uint4 (&x)[MINE]) {
       const int8_t* codes = which ? a.codes[1] : a.codes[0];
 #pragma unroll
       for (int i = 0; i < MINE; ++i) {
         const int u = min(warp + i * ISSUER, UNITS - 1), k = u / PER_KEYS;
-        x[i] = ldg16(codes + __shfl_sync(0xffffffffu, place.codes, k >> 1) + ((k & 1) * 8 + key) * D + (u % PER_KEYS) * 64 + c * 16);
+        const long long at = __shfl_sync(0xffffffffu, place.codes, k >> 1);
+#ifdef NB_DEBUG_CHECKS
+        if (!__shfl_sync(0xffffffffu, place.in, k >> 1)) continue;
+#endif
+        x[i] = ldg16(codes + at + ((k & 1) * 8 + key) * D + (u % PER_KEYS) * 64 + c * 16);
       }
     };
     auto put = [&](uint32_t tile, const uint4 (&x)[MINE], bool offset) {

@@ -1,0 +1,88 @@
+"""Edges of the serving operations: where their loads lie, what starts off a boundary, what is hidden or comes in an unusual order.
+
+The definitions in 64 bits are those of ``test_serving.py``.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import nabla_b200 as nb
+from nabla_b200.nn import functional as F
+
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def T(x):
+    return nb.Tensor.from_torch(x)
+
+
+def gen(device, seed):
+    return torch.Generator(device).manual_seed(seed)
+
+
+# ---------------------------------------------------------------- where loads lie
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_loads_of_few_rows_stay_in_their_block(block):
+    """A range of keys may be empty (more ranges than keys, tiles that see less than their line has): its loads lie in the block all the same."""
+    from nabla_b200.native import load
+
+    ask = load("libnb_serving.so").nb_cached_attention_last_row
+    for keys in [*range(0, 300), 511, 512, 513, 1499, 1500, 4095, 120001]:
+        for splits in (1, 2, 4, 8):                              # a cluster's ranges
+            per = -(-keys // (32 * splits)) * 32
+            for s in range(splits):
+                assert ask(keys, s * per, per, block) < block, (keys, splits, s)
+        for unit in (0, 1, 2, 3, 11, 937, 1 << 20):                # a line's pieces
+            for pieces in (1, 3):
+                assert ask(keys, unit * 128, pieces * 128, block) < block, (keys, unit, pieces)
+
+
+_CHECKED = r"""
+import torch
+import nabla_b200 as nb
+from nabla_b200 import native
+from nabla_b200.nn import functional as F
+assert native.DEBUG_KERNELS
+T = nb.Tensor.from_torch
+g = torch.Generator("cuda").manual_seed(1)
+rand = lambda *s: torch.randn(s, generator=g, device="cuda")
+for n in (16, 32, 64, 128):
+    for d, dtype in ((64, torch.float32), (128, torch.bfloat16)):
+        for new in (1, 3, 40, 200):
+            # few tokens in a table with room for many, in the cache's last blocks
+            b, h, used, columns = 3, 2, 512 // n, 4096 // n
+            cache = F.init_kv_cache(b * used, h, d, n, device=nb.Accelerator(0))
+            table = torch.full((b, columns), -1, dtype=torch.int32, device="cuda")
+            table[:, :used] = torch.arange(b * used, device="cuda").flip(0).view(b, used)
+            past, count = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 37, 5], [new, new - 1, min(new, 1)]))
+            x = [T(rand(b, new, h, d).to(dtype)) for _ in range(2)]
+            cache = F.kv_cache_write(cache, *x, T(table), T(past), T(count))
+            for group in (1, 8):
+                F.cached_attention(T(rand(b, new, h * group, d).to(dtype)), cache, T(table), T(past), T(count)).to_torch()
+            F.kv_cache_read(cache, T(table), T(past * 0), T(past + count), 250)[0].to_torch()
+torch.cuda.synchronize()
+native.check_status()
+native.debug_check()
+native.debug_selftest("libnb_serving.so", 12, 8, 64, 16)
+print("FAILED CHECKS", native.debug_report()["count"])
+"""
+
+
+@pytest.mark.gpu
+def test_the_checked_build_finds_every_load_in_the_cache():
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    from nabla_b200.csrc import build
+
+    build.build_all(debug=True)
+    root = Path(__file__).resolve().parent.parent
+    env = dict(os.environ, NABLA_B200_DEBUG_KERNELS="1", PYTHONPATH=str(root))
+    r = subprocess.run([sys.executable, "-c", _CHECKED], capture_output=True, text=True, env=env, timeout=600, cwd=root)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-4000:]
+    assert "FAILED CHECKS 4" in r.stdout           # the self-test's, one for each unit of the library
