@@ -43,7 +43,8 @@ __global__ void __launch_bounds__(THREADS) adjust_kernel(const LogitsArgs a) {
   const uint32_t one = packed ? 65536u : 2u;
   follow_grid();
   const int b = blockIdx.x >> a.slice_log, s = blockIdx.x & ((1 << a.slice_log) - 1);
-  // groups of 8 tokens start where 8 logits of memory do: `shift` tokens of the row's first group belong to the row before
+  // groups of 8 tokens start where 8 logits of memory do: `shift` tokens of the row's first group belong to the row before. (in and out lie
+  // alike, which the entry checks)
   const T* in = static_cast<const T*>(a.in) + (long long)b * a.vocab;
   T* out = static_cast<T*>(a.out) + (long long)b * a.vocab;
   const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(in) / sizeof(T) & 7);
@@ -173,11 +174,12 @@ static cudaError_t launch_adjust(const LogitsArgs& a, cudaStream_t stream) {
 
 }  // namespace nbc
 
-// wide: bit 0 the history, bit 1 `length`, bit 2 `prompt` are 64-bit numbers.
+// wide: bit 0 the history, bit 1 `length`, bit 2 `prompt` are 64-bit numbers. -1: in and out do not start equally far from a boundary of 16 bytes.
 extern "C" int nb_adjust_logits(const void* in, void* out, const void* history, const void* length, const void* prompt, const float* repetition,
                                 const float* presence, const float* frequency, const float* bias, long long bias_sb, const void* allowed, int wide,
                                 int batch, int vocab, int longest, int words, int fp32, void* stream) {
   using namespace nbc;
+  if ((reinterpret_cast<uintptr_t>(in) ^ reinterpret_cast<uintptr_t>(out)) & 15) return -1;
   LogitsArgs a = {};
   a.in = in, a.out = out;
   a.history = Whole{history, wide & 1}, a.length = Whole{length, wide >> 1 & 1}, a.prompt = Whole{prompt, wide >> 2 & 1};

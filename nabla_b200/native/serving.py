@@ -110,6 +110,8 @@ def _scratch(*sizes: int) -> int:
 def adjust_logits(logits, history, length, prompt, repetition, presence, frequency, bias, allowed):
     vocab = logits.shape[-1]
     x = logits.contiguous()
+    if x.data_ptr() & 15:         # a dense view that starts off a boundary; the kernel writes vectors where it reads vectors
+        x = x.clone()
     b = x.numel() // vocab
     history, length, prompt, repetition, presence, frequency, bias, allowed = (
         t.contiguous() if t is not None else None for t in (history, length, prompt, repetition, presence, frequency, bias, allowed))

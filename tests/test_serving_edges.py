@@ -86,3 +86,60 @@ def test_the_checked_build_finds_every_load_in_the_cache():
     r = subprocess.run([sys.executable, "-c", _CHECKED], capture_output=True, text=True, env=env, timeout=600, cwd=root)
     assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-4000:]
     assert "FAILED CHECKS 4" in r.stdout           # the self-test's, one for each unit of the library
+
+
+# ---------------------------------------------------------------- logits that start off a boundary
+def off_boundary(x, by):
+    """A dense copy of x that starts ``by`` elements behind a boundary."""
+    return torch.zeros(x.numel() + by, device=x.device, dtype=x.dtype)[by:].view(x.shape).copy_(x)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_kernel_of_logits_is_given_rows_that_start_alike(dtype, monkeypatch):
+    """It writes vectors where it reads vectors, so both addresses have to be the same distance from a boundary of 16 bytes."""
+    from nabla_b200.native import load, serving
+
+    given = []
+
+    class Library:
+        def nb_adjust_logits(self, x, out, *more):
+            given.append((x.value, out.value))
+            return 0
+
+    monkeypatch.setattr(serving, "_L", Library)
+    monkeypatch.setattr(serving, "stream_ptr", lambda: None)
+    for by in range(9):
+        for rows in (1, 3):
+            serving.adjust_logits(off_boundary(torch.zeros(rows, 33, dtype=dtype), by), *[None] * 8)
+    assert len(given) == 18 and all((x - out) % 16 == 0 for x, out in given)
+    # and the entry refuses others
+    entry = load("libnb_serving.so").nb_adjust_logits
+    import ctypes
+
+    entry.argtypes = [ctypes.c_void_p] * 9 + [ctypes.c_longlong, ctypes.c_void_p] + [ctypes.c_int] * 6 + [ctypes.c_void_p]
+    for x, out in ((1 << 20 | 2, 1 << 21), (1 << 20, 1 << 21 | 8)):
+        assert entry(x, out, *[None] * 7, 0, None, 0, 1, 33, 0, 0, int(dtype == torch.float32), None) == -1
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,vocab", [(1, 33), (3, 4099), (5, 8192)])
+def test_logits_that_start_off_a_boundary(rows, vocab, dtype, device):
+    """The last token's logits of a prompt, as a view: the same as from a tensor of their own, to the last bit."""
+    g = gen(device, 51)
+    z = (torch.randn((rows, vocab), generator=g, device=device) * 3).to(dtype)
+    history = torch.randint(0, vocab, (rows, 50), generator=g, device=device, dtype=torch.int32)
+    bias = torch.randn(vocab, generator=g, device=device)
+    words = torch.randint(-(1 << 31), 1 << 31, (rows, -(-vocab // 32)), generator=g, device=device).to(torch.int32)
+    over = torch.full((rows,), 1.2, device=device)
+    calls = (lambda x: F.adjust_logits(x), lambda x: F.adjust_logits(x, T(history), repetition=T(over), presence=T(over), bias=T(bias), allowed=T(words)),
+             lambda x: F.adjust_logits(x, bias=T(off_boundary(bias, 1))))
+    for call in calls:
+        want = call(T(z)).to_torch()
+        compiled = nb.compile(call)
+        for by in (*range(1, 9), 0, 3):
+            assert torch.equal(call(T(off_boundary(z, by))).to_torch(), want)
+            assert torch.equal(compiled(T(off_boundary(z, by))).to_torch(), want)
+    whole = torch.randn((1, 4, vocab), generator=g, device=device).to(dtype)
+    last = nb.squeeze(nb.slice_tensor(T(whole), (0, 3, 0), (1, 1, vocab)), axis=1)
+    assert torch.equal(F.adjust_logits(last, bias=T(bias)).to_torch(), F.adjust_logits(T(whole[:, 3].clone()), bias=T(bias)).to_torch())
