@@ -361,6 +361,11 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           gt[2 * c + k] = fmaf(fmaxf(x, y), fs[2 * c + k], adds[2 * c + k]);
         }
       }
+      if (kv0 + BT - 1 > first_t[t]) {     // the scale of 16 keys that a row does not see may be NaN
+#pragma unroll
+        for (int k = 0; k < GROUPS; ++k)
+          if (kv0 + 16 * k > last) fs[k] = 1.f, adds[k] = 0.f, gt[k] = -INFINITY;
+      }
       const float mx = fmaxf(fmaxf(fmaxf(gt[0], gt[1]), fmaxf(gt[2], gt[3])), fmaxf(fmaxf(gt[4], gt[5]), fmaxf(gt[6], gt[7])));
       // the reference follows the maximum only when that has grown by 2^8: weights stay below 2^8
       float half = 1.f;                    // the root of what the sums so far are multiplied by (the factor may fall out of the range of fp32)

@@ -159,10 +159,11 @@ class CachedAttentionOp(Operation):
         p = torch.exp(s - torch.where(top == float("-inf"), 0.0, top))
         p = torch.where(seen[:, None, None], p, 0.0)
         total = p.sum(-1, keepdim=True)
-        v = torch.where(there[..., None, None], v, 0.0)      # hidden places may hold anything
-        hidden = torch.arange(k.shape[1], device=q.device) >= (past + count)[:, None]
-        v = torch.where(hidden[..., None, None], 0.0, v)
-        o = torch.einsum("bhgtk,bkhd->bthgd", p / torch.where(total == 0, 1.0, total), v)
+        # what a row does not see may be anything, what it sees and is not finite (all that a block holds for a head) makes it NaN
+        fine = torch.isfinite(v).all(-1)
+        o = torch.einsum("bhgtk,bkhd->bthgd", p / torch.where(total == 0, 1.0, total), torch.where(fine[..., None], v, 0.0))
+        reached = torch.einsum("btk,bkh->bth", seen.float(), (~fine).float()) > 0
+        o = torch.where(reached[..., None, None], float("nan"), o)
         return o.reshape(b, t, hq, d).to(q.dtype)
 
     def sharding_rule(self, input_shapes, output_shapes, **kw):

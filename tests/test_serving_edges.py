@@ -143,3 +143,62 @@ def test_logits_that_start_off_a_boundary(rows, vocab, dtype, device):
     whole = torch.randn((1, 4, vocab), generator=g, device=device).to(dtype)
     last = nb.squeeze(nb.slice_tensor(T(whole), (0, 3, 0), (1, 1, vocab)), axis=1)
     assert torch.equal(F.adjust_logits(last, bias=T(bias)).to_torch(), F.adjust_logits(T(whole[:, 3].clone()), bias=T(bias)).to_torch())
+
+
+# ---------------------------------------------------------------- what is hidden
+def same_answers(got, want, vmax):
+    """Two answers to the same question: each is off by the rounding of the result, and of weights, to the type (bf16: 8 and 11 bits; fp32: weights to 22 bits,
+    exponentials and sums) at most. Scores are the same sums of the same products."""
+    tol = 2.0 ** -7 * want.double().abs() + 2.0 ** -9 * vmax if got.dtype == torch.bfloat16 else torch.full_like(want, 2.0 ** -17 * vmax, dtype=torch.float64)
+    return bool(((got.double() - want.double()).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("new", [3, 40, 150, 300])
+def test_a_row_does_not_see_the_nan_of_a_later_token(new, which, block, dtype, device):
+    """A new token that is not finite makes its block NaN: rows in front of that block come out as if it were not there, those that reach it as NaN."""
+    g = gen(device, 52)
+    b, hq, h, d, past = 2, 8, 2, 64, 2 * block - 2
+    columns = (past + new) // block + 2
+    cache = {}
+    for name in ("k", "v"):
+        cache[name] = torch.randint(-127, 128, (b * columns, h, block, d), generator=g, device=device, dtype=torch.int8)
+        cache[name + "_scale"] = torch.rand((b * columns, h), generator=g, device=device) * 0.02 + 0.01
+    table = torch.arange(b * columns, device=device, dtype=torch.int32).view(b, columns)
+    first = torch.full((b,), past, device=device, dtype=torch.int32)
+    q = torch.randn((b, new, hq, d), generator=g, device=device).to(dtype)
+    call = lambda: F.cached_attention(T(q), {k: T(v) for k, v in cache.items()}, T(table), T(first)).to_torch()  # noqa: E731
+    want = call()
+    assert torch.isfinite(want).all()
+    for column in sorted({2, (past + new - 1) // block}):                # the first block of new tokens alone, the last of them
+        start = column * block - past                                    # the first row that sees it
+        assert 0 < start < new
+        kept = cache[which][column, 1].clone()                           # of the first sequence and the second head
+        cache[which][column, 1] = math.nan
+        got = call()
+        cache[which][column, 1] = kept
+        assert torch.isnan(got[0, start:, hq // 2:]).all()
+        for x, y in ((got[0, :start], want[0, :start]), (got[0, :, :hq // 2], want[0, :, :hq // 2]), (got[1], want[1])):
+            assert same_answers(x, y, 127 * 0.03)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("new", [20, 150])
+def test_a_later_token_that_is_not_finite_leaves_earlier_answers_alone(new, device):
+    """The same through the cache's own writing: infinities in a key and in a value of the last new token."""
+    g = gen(device, 53)
+    h, d, n = 2, 128, 16
+    q, k, v = (torch.randn((1, new, h, d), generator=g, device=device).to(torch.bfloat16) for _ in range(3))
+    table, past = T(torch.arange(20, device=device, dtype=torch.int32)[None]), T(torch.zeros(1, device=device, dtype=torch.int32))
+
+    def answer():
+        cache = F.kv_cache_write(F.init_kv_cache(20, h, d, n, device=past.device), T(k), T(v), table, past)
+        return F.cached_attention(T(q), cache, table, past).to_torch()
+
+    want = answer()
+    k[0, -1, 0, 5], v[0, -1, 1, 7] = math.inf, -math.inf
+    got, start = answer(), (new - 1) // n * n
+    assert torch.isnan(got[:, start:]).all() and same_answers(got[:, :start], want[:, :start], 6.0)
