@@ -9,18 +9,24 @@ is what autodiff replays (backward for VJP, forward for JVP) and what ``print(tr
 """
 from __future__ import annotations
 
+import contextlib
+import itertools
 import weakref
+from contextvars import ContextVar
 from typing import Any, Callable, Iterable
 
 from ..common import pytree
 from ..tensor.impl import TensorImpl
 
 
+_serials = itertools.count()
+
+
 class OpNode:
     """One recorded operation call."""
 
     __slots__ = ("op", "arg_leaves", "arg_treedef", "kwargs", "op_kwargs", "out_refs", "out_treedef", "_hash",
-                 "__weakref__")
+                 "serial", "after", "__weakref__")
 
     def __init__(self, op, arg_leaves: list, arg_treedef, kwargs: dict, op_kwargs: dict):
         self.op = op
@@ -31,6 +37,8 @@ class OpNode:
         self.out_refs: list[weakref.ref] = []
         self.out_treedef = None
         self._hash = None
+        self.serial = next(_serials)          # nodes are numbered as they are made
+        self.after: list[TensorImpl] = []     # results that have to be there first, though they are no arguments
 
     # ---- arguments
     def input_impls(self) -> list[TensorImpl]:
@@ -93,7 +101,7 @@ def topo_nodes(output_impls: Iterable[TensorImpl], stop: Callable[[TensorImpl], 
         stack.append((n, 0))
         while stack:
             node, i = stack.pop()
-            inputs = node.arg_leaves
+            inputs = [*node.arg_leaves, *node.after] if node.after else node.arg_leaves
             advanced = False
             while i < len(inputs):
                 a = inputs[i]
@@ -109,6 +117,56 @@ def topo_nodes(output_impls: Iterable[TensorImpl], stop: Callable[[TensorImpl], 
             if not advanced:
                 order.append(node)
     return order
+
+
+# ---------------------------------------------------------------- updates in place
+# A compiled function is run later from what its results need, so the place of an update among the readers of what it updates has to be in the graph.
+_UPDATES: ContextVar[list | None] = ContextVar("nabla_updates", default=None)
+
+
+@contextlib.contextmanager
+def collect_updates():
+    """The updates in place that are recorded meanwhile: (node, what it updates, its results)."""
+    updates: list[tuple[OpNode, list[TensorImpl], list[TensorImpl]]] = []
+    token = _UPDATES.set(updates)
+    try:
+        yield updates
+    finally:
+        _UPDATES.reset(token)
+
+
+def note_update(old: Iterable[TensorImpl], new: Iterable[TensorImpl]) -> None:
+    """``new``, all of one node, will lie where ``old`` do."""
+    updates, new = _UPDATES.get(), list(new)
+    if updates is not None and new[0].output_refs is not None:
+        updates.append((new[0].output_refs, list(old), new))
+
+
+def order_updates(updates, targets: Iterable[TensorImpl], stop: Callable[[TensorImpl], bool]) -> dict[int, TensorImpl]:
+    """Gives every reader of what is updated the place that it has in the program: one recorded before an update comes before it, one recorded
+    after it reads the update's result. Returns the last result for (the id of) each updated tensor."""
+    readers: dict[int, list[OpNode]] = {}
+    for n in topo_nodes([*targets, *(o for _, _, new in updates for o in new)], stop):
+        for a in {id(a): a for a in n.input_impls()}.values():
+            readers.setdefault(id(a), []).append(n)
+    now: dict[int, TensorImpl] = {}
+
+    def newest(impl: TensorImpl) -> TensorImpl:
+        while id(impl) in now:
+            impl = now[id(impl)]
+        return impl
+
+    for node, old, new in updates:
+        for was, is_ in zip(map(newest, old), new):
+            for n in readers.pop(id(was), ()):
+                if n.serial < node.serial:
+                    node.after += [o for o in n.outputs() if o is not None]
+                elif n is not node:
+                    n.arg_leaves = [is_ if a is was else a for a in n.arg_leaves]
+                    n._hash = None
+                    readers.setdefault(id(is_), []).append(n)
+            now[id(was)] = is_
+    return {i: newest(impl) for i, impl in now.items()}
 
 
 class Trace:

@@ -16,6 +16,7 @@ import math
 import torch
 
 from .. import config
+from ..core.graph.tracing import note_update
 from ..core.sharding.propagation import OpShardingRule
 from ..core.tensor.api import Tensor
 from ..types import DType
@@ -277,6 +278,16 @@ def _same_device(*ts: Tensor) -> None:
     _need(len(devices) == 1, f"operands on several devices: {', '.join(sorted(str(d) for d in devices))}")
 
 
+def _now(out) -> tuple[Tensor, ...]:
+    """What reads or writes a cache is computed at once, so that writes and reads take place in the order of the program; in a function that is
+    being compiled, its recording keeps that order."""
+    if not config.get_flag("TRACING"):
+        from ..core.graph.engine import GRAPH
+
+        GRAPH.evaluate(*out)
+    return tuple(out)
+
+
 # ---------------------------------------------------------------- entry points
 def init_kv_cache(num_blocks: int, kv_heads: int, head_dim: int, block_size: int = 64, device=None) -> dict[str, Tensor]:
     """An empty cache of ``num_blocks`` blocks of ``block_size`` tokens (16, 32, 64 or 128) for heads of 64 or 128: two bytes
@@ -305,9 +316,9 @@ def kv_cache_write(cache: dict[str, Tensor], k: Tensor, v: Tensor, block_table: 
     front are rounded to the new scale, and starts anew when a token is written to the block's first row. Infinities and NaN make the
     scale of their block and head NaN, and with it all that the block holds for that head.
 
-    The cache is updated where it lies: the tensors that come back are those that were passed in, and values read from the cache earlier
-    have to be realized by then. Under ``compile(cuda_graph=True)`` donate the cache, else the graph copies it. ``inplace=False`` works on a
-    copy."""
+    The cache is updated where it lies: the tensors that come back are those that were passed in. Writes, reads and attention take place in the
+    order in which they are called, in compiled functions too; what other operations made of the cache's tensors has to be realized before a write
+    outside of them. Under ``compile(cuda_graph=True)`` donate the cache, else the graph copies it. ``inplace=False`` works on a copy."""
     parts, (blocks, heads, n, d) = _cache(cache)
     _tensor(k, "k", _FLOATS, (None, None, heads, d))
     batch, new = _shape(k)[:2]
@@ -315,11 +326,9 @@ def kv_cache_write(cache: dict[str, Tensor], k: Tensor, v: Tensor, block_table: 
     _places(block_table, past, count, batch, "past", n)
     more = () if count is None else (count,)
     _same_device(*parts, k, v, block_table, past, *more)
-    out = _write(*parts, k, v, block_table, past, *more, inplace=bool(inplace))
-    if inplace and not config.get_flag("TRACING"):
-        from ..core.graph.engine import GRAPH
-
-        GRAPH.evaluate(*out)       # now: a later write must not come before a read that was asked for in between
+    out = _now(_write(*parts, k, v, block_table, past, *more, inplace=bool(inplace)))
+    if inplace and config.get_flag("TRACING"):
+        note_update((t._impl for t in parts), (t._impl for t in out))
     return dict(zip(("k", "k_scale", "v", "v_scale"), out))
 
 
@@ -333,7 +342,7 @@ def kv_cache_read(cache: dict[str, Tensor], block_table: Tensor, start: Tensor, 
     _places(block_table, start, count, _shape(block_table)[0], "start", n)
     _need(int(max_tokens) >= 0, "max_tokens is negative")
     _same_device(*parts, block_table, start, count)
-    return tuple(_read(*parts, block_table, start, count, max_tokens=int(max_tokens), dtype=dtype.to_torch()))
+    return _now(_read(*parts, block_table, start, count, max_tokens=int(max_tokens), dtype=dtype.to_torch()))
 
 
 def cached_attention(q: Tensor, cache: dict[str, Tensor], block_table: Tensor, past: Tensor, count: Tensor | None = None, *, causal: bool = True,
@@ -352,7 +361,7 @@ def cached_attention(q: Tensor, cache: dict[str, Tensor], block_table: Tensor, p
     _need(scale > 0 and math.isfinite(scale), "scale has to be positive")
     more = () if count is None else (count,)
     _same_device(q, *parts, block_table, past, *more)
-    return _attend(q, *parts, block_table, past, *more, causal=bool(causal), scale=scale)
+    return _now((_attend(q, *parts, block_table, past, *more, causal=bool(causal), scale=scale),))[0]
 
 
 def adjust_logits(logits: Tensor, history: Tensor | None = None, length: Tensor | None = None, prompt_length: Tensor | None = None, *,

@@ -46,7 +46,7 @@ from .. import config, native
 from ..core.common import pytree
 from ..core.graph import fusion
 from ..core.graph.engine import GRAPH, _STATS, store_outputs
-from ..core.graph.tracing import OpNode, topo_nodes
+from ..core.graph.tracing import OpNode, collect_updates, order_updates, topo_nodes
 from ..core.tensor.api import Tensor
 from ..core.tensor.impl import TensorImpl
 from . import tape
@@ -532,16 +532,22 @@ class CompiledFunction:
             p_args.append(pytree.tree_unflatten(t_, ph_leaves[pos: pos + t_.num_leaves]))
             pos += t_.num_leaves
         p_kwargs = pytree.tree_unflatten(td_k, ph_leaves[pos:])
-        with config.tracing(True), config.eager_max_graph(False), config.capturable_trace(self.use_cuda_graph):
+        with config.tracing(True), config.eager_max_graph(False), config.capturable_trace(self.use_cuda_graph), collect_updates() as updates:
             result = self.fn(*p_args, **p_kwargs)
         out_leaves, out_td = pytree.tree_flatten(result)
         rec.out_treedef = out_td
-        targets = []
+        targets, written = [], set()
+        if updates:                                 # they take place whether or not their results are returned
+            promised = [o._impl for o in out_leaves if isinstance(o, Tensor)]
+            now = order_updates(updates, promised, lambda impl: impl.is_realized)
+            out_leaves = [Tensor(impl=now[id(o._impl)]) if isinstance(o, Tensor) and id(o._impl) in now else o for o in out_leaves]
+            targets = [o for _, _, new in updates for o in new]
+            written = {id(o) for o in targets}
         for o in out_leaves:
             if isinstance(o, Tensor):
                 rec.out_impls.append(o._impl)
                 rec.out_static.append(None)
-                if not o._impl.is_realized:
+                if not o._impl.is_realized and id(o._impl) not in written:
                     targets.append(o._impl)
             else:
                 rec.out_impls.append(None)

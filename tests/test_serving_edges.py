@@ -202,3 +202,116 @@ def test_a_later_token_that_is_not_finite_leaves_earlier_answers_alone(new, devi
     k[0, -1, 0, 5], v[0, -1, 1, 7] = math.inf, -math.inf
     got, start = answer(), (new - 1) // n * n
     assert torch.isnan(got[:, start:]).all() and same_answers(got[:, :start], want[:, :start], 6.0)
+
+
+# ---------------------------------------------------------------- the order of reads and writes
+class _Program:
+    """A cache of one sequence that holds three tokens, and others to be written over them."""
+
+    def __init__(self, device):
+        g = gen(device, 54)
+        self.k, self.other, self.q = (T(torch.randn((1, 3, 2, 64), generator=g, device=device)) for _ in range(3))
+        self.table, self.zero = (T(torch.tensor(x, device=device, dtype=torch.int32)) for x in ([[3, 1]], [0]))
+        self.three, self.five = (T(torch.tensor([x], device=device, dtype=torch.int32)) for x in (3, 5))
+        self.device = self.k.device
+
+    def cache(self):
+        return F.kv_cache_write(F.init_kv_cache(4, 2, 64, 16, device=self.device), self.k, self.k, self.table, self.zero)
+
+    def attend(self, cache):
+        return F.cached_attention(self.q, cache, self.table, self.zero)
+
+    def read(self, cache):
+        return F.kv_cache_read(cache, self.table, self.zero, self.three, 3, dtype=nb.DType.float32)
+
+    def write(self, cache, inplace=True):
+        return F.kv_cache_write(cache, self.other, self.other, self.table, self.zero, inplace=inplace)
+
+    def before(self):
+        c = self.cache()
+        return self.attend(c).to_torch(), self.read(c)[0].to_torch()
+
+    def after(self):
+        c = self.write(self.cache())
+        return self.attend(c).to_torch(), self.read(c)[0].to_torch()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_what_was_read_before_a_write_is_what_was_there(device):
+    """Answers that are looked at only after the next tokens were written."""
+    p = _Program(device)
+    (o, r), (o2, r2) = p.before(), p.after()
+    assert not torch.equal(o, o2) and not torch.equal(r, r2)
+    c = p.cache()
+    early = p.attend(c), p.read(c)[0]
+    copy = p.write(c, inplace=False)
+    later = p.write(c)
+    assert torch.equal(early[0].to_torch(), o) and torch.equal(early[1].to_torch(), r)
+    assert torch.equal(p.attend(c).to_torch(), o2) and torch.equal(p.attend(later).to_torch(), o2)
+    # a copy is of the cache as it was when it was asked for
+    c = p.cache()
+    copy = p.write(c, inplace=False)
+    F.kv_cache_write(c, p.q, p.q, p.table, p.three)
+    assert torch.equal(p.attend(copy).to_torch(), o2)
+    five = [F.kv_cache_read(x, p.table, p.zero, p.five, 5)[0].to_torch() for x in (copy, c)]
+    assert (five[0][:, 3:] == 0).all() and (five[1][:, 3:] != 0).any()
+    # a compiled step in between
+    c = p.cache()
+    early = p.attend(c)
+    nb.compile(p.write)(c)
+    assert torch.equal(early.to_torch(), o) and torch.equal(p.attend(c).to_torch(), o2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("form", ["read, write", "write, read", "the old name", "not returned", "the old name returned", "two writes", "another reader"])
+def test_compiled_programs_keep_the_order_of_reads_and_writes(form, device):
+    p = _Program(device)
+    (o, r), (o2, r2) = p.before(), p.after()
+
+    def program(c):
+        if form == "read, write":
+            early = p.attend(c), p.read(c)[0]
+            return p.write(c), early
+        if form == "write, read":
+            early = p.attend(c), p.read(c)[0]
+            c = p.write(c)
+            return early, c, p.attend(c), p.read(c)[0]
+        if form == "the old name":
+            new = p.write(c)
+            return p.attend(c), p.read(c)[0], new
+        if form == "not returned":
+            p.write(c)
+            return p.attend(c), p.read(c)[0]
+        if form == "the old name returned":
+            early = p.read(c)[0]
+            p.write(c)
+            return c, early
+        if form == "two writes":
+            early = p.read(c)[0]
+            p.write(c)
+            middle = p.read(c)[0]
+            F.kv_cache_write(c, p.k, p.k, p.table, p.zero)
+            return c, middle, early, p.attend(c)
+        early = c["k_scale"] * 2.0
+        p.write(c)
+        return c["k_scale"] * 2.0, early
+
+    f = nb.compile(program)
+    c = p.cache()
+    scale, scale2 = c["k_scale"].to_torch() * 2.0, p.write(p.cache())["k_scale"].to_torch() * 2.0
+    for _ in range(4):                       # recorded, replayed, and without Python
+        c = p.cache()
+        got = _leaves(f(c))
+        codes = c["k"].to_torch()
+        want = {"read, write": [None] * 4 + [o, r], "write, read": [o, r] + [None] * 4 + [o2, r2], "the old name": [o2, r2] + [None] * 4, "not returned": [o2, r2],
+                "the old name returned": [None] * 4 + [r], "two writes": [None] * 4 + [r2, r, o], "another reader": [scale2, scale]}[form]
+        assert len(got) == len(want) and all(w is None or torch.equal(x, w) for x, w in zip(got, want))
+        assert torch.equal(codes, (p.cache() if form == "two writes" else p.write(p.cache()))["k"].to_torch())
+        if None in want:                     # the cache that comes back is the one that was passed in
+            assert got[want.index(None)].data_ptr() == codes.data_ptr()
+
+
+def _leaves(x):
+    from nabla_b200.core.common import pytree
+
+    return [t.to_torch() for t in pytree.tree_leaves(x) if isinstance(t, nb.Tensor)]
