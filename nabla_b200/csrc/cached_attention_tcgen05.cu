@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
     for (int j = 0; j < n_max; ++j) {
       const int st = j & 1;
       const uint32_t ph = ((j >> 1) & 1) ^ 1;
-      ok = mbar_wait(&k_empty[st], ph);
+      ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ph));      // (the warp exchanges below)
       if (!ok) break;
       put(smem_u32(smem + L::K + st * L::TILE), kr, true);
       if (threadIdx.x < GROUPS) {
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
       fence_proxy_async_smem();
       mbar_arrive(&k_full[st]);
       get(0, next, kr);
-      ok = mbar_wait(&v_empty[st], ph);
+      ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ph));
       if (!ok) break;
       put(smem_u32(smem + L::V + st * L::TILE), vr, false);
       fence_proxy_async_smem();

@@ -315,3 +315,19 @@ def _leaves(x):
     from nabla_b200.core.common import pytree
 
     return [t.to_torch() for t in pytree.tree_leaves(x) if isinstance(t, nb.Tensor)]
+
+
+# ---------------------------------------------------------------- waits
+def test_warps_that_exchange_give_up_together():
+    """A bounded wait ends by each lane's own clock. Lanes that go on to exchange values with the others have to leave as one, or the wait for those
+    that left has no bound."""
+    import re
+    from pathlib import Path
+
+    source = (Path(nb.__file__).parent / "csrc" / "cached_attention_tcgen05.cu").read_text()
+    converting = source[source.index("if (warp < ISSUER) {"):source.index("} else if (warp == ISSUER) {")]
+    assert "__shfl_sync(0xffffffffu" in converting
+    assert len(re.findall(r"mbar_wait\(", converting)) == len(re.findall(r"__all_sync\(0xffffffffu, mbar_wait\(", converting)) == 2
+    softmax = source[source.index("} else if (warp == ISSUER) {"):]
+    softmax = softmax[softmax.index("  } else {"):]
+    assert len(re.findall(r"mbar_wait\(", softmax)) == len(re.findall(r"ok = __all_sync\(0xffffffffu, ok\);", softmax)) == 2
