@@ -37,7 +37,6 @@ __device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
 // for 69 MB, of which 8 are starts, the joining kernel and the way from the table to the first code. One sequence of 700 with 16 heads: 6 us.
 // Slower were copies through shared memory (37 us for the first), and products of whole numbers with the weights in fixed point, which need no 16-bit floats
 // but the maximum first and then more registers (35 to 43 us).
-constexpr float ROOM = 7.f;      // see the weights
 // Four-float piece c of a row of outputs in shared memory: pieces are turned so that the 8 lanes that an access serves at once meet different banks
 // (lane (g, t) writes pieces g * D / 32 ... of rows 2t and 2t + 1).
 template <int D>
@@ -300,8 +299,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
           for (int e = 0; e < 4; ++e)
             if (key0 + 16 * i + 8 * (e >> 1) + g > lim[u][e & 1]) s[u][i][e] = -INFINITY;
     }
-    // the reference that weights are taken against follows the maximum only when that has grown by 2^8. They are taken 2^7 larger, so that they stay
-    // below 2^15 and small ones, and the second parts of those of fp32 calls, keep their bits (16-bit floats have none below 2^-24)
+    // the reference that weights are taken against follows the maximum only when that has grown by 2^8
 #pragma unroll
     for (int u = 0; u < RT; ++u)
 #pragma unroll

@@ -73,8 +73,12 @@ __device__ __forceinline__ void store_part(const AttendArgs& a, int part, int b,
 //  - weights, to 11 bits. fp32 calls carry queries and weights as two such parts (22 bits) and take two products.
 // Scales never meet a rounding: a key's goes into its score, and a value's into the exponent of its weight. With
 //     t_j = scale * log2(e) * s_k(j) * (q . k_j) + log2 s_v(j),   m = max t_j,   P_j = 2^(t_j - m)
-// the output is sum P_j v_j / sum (P_j / s_v(j)), and the largest P is 1 however the scales differ. Where they differ so much that a P which counts in
+// the output is sum P_j v_j / sum (P_j / s_v(j)), and the largest P is near 1 however the scales differ. Where they differ so much that a P which counts in
 // the lower sum falls out of the range of fp32, P_j / s_v(j) is taken as an exponential of its own.
+// The m that weights are taken against is the largest t so far or up to 8 below it, and they are taken 2^ROOM larger: they stay below 2^15, and small ones, and
+// the second parts of those of fp32 calls, keep their bits (16-bit floats have none below 2^-24). What is lost of a weight is at most 2^-32 of
+// the largest: with 2^-25, a million keys that have 2 % of the sum together gave nothing to the output.
+constexpr float ROOM = 7.f;
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

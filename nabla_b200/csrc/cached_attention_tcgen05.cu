@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           if (kv0 + 16 * k > last) fs[k] = 1.f, adds[k] = 0.f, gt[k] = -INFINITY;
       }
       const float mx = fmaxf(fmaxf(fmaxf(gt[0], gt[1]), fmaxf(gt[2], gt[3])), fmaxf(fmaxf(gt[4], gt[5]), fmaxf(gt[6], gt[7])));
-      // the reference follows the maximum only when that has grown by 2^8: weights stay below 2^8
+      // the reference follows the maximum only when that has grown by 2^8
       float half = 1.f;                    // the root of what the sums so far are multiplied by (the factor may fall out of the range of fp32)
       bool grow = false;
       if (m == -INFINITY) {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
         m = mx;
         grow = true;
       }
-      const float base = m == -INFINITY ? 0.f : m;
+      const float base = m == -INFINITY ? 0.f : m - ROOM;
       if (__any_sync(0xffffffffu, grow)) {
         // the output is not being written now: s_full also tracks the product of the weights before
         l = l * half * half;
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           if (small >> k & 1) l += sum;
         }
       }
-      // Scores far from 0: an exponent is rounded as that of the maximum was, and less that then, so that the largest weight is 1 however far they are. It
+      // Scores far from 0: an exponent is rounded as that of the maximum was, and less that then, so that the largest weight is 2^ROOM however far they are. It
       // takes the score's place (rare). Near 0 the rounding of the sum of the two constants does not count (2^-15 at 512)
       float far = fabsf(base);
 #pragma unroll
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
                                  __uint_as_float(v[4 * i + 3]) * inverse);
           if (none) x = make_float4(0.f, 0.f, 0.f, 0.f);
           if (a.splits > 1) {
-            store_part<D>(a, sp, b, h, row, 8 * c + i, x, none ? -INFINITY : m + __log2f(l));
+            store_part<D>(a, sp, b, h, row, 8 * c + i, x, none ? -INFINITY : m - ROOM + __log2f(l));
           } else {
             store_out<__nv_bfloat16, D>(a, b, h, row, 8 * c + i, x);
           }

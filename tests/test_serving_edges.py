@@ -331,3 +331,24 @@ def test_warps_that_exchange_give_up_together():
     softmax = source[source.index("} else if (warp == ISSUER) {"):]
     softmax = softmax[softmax.index("  } else {"):]
     assert len(re.findall(r"mbar_wait\(", softmax)) == len(re.findall(r"ok = __all_sync\(0xffffffffu, ok\);", softmax)) == 2
+
+
+# ---------------------------------------------------------------- sums of very many weights
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,new,hq", [(75, 9, 4), (1, 40, 4), (2, 1, 4)])
+def test_a_million_small_weights_count(batch, new, hq):
+    """One key that has 2^25.5 times the weight of each of a million others: they have 2.2 % of the sum. All values are 1, and so is the answer; a
+    form that loses the others' values and not their part of the sum gives 0.978."""
+    n, d, keys = 128, 64, 1 << 20
+    columns = keys // n + 1
+    cache = {"k": torch.zeros((columns, 1, n, d), dtype=torch.int8, device="cuda"), "v": torch.full((columns, 1, n, d), 100, dtype=torch.int8, device="cuda")}
+    cache["k"][0, 0, 0, 0] = 127
+    for name in ("k_scale", "v_scale"):
+        cache[name] = torch.full((columns, 1), 0.01, device="cuda")
+    q = torch.zeros((batch, new, hq, d), dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 13.9375                                 # times 1.27, over ln 2: 25.54
+    table = torch.arange(columns, dtype=torch.int32, device="cuda").expand(batch, -1).contiguous()
+    past = torch.full((batch,), keys, dtype=torch.int32, device="cuda")
+    got = F.cached_attention(T(q), {k: T(v) for k, v in cache.items()}, T(table), T(past), scale=1.0).to_torch()
+    # the result's rounding; a weight of 2^-25.54 against a largest of 1 loses up to half of 16-bit floats' last bit, 2^-25, taken 2^7 larger: 2^-32 for each of 2^20
+    assert ((got.double() - 1).abs() <= 2.0 ** -8 + 2.0 ** -12).all(), (got.double() - 1).abs().max().item()
