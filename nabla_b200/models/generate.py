@@ -39,7 +39,9 @@ def init_caches(cfg: TransformerConfig, batch: int, max_tokens: int, block_size:
 def decode(params: dict[str, Any], tokens: Tensor, caches: list[dict[str, Tensor]], table: Tensor, past: Tensor, cfg: TransformerConfig,
            count: Tensor | None = None, positions: Tensor | None = None) -> tuple[Tensor, list[dict[str, Tensor]]]:
     """tokens (B, S), the first ``count`` (B,) of them behind ``past`` (B,) tokens that the caches hold -> logits (B, S, vocab) and the caches.
-    ``positions`` (B, S) index the position embedding: ``past + i`` by default."""
+    ``positions`` (B, S) index the position embedding: ``past + i`` by default, 0 for what lies behind ``count``."""
+    from ..ops.comparison import less
+    from ..ops.control_flow import where
     from ..ops.creation import arange
     from ..ops.unary import cast
     from ..ops.view import unsqueeze
@@ -47,7 +49,10 @@ def decode(params: dict[str, Any], tokens: Tensor, caches: list[dict[str, Tensor
     B, S = (int(n) for n in tokens.shape)
     H, hd = cfg.n_heads, cfg.head_dim
     if positions is None:
-        positions = unsqueeze(cast(past, DType.int64), axis=1) + arange(0, S, 1, dtype=DType.int64, device=tokens.device)
+        i = arange(0, S, 1, dtype=DType.int64, device=tokens.device)
+        positions = unsqueeze(cast(past, DType.int64), axis=1) + i
+        if count is not None:               # there may be no such position
+            positions = where(less(i, unsqueeze(cast(count, DType.int64), axis=1)), positions, positions * 0)
     x = gather(params["tok_emb"], tokens, axis=0) + gather(params["pos_emb"], positions, axis=0)
     out = []
     for p, cache in zip(params["layers"], caches):

@@ -352,3 +352,31 @@ def test_a_million_small_weights_count(batch, new, hq):
     got = F.cached_attention(T(q), {k: T(v) for k, v in cache.items()}, T(table), T(past), scale=1.0).to_torch()
     # the result's rounding; a weight of 2^-25.54 against a largest of 1 loses up to half of 16-bit floats' last bit, 2^-25, taken 2^7 larger: 2^-32 for each of 2^20
     assert ((got.double() - 1).abs() <= 2.0 ** -8 + 2.0 ** -12).all(), (got.double() - 1).abs().max().item()
+
+
+# ---------------------------------------------------------------- the end of a model's positions
+@pytest.mark.parametrize("device", DEVICES)
+def test_ragged_tokens_at_the_end_of_the_positions(device):
+    """A sequence with fewer new tokens than the others whose padding lies behind the model's last position."""
+    from nabla_b200.models import generate as G
+    from nabla_b200.models import transformer as M
+
+    cfg = M.TransformerConfig(n_layers=1, d_model=128, n_heads=2, d_ff=256, vocab=100, max_seq=20, dtype=nb.DType.float32)
+    with nb.default_device(nb.Accelerator(0) if device == "cuda" else nb.CPU()):
+        nb.seed(3)
+        params = M.init_params(cfg)
+    tokens = torch.randint(0, cfg.vocab, (2, 20), generator=gen("cpu", 55)).to(device)
+    of = lambda *x: T(torch.tensor(x, device=device, dtype=torch.int32))  # noqa: E731
+
+    def step(caches, table, tokens, past, count, positions=None):
+        logits, caches = G.decode(params, T(tokens.contiguous()), caches, table, past, cfg, count, positions)
+        return logits.to_torch(), caches
+
+    got = []
+    for given in (False, True):
+        caches, table = G.init_caches(cfg, 2, 20, 16, device=params["tok_emb"].device)
+        _, caches = step(caches, table, tokens[:, :18], of(0, 0), of(18, 3))
+        positions = T(torch.tensor([[18, 19, 0, 0], [3, 4, 5, 6]], device=device)) if given else None
+        logits, caches = step(caches, table, tokens[:, 16:20], of(18, 3), of(2, 4), positions)
+        got.append(torch.cat([logits[0, :2], logits[1]]))
+    assert torch.isfinite(got[0]).all() and torch.equal(got[0], got[1])
