@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -380,3 +381,40 @@ def test_ragged_tokens_at_the_end_of_the_positions(device):
         logits, caches = step(caches, table, tokens[:, 16:20], of(18, 3), of(2, 4), positions)
         got.append(torch.cat([logits[0, :2], logits[1]]))
     assert torch.isfinite(got[0]).all() and torch.equal(got[0], got[1])
+
+
+# ---------------------------------------------------------------- meshes
+@pytest.mark.parametrize("compiled", [False, True])
+def test_a_cache_whose_heads_are_split_is_written_where_it_lies(compiled):
+    """Each device writes its own heads into its own part of the cache, and reads before a write are of what was there."""
+    g = gen("cpu", 56)
+    b, t, h, d, n = 2, 3, 4, 64, 16
+    whole = {}
+    for name in ("k", "v"):
+        whole[name] = torch.randint(-127, 128, (8, h, n, d), generator=g, dtype=torch.int8)
+        whole[name + "_scale"] = torch.rand((8, h), generator=g) * 0.02 + 0.01
+    table, past = T(torch.randperm(8, generator=g)[:6].view(b, 3).to(torch.int32)), T(torch.tensor([5, 20], dtype=torch.int32))
+    k, v = (torch.randn((b, t, h, d), generator=g) for _ in range(2))
+    q = torch.randn((b, t, 2 * h, d), generator=g)
+    mesh = nb.DeviceMesh("m", (2,), ("tp",))
+    split = lambda x, at: T(x).shard(mesh, tuple("tp" if i == at else None for i in range(x.dim())))  # noqa: E731
+
+    def step(cache, q, k, v):
+        early = F.cached_attention(q, cache, table, past)
+        cache = F.kv_cache_write(cache, k, v, table, past)
+        return cache, early, F.cached_attention(q, cache, table, past)
+
+    plain = {name: T(x.clone()) for name, x in whole.items()}
+    _, early, late = step(plain, T(q), T(k), T(v))
+    parts = {name: split(x.clone(), 1) for name, x in whole.items()}
+    nb.realize_all(*parts.values())
+    lies = {name: [x.data_ptr() for x in p._impl._buffers] for name, p in parts.items()}
+    f = nb.compile(step) if compiled else step
+    for again in range(2 if compiled else 1):
+        got, early2, late2 = f(parts, split(q, 2), split(k, 2), split(v, 2))
+        for name in parts:
+            assert [x.data_ptr() for x in got[name]._impl._buffers] == lies[name]
+            assert np.array_equal(parts[name].to_numpy(), plain[name].to_numpy())
+        want = (early if again == 0 else late).to_torch()         # the second call finds the new tokens already there
+        assert torch.allclose(torch.from_numpy(early2.to_numpy()), want, atol=1e-5)
+        assert torch.allclose(torch.from_numpy(late2.to_numpy()), late.to_torch(), atol=1e-5)
