@@ -38,7 +38,7 @@ class OpNode:
         self.out_treedef = None
         self._hash = None
         self.serial = next(_serials)          # nodes are numbered as they are made
-        self.after: list[TensorImpl] = []     # results that have to be there first, though they are no arguments
+        self.after: tuple[TensorImpl, ...] = ()      # results that have to be there first, though they are no arguments
 
     # ---- arguments
     def input_impls(self) -> list[TensorImpl]:
@@ -160,7 +160,7 @@ def order_updates(updates, targets: Iterable[TensorImpl], stop: Callable[[Tensor
         for was, is_ in zip(map(newest, old), new):
             for n in readers.pop(id(was), ()):
                 if n.serial < node.serial:
-                    node.after += [o for o in n.outputs() if o is not None]
+                    node.after += tuple(o for o in n.outputs() if o is not None)
                 elif n is not node:
                     n.arg_leaves = [is_ if a is was else a for a in n.arg_leaves]
                     n._hash = None

@@ -9,10 +9,11 @@
 // feed the second product from there, the outputs are in columns 256 + t * D.
 //
 // Scales are one per 16 keys or more, so a row's 128 scores have 8 of them: the maximum is taken over each 16 scores first, then with the scales.
+// Scores of keys that a row does not see are put out of sight before that, and whole groups of them are taken without their scale, which may be NaN.
 // Keys keep the offset of their codes (1152 each), and the product's part of it, 1152 times the sum of the query's numbers, is taken from the
 // scores; values do not, their offset would cancel against far smaller sums.
 //
-// 2 x 2048 new tokens behind 2048, 16 heads over 4 of 128: 143 us for 93 GFLOP, 650 TFLOP/s, 40 % of the library's rate for a plain product. What bounds it: the
+// 2 x 2048 new tokens behind 2048, 16 heads over 4 of 128: 144 us for 93 GFLOP, 645 TFLOP/s, 40 % of the library's rate for a plain product. What bounds it: the
 // exponentials (2048 clocks of some 4600 for a tile of 128 keys and two of 128 rows) and the way from a product to its weights to the next product, which only
 // the other group's work covers. Making the codes costs 12 us of it. Two threads for a row (219 us), groups that take turns (186), weights without the
 // maximum first (153) and scores of 64 keys at a time (162) were slower.

@@ -7,11 +7,12 @@
 // so a block's scale only grows until its first row is written anew, and the rows in front are rounded again only when it does. A new
 // value that is not finite makes the scale NaN: all that the block holds reads as NaN, as the product with that value would be.
 //
-// Both kernels are bound by memory. One block of threads takes the rows of one cache block and head: it holds the new values in registers
-// between the maximum and the codes, so they are read once. Codes are made and read by adding numbers whose low bits they then are (two or three
-// instructions a code; with conversions and 64-bit divisions for the places the kernels were bound by instructions: writing 26.8, reading 36.6 us).
-// Writing 4 x 2048 tokens of 16 heads of 128, bf16: 19.9 us for 101 MB, 5.1 TB/s. Reading 16 sequences of up to 4001, 4 heads: 32.3 us for
-// 180 MB, 5.6 TB/s. One token for each of 64 sequences: 3.7 us, a launch and five accesses one after the other.
+// One block of threads takes the rows of one cache block and head: it holds the new values in registers between the maximum and the codes, so they
+// are read once. Codes are made and read by adding numbers whose low bits they then are (two or three instructions a code; with conversions and
+// 64-bit divisions for the places the kernels were bound by instructions: writing 26.8, reading 36.6 us).
+// Reading is bound by memory: 16 sequences of up to 4001, 4 heads, 32.3 us for 180 MB, 5.6 TB/s. Writing by memory and nearly as much by
+// instructions (the pipe for whole numbers 68 % busy): 4 x 2048 tokens of 16 heads of 128, bf16, 20 us for 101 MB, 5.0 TB/s. One token
+// for each of 64 sequences: 3.7 us, a launch and five accesses one after the other.
 #include "kv_cache.cuh"
 
 namespace nbc {

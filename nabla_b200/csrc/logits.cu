@@ -1,5 +1,5 @@
-// Adjusting logits before a token is chosen. Per row b and token v, in fp32, rounded once:
-//   z' = z / r or z * r       (z > 0 or not) where v stands in the row's history            repetition
+// Adjusting logits before a token is chosen. Per row b and token v, in fp32, rounded to the type of the logits at the end:
+//   z' = z / r or z * r       (z > 0 or not) where v stands in the row's history            repetition (z / r as z * (1 / r), two roundings of fp32)
 //   z' -= frequency * n + presence * [n > 0]          n: times that v stands in the history behind the prompt
 //   z' += bias[v]
 //   z' = -inf                 where the grammar's bit of v is 0
@@ -9,8 +9,8 @@
 // whole numbers: their order does not matter.
 // 256 rows of 32001 with histories of up to 2001, an odd row length, a bias and a grammar: 18.5 us in bf16, 21.6 in fp32; 13.9 and 17.5 without the bias, whose
 // rows start off boundaries, 10.9 and 14.7 without the histories, 5.6 in bf16 without any of the three (6.1 TB/s). One row of 32000 with 300 tokens: 2.8.
-// What bounds it are loads that wait for loads (10 of 17 stalled cycles) and going over the history for each slice. Blocks of 512 threads, and five or
-// six resident blocks were slower (20 to 24 us in bf16).
+// What bounds it are loads that wait for loads (4 of 11 cycles between a warp's instructions) and going over the history for each slice: 12 million
+// instructions, 2.3 a clock. Blocks of 512 threads, and five or six resident blocks were slower (20 to 24 us in bf16).
 #include "kv_cache.cuh"
 
 namespace nbc {

@@ -334,7 +334,7 @@ def kv_cache_write(cache: dict[str, Tensor], k: Tensor, v: Tensor, block_table: 
 
 def kv_cache_read(cache: dict[str, Tensor], block_table: Tensor, start: Tensor, count: Tensor, max_tokens: int, dtype=None) -> tuple[Tensor, Tensor]:
     """Keys and values of positions ``start`` ... ``start + count - 1`` of each sequence as numbers: two tensors (batch, max_tokens, heads,
-    head_dim) of ``dtype`` (bf16 by default, or fp32). Rows from ``count`` on, and those of positions without a block, are zero."""
+    head_dim) of ``dtype`` (bf16 by default, or fp32). Rows from ``count`` on, and those of positions without a block, are zero. What is read is what the cache holds at the call."""
     parts, (blocks, heads, n, d) = _cache(cache)
     dtype = DType.bfloat16 if dtype is None else dtype
     _need(dtype in _FLOATS, "dtype has to be bfloat16 or float32", TypeError)
@@ -351,7 +351,8 @@ def cached_attention(q: Tensor, cache: dict[str, Tensor], block_table: Tensor, p
 
     ``q``: (batch, new, heads, head_dim), bf16 or fp32; ``heads`` is a multiple of the cache's heads, which groups of neighbouring query
     heads share. Query i of a sequence stands at position ``past + i`` and sees positions 0 ... ``past + i``, with ``causal=False`` all of the
-    ``past + count``. Queries from ``count`` on, and those that see no key, come out as zeros. ``scale`` is 1 / sqrt(head_dim) by default."""
+    ``past + count``. Queries from ``count`` on, and those that see no key, come out as zeros; a block with a NaN scale makes the queries that
+    reach it NaN and no others. ``scale`` is 1 / sqrt(head_dim) by default."""
     parts, (blocks, heads, n, d) = _cache(cache)
     _tensor(q, "q", _FLOATS, (None, None, None, d))
     batch, _, hq, _ = _shape(q)
@@ -367,7 +368,7 @@ def cached_attention(q: Tensor, cache: dict[str, Tensor], block_table: Tensor, p
 def adjust_logits(logits: Tensor, history: Tensor | None = None, length: Tensor | None = None, prompt_length: Tensor | None = None, *,
                   repetition: Tensor | None = None, presence: Tensor | None = None, frequency: Tensor | None = None, bias: Tensor | None = None,
                   allowed: Tensor | None = None) -> Tensor:
-    """Logits (batch, vocab), bf16 or fp32, as the choice of the next token is to see them, computed in fp32 and rounded once:
+    """Logits (batch, vocab), bf16 or fp32, as the choice of the next token is to see them, computed in fp32 and rounded to their type at the end:
 
     * ``repetition`` (batch,): a token that stands in its row's history gets z / repetition where z > 0, else z * repetition;
     * ``frequency``, ``presence`` (batch,): a token that stands n > 0 times behind the prompt loses frequency * n + presence;
