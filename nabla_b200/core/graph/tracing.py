@@ -124,10 +124,20 @@ def topo_nodes(output_impls: Iterable[TensorImpl], stop: Callable[[TensorImpl], 
 _UPDATES: ContextVar[list | None] = ContextVar("nabla_updates", default=None)
 
 
+class Update:
+    """``node`` updates ``old`` in place. ``new``, of the same node, lie where those do; a node whose results need not (a branch or a loop that
+    updates) has none, and ``outs`` are its results."""
+
+    __slots__ = ("node", "old", "new", "outs")
+
+    def __init__(self, node: OpNode, old: list[TensorImpl], new: list[TensorImpl], outs: list[TensorImpl]):
+        self.node, self.old, self.new, self.outs = node, old, new, outs
+
+
 @contextlib.contextmanager
 def collect_updates():
-    """The updates in place that are recorded meanwhile: (node, what it updates, its results)."""
-    updates: list[tuple[OpNode, list[TensorImpl], list[TensorImpl]]] = []
+    """The updates in place that are recorded meanwhile."""
+    updates: list[Update] = []
     token = _UPDATES.set(updates)
     try:
         yield updates
@@ -136,17 +146,26 @@ def collect_updates():
 
 
 def note_update(old: Iterable[TensorImpl], new: Iterable[TensorImpl]) -> None:
-    """``new``, all of one node, will lie where ``old`` do."""
     updates, new = _UPDATES.get(), list(new)
     if updates is not None and new[0].output_refs is not None:
-        updates.append((new[0].output_refs, list(old), new))
+        updates.append(Update(new[0].output_refs, list(old), new, new))
 
 
-def order_updates(updates, targets: Iterable[TensorImpl], stop: Callable[[TensorImpl], bool]) -> dict[int, TensorImpl]:
+def note_updates_within(outs: Iterable[TensorImpl], inner: list[Update]) -> None:
+    """``outs`` are results of a node that runs functions of its own, which were seen to update ``inner`` when they were tried."""
+    updates, outs = _UPDATES.get(), list(outs)
+    if updates is None or not inner or not outs:
+        return
+    node = outs[0].output_refs
+    touched = {id(o) for u in inner for o in u.old}
+    updates.append(Update(node, [a for a in node.input_impls() if id(a) in touched], [], outs))
+
+
+def order_updates(updates: list[Update], targets: Iterable[TensorImpl], stop: Callable[[TensorImpl], bool]) -> dict[int, TensorImpl]:
     """Gives every reader of what is updated the place that it has in the program: one recorded before an update comes before it, one recorded
     after it reads the update's result. Returns the last result for (the id of) each updated tensor."""
     readers: dict[int, list[OpNode]] = {}
-    for n in topo_nodes([*targets, *(o for _, _, new in updates for o in new)], stop):
+    for n in topo_nodes([*targets, *(o for u in updates for o in u.outs)], stop):
         for a in {id(a): a for a in n.input_impls()}.values():
             readers.setdefault(id(a), []).append(n)
     now: dict[int, TensorImpl] = {}
@@ -156,16 +175,21 @@ def order_updates(updates, targets: Iterable[TensorImpl], stop: Callable[[Tensor
             impl = now[id(impl)]
         return impl
 
-    for node, old, new in updates:
-        for was, is_ in zip(map(newest, old), new):
+    for u in updates:
+        for k, was in enumerate(map(newest, u.old)):
+            is_ = u.new[k] if u.new else None
             for n in readers.pop(id(was), ()):
-                if n.serial < node.serial:
-                    node.after += tuple(o for o in n.outputs() if o is not None)
-                elif n is not node:
+                if n.serial < u.node.serial:
+                    u.node.after += tuple(o for o in n.outputs() if o is not None)
+                elif n is not u.node and is_ is None:
+                    n.after += tuple(u.outs)
+                elif n is not u.node:
                     n.arg_leaves = [is_ if a is was else a for a in n.arg_leaves]
                     n._hash = None
-                    readers.setdefault(id(is_), []).append(n)
-            now[id(was)] = is_
+                if n.serial >= u.node.serial:
+                    readers.setdefault(id(was if is_ is None else is_), []).append(n)
+            if is_ is not None:
+                now[id(was)] = is_
     return {i: newest(impl) for i, impl in now.items()}
 
 

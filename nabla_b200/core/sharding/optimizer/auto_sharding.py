@@ -39,7 +39,7 @@ def candidate_specs(shape: tuple[int, ...], mesh: DeviceMesh) -> list[list[Any]]
 def estimate_cost(func: Callable, args: tuple, mesh: DeviceMesh, specs: list) -> float:
     """Trace ``func`` on inputs laid out as ``specs`` (lazily: nothing executes) and sum op and
     communication costs of the recorded graph."""
-    from ...graph.tracing import topo_nodes
+    from ...graph.tracing import collect_updates, topo_nodes
     from ...tensor.api import Tensor
     from ....ops.communication import shard
 
@@ -49,7 +49,8 @@ def estimate_cost(func: Callable, args: tuple, mesh: DeviceMesh, specs: list) ->
             placed.append(shard(a, mesh, list(s)))
         else:
             placed.append(a)
-    out = func(*placed)
+    with collect_updates():                    # of no recording
+        out = func(*placed)
     impls = [t._impl for t in pytree.tensor_leaves(out)]
     nodes = topo_nodes(impls, lambda i: i.is_realized)
     total = 0.0

@@ -20,7 +20,7 @@ import torch
 
 from .. import config
 from ..core.common import pytree
-from ..core.graph.tracing import OpNode
+from ..core.graph.tracing import OpNode, collect_updates, note_updates_within
 from ..core.tensor.api import Tensor, realize_all
 from ..core.tensor.impl import TensorImpl
 from .base import Operation, _align_batch_dims, ensure_tensor
@@ -298,13 +298,16 @@ def cond(pred, true_fn: Callable, false_fn: Callable, *operands: Any):
     if not (isinstance(pred, Tensor) and config.get_flag("TRACING")):
         return true_fn(*operands) if _host_bool(pred) else false_fn(*operands)
     # both branches are traced lazily to learn (and check) the output structure
-    t_out = true_fn(*operands)
-    f_out = false_fn(*operands)
+    with collect_updates() as updates:
+        t_out = true_fn(*operands)
+        f_out = false_fn(*operands)
     t_leaves, out_td = pytree.tree_flatten(t_out)
     f_leaves, _ = pytree.tree_flatten(f_out)
     _same_structure(t_leaves, f_leaves, "cond")
     if config.is_capturable_trace():
         # stays on the device: both branches are part of the graph, `where` selects per call
+        if updates:
+            raise ValueError("cond in a captured function runs both branches, so neither may update its operands in place (inplace=False works on copies)")
         sel = [where(pred, a, b) if isinstance(a, Tensor) else a for a, b in zip(t_leaves, f_leaves)]
         return pytree.tree_unflatten(out_td, sel)
     op_leaves, op_td = pytree.tree_flatten(tuple(operands))
@@ -313,7 +316,9 @@ def cond(pred, true_fn: Callable, false_fn: Callable, *operands: Any):
     templates = [l for l in t_leaves if isinstance(l, Tensor)]
     kwargs = {"true_fn": true_fn, "false_fn": false_fn, "operand_treedef": op_td, "n_operands": len(op_tensors),
               "operand_leaves": [(isinstance(l, Tensor), None if isinstance(l, Tensor) else l) for l in op_leaves]}
-    outs = iter(_cond_op.build([pred, *op_tensors, *extra], templates, kwargs))
+    outs = _cond_op.build([pred, *op_tensors, *extra], templates, kwargs)
+    note_updates_within((o._impl for o in outs), updates)
+    outs = iter(outs)
     return pytree.tree_unflatten(out_td, [next(outs) if isinstance(l, Tensor) else l for l in t_leaves])
 
 
@@ -389,13 +394,16 @@ def while_loop(cond_fn: Callable, body_fn: Callable, init_val: Any):
     st_tensors = [l for l in st_leaves if isinstance(l, Tensor)]
     if config.get_flag("TRACING") and st_tensors:
         # one lazy application of the body checks that the state keeps its structure
-        probe = _apply_state(body_fn, state)
+        with collect_updates() as updates:
+            probe = _apply_state(body_fn, state)
         probe = tuple(probe) if isinstance(probe, (tuple, list)) else (probe,)
         _same_structure(st_leaves, pytree.tree_flatten(probe)[0], "while_loop")
         extra = [t for t in _closure_tensors(cond_fn, body_fn) if all(t._impl is not o._impl for o in st_tensors)]
         kwargs = {"cond_fn": cond_fn, "body_fn": body_fn, "state_treedef": st_td, "n_state": len(st_tensors),
                   "state_leaves": [(isinstance(l, Tensor), None if isinstance(l, Tensor) else l) for l in st_leaves]}
-        outs = iter(_while_op.build([*st_tensors, *extra], st_tensors, kwargs))
+        outs = _while_op.build([*st_tensors, *extra], st_tensors, kwargs)
+        note_updates_within((o._impl for o in outs), updates)
+        outs = iter(outs)
         state = tuple(pytree.tree_unflatten(st_td, [next(outs) if isinstance(l, Tensor) else l for l in st_leaves]))
     else:
         state = _while_eager(cond_fn, body_fn, state)

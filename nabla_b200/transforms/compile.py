@@ -541,7 +541,7 @@ class CompiledFunction:
             promised = [o._impl for o in out_leaves if isinstance(o, Tensor)]
             now = order_updates(updates, promised, lambda impl: impl.is_realized)
             out_leaves = [Tensor(impl=now[id(o._impl)]) if isinstance(o, Tensor) and id(o._impl) in now else o for o in out_leaves]
-            targets = [o for _, _, new in updates for o in new]
+            targets = [o for u in updates for o in u.outs]
             written = {id(o) for o in targets}
         for o in out_leaves:
             if isinstance(o, Tensor):

@@ -418,3 +418,58 @@ def test_a_cache_whose_heads_are_split_is_written_where_it_lies(compiled):
         want = (early if again == 0 else late).to_torch()         # the second call finds the new tokens already there
         assert torch.allclose(torch.from_numpy(early2.to_numpy()), want, atol=1e-5)
         assert torch.allclose(torch.from_numpy(late2.to_numpy()), late.to_torch(), atol=1e-5)
+
+
+# ---------------------------------------------------------------- branches and loops
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_branch_that_writes_writes_only_when_it_is_taken(device):
+    """cond and while_loop are recorded by trying their functions: what these update when they are tried is no update of the program."""
+    p = _Program(device)
+    (o, r), (o2, r2) = p.before(), p.after()
+
+    def program(go, c):
+        early = p.read(c)[0]
+        scale = nb.cond(go, lambda c: p.write(c)["k_scale"] * 1.0, lambda c: c["k_scale"] * 1.0, c)
+        return early, scale, p.read(c)[0], p.attend(c)
+
+    f = nb.compile(program)
+    for go in (False, True, False, True):
+        for call in (f, program):
+            c = p.cache()
+            early, scale, late, answer = call(T(torch.tensor(go, device=device)), c)
+            assert torch.equal(early.to_torch(), r) and torch.equal(late.to_torch(), r2 if go else r) and torch.equal(answer.to_torch(), o2 if go else o)
+            assert torch.equal(scale.to_torch(), c["k_scale"].to_torch())
+            assert torch.equal(c["k"].to_torch(), (p.write(p.cache()) if go else p.cache())["k"].to_torch())
+
+    # tokens one after the other
+    def loop(c, n):
+        def body(i, c):
+            at = nb.reshape(nb.cast(i, nb.DType.int32), (1,))
+            k = F.kv_cache_read(c, p.table, p.zero, p.zero + 1, 1, dtype=nb.DType.float32)[0]
+            return i + 1, F.kv_cache_write(c, k, k, p.table, at)
+
+        i, c = nb.while_loop(lambda i, c: i < n, body, (n * 0 + 1, c))
+        return c, p.read(c)[0]
+
+    g = nb.compile(loop)
+    for n in (1, 3, 2):
+        for call in (g, loop):
+            c = p.cache()
+            got, rows = call(c, T(torch.tensor(n, device=device)))
+            assert got["k"].to_torch().data_ptr() == c["k"].to_torch().data_ptr()
+            rows = rows.to_torch()
+            assert all(torch.equal(rows[:, i], rows[:, 0]) for i in range(n)) and (n == 3 or torch.equal(rows[:, 2], r[:, 2]))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_captured_cond_does_not_update_in_place(device):
+    """It runs both branches and selects."""
+    p = _Program(device)
+    go = T(torch.tensor(False, device=device))
+    f = nb.compile(lambda go, c: nb.cond(go, p.write, lambda c: c, c), cuda_graph=True)
+    with pytest.raises(ValueError, match="in place"):
+        f(go, p.cache())
+    f = nb.compile(lambda go, c: nb.cond(go, lambda c: p.write(c, inplace=False), lambda c: c, c), cuda_graph=True)
+    for go, want in ((False, p.before()[0]), (True, p.after()[0])):
+        c = p.cache()
+        assert torch.equal(p.attend(f(T(torch.tensor(go, device=device)), c)).to_torch(), want) and torch.equal(p.attend(c).to_torch(), p.before()[0])
