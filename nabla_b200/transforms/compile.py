@@ -1001,9 +1001,9 @@ def _tell_stream(rec: "_Recorded") -> None:
 
 @_functools.lru_cache(None)                         # (a taped call asks)
 def _counted_modules() -> tuple:
-    from ..native import attention, gemm, kernels, serving
+    from ..native import attention, gemm, heads, kernels, serving
 
-    return gemm, kernels, attention, serving
+    return gemm, kernels, attention, serving, heads
 
 
 _LEAF_KINDS = {"bias_grads", "sum_axes", "next_step", "scale_gemm", "gemm_scale"}
