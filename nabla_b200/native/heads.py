@@ -26,7 +26,7 @@ def _L():
         lib = load("libnb_heads.so")
         lib.nb_norm_rotary.argtypes = [c_vp] * 14 + [c_int] * 10 + [c_d, c_f, c_vp, c_int, c_vp, c_int, c_vp]
         lib.nb_norm_rotary.restype = c_int
-        lib.nb_norm_rotary_scratch.argtypes = [c_int] * 3
+        lib.nb_norm_rotary_scratch.argtypes = [c_int] * 6
         lib.nb_norm_rotary_scratch.restype = c_ll
         _lib = lib
     r = recorder()
@@ -65,7 +65,7 @@ def norm_rotary(parts, dys, positions, gains, *, eps: float, base: float, rotary
     grads, scratch = [None, None], None
     if dys is not None and any(g is not None for g in gains):
         grads = [torch.empty((d,), dtype=x.dtype, device=x.device) if g is not None else None for g in gains]
-        scratch = torch.empty(_scratch(b, t, d), dtype=torch.float32, device=x.device)
+        scratch = torch.empty(_scratch(b, t, sum(p.shape[2] for p in parts), d, rotary_dim, int(positions.dim() == 1)), dtype=torch.float32, device=x.device)
     dy = [ptr(y) for y in dys] + [c_vp(0)] * (3 - len(dys)) if dys is not None else [c_vp(0)] * 3
     rc = _L().nb_norm_rotary(ptr(parts[0]), ptr(parts[1]), ptr(v), *dy, *outs, ptr(gains[0]), ptr(gains[1]), ptr(grads[0]), ptr(grads[1]),
                              ptr(positions), int(positions.dtype == torch.int64), int(positions.dim() == 1), b, t, hq, parts[1].shape[2],
