@@ -1,4 +1,4 @@
-"""Python wrappers of the serving kernels (``csrc/kv_cache.cu``, ``csrc/cached_attention.cu``, ``csrc/logits.cu``).
+"""Python wrappers of the serving kernels (``csrc/kv_cache.cu``, ``csrc/cached_attention.cu``, ``csrc/logits.cu``, ``csrc/sample.cu``).
 
 Arguments are torch CUDA tensors whose shapes and types ``ops/serving.py`` has checked; scratch comes from torch's caching allocator.
 ``launch_count`` counts kernel launches issued from here.
@@ -25,6 +25,7 @@ def _L():
             "nb_kv_write": [c_vp] * 9 + [c_int] * 8 + [c_ll] * 6 + [c_int, c_vp],
             "nb_kv_read": [c_vp] * 9 + [c_int] * 9 + [c_vp],
             "nb_cached_attention": [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_vp, c_int, c_vp, c_vp],
+            "nb_sample_tokens": [c_vp] * 7 + [c_int] * 4 + [c_vp],
             "nb_adjust_logits": [c_vp] * 9 + [c_ll, c_vp] + [c_int] * 6 + [c_vp],
         }
         for name, args in sig.items():
@@ -122,4 +123,13 @@ def adjust_logits(logits, history, length, prompt, repetition, presence, frequen
     _ok(_L().nb_adjust_logits(ptr(x), ptr(out), ptr(history), ptr(length), ptr(prompt), ptr(repetition), ptr(presence), ptr(frequency), ptr(bias),
                               0 if bias is None or bias.dim() == 1 else vocab, ptr(allowed), _wide(history, length, prompt), b, vocab, longest,
                               allowed.shape[-1] if allowed is not None else 0, int(x.dtype == torch.float32), stream_ptr()), "adjust_logits")
+    return out
+
+
+def sample_tokens(logits, uniform, temperature, top_k, top_p, min_p):
+    x = logits if logits.is_contiguous() else logits.contiguous()
+    uniform, temperature, top_k, top_p, min_p = (t.contiguous() if t is not None else None for t in (uniform, temperature, top_k, top_p, min_p))
+    out = torch.empty(x.shape[0], dtype=torch.int64, device=x.device)
+    _ok(_L().nb_sample_tokens(ptr(x), ptr(uniform), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), ptr(out), _wide(top_k), x.shape[0], x.shape[1],
+                              int(x.dtype == torch.float32), stream_ptr()), "sample_tokens")
     return out

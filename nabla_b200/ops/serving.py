@@ -1,4 +1,4 @@
-"""Operations of a decoder that answers: a key / value cache in 8 bits, attention over it, and the adjustment of logits.
+"""Operations of a decoder that answers: a key / value cache in 8 bits, attention over it, the adjustment of logits and the draw of tokens.
 
 The cache is a dict of four tensors, ``{"k", "k_scale", "v", "v_scale"}``: codes (blocks, heads, block_size, head_dim) in int8 and one fp32
 scale per block and head (blocks, heads); a code of a block stands for code * scale. Which blocks are a sequence's says a table (batch,
@@ -6,8 +6,8 @@ columns) of whole numbers: position t of sequence b lies in row ``t % block_size
 no block (negative, or not below the number of blocks) is a place without tokens: writes to it are dropped, reads give zeros, attention
 sees no key there. Sequences may share blocks that are only read; a block that a call writes belongs to one sequence.
 
-Each is one ``Operation`` with hand-written kernels on CUDA (``csrc/kv_cache.cu``, ``cached_attention.cu``, ``logits.cu``) and an equivalent
-torch expression on the CPU. They have no derivatives. On a mesh the heads of the cache may be split as those of the model are.
+Each is one ``Operation`` with hand-written kernels on CUDA (``csrc/kv_cache.cu``, ``cached_attention.cu``, ``logits.cu``,
+``sample.cu``) and an equivalent torch expression on the CPU. They have no derivatives. On a mesh the heads of the cache may be split as those of the model are.
 """
 from __future__ import annotations
 
@@ -226,7 +226,55 @@ class AdjustLogitsOp(Operation):
         return OpShardingRule([dict(m) for m in ins], [dict(rows)])
 
 
-_write, _read, _attend, _adjust = KVCacheWriteOp(), KVCacheReadOp(), CachedAttentionOp(), AdjustLogitsOp()
+# ================================================================ draw
+LEAST_WEIGHT = 2.0 ** -44            # beside the likeliest token: what is less likely is not drawn
+MOST_VOCAB = 1 << 20
+
+
+class SampleTokensOp(Operation):
+    """``which`` names the operands behind the logits and the random numbers, in their order."""
+
+    def kernel(self, logits, uniform, *more, which: tuple[str, ...]):
+        if logits.device.type == "meta" or not logits.shape[0]:
+            return torch.empty(logits.shape[:1], dtype=torch.int64, device=logits.device)
+        given = dict(zip(which, more))
+        temperature, top_k, top_p, min_p = (given.get(n) for n in ("temperature", "top_k", "top_p", "min_p"))
+        if _runs_native(logits):
+            from ..native import serving
+
+            return serving.sample_tokens(logits, uniform, temperature, top_k, top_p, min_p)
+        z = torch.where(logits > float("-inf"), logits, float("-inf")).double()          # NaN too is nowhere
+        b, v = z.shape
+        hot = temperature > 0 if temperature is not None else torch.ones(b, dtype=torch.bool, device=z.device)
+        t = torch.where(hot, temperature, 1.0).double() if temperature is not None else torch.ones(b, dtype=torch.float64, device=z.device)
+        zs, order = torch.sort(z, dim=-1, descending=True, stable=True)
+        top = zs[:, :1]
+        w = torch.exp((zs - torch.where(torch.isinf(top), 0.0, top)) / t[:, None])
+        w = torch.where(zs == top, 1.0, torch.where(torch.isinf(top) | torch.isinf(zs) | (w < LEAST_WEIGHT), 0.0, w))
+        w = torch.where(zs > float("-inf"), w, 0.0)
+        rank = torch.arange(v, device=z.device)
+        keep = (rank == 0) | hot[:, None]
+        if top_k is not None:
+            keep &= (rank < top_k[:, None]) | (top_k[:, None] <= 0)
+        w = torch.where(keep, w, 0.0)
+        if top_p is not None:
+            p = top_p.double()[:, None]
+            w = torch.where((w.cumsum(-1) - w < p * w.sum(-1, keepdim=True)) | ~(p < 1) | (rank == 0), w, 0.0)
+        if min_p is not None:
+            m = min_p.double()[:, None]
+            w = torch.where((w >= m.clamp(max=1.0)) | ~(m > 0), w, 0.0)
+        weights = torch.zeros_like(w).scatter_(1, order, w)
+        total = weights.cumsum(-1)
+        u = uniform.double()[:, None]
+        token = (total <= torch.where(u > 0, u, 0.0) * total[:, -1:]).sum(-1)
+        last = torch.where(weights > 0, rank, -1).amax(-1)                                # -1: a row without a token
+        return torch.minimum(token, last)
+
+    def sharding_rule(self, input_shapes, output_shapes, **kw):
+        return OpShardingRule([{0: ["b"], 1: ["bcast_v"]}] + [{0: ["b"]} for _ in input_shapes[1:]], [{0: ["b"]}])
+
+
+_write, _read, _attend, _adjust, _sample = KVCacheWriteOp(), KVCacheReadOp(), CachedAttentionOp(), AdjustLogitsOp(), SampleTokensOp()
 
 
 # ---------------------------------------------------------------- checks of arguments
@@ -397,3 +445,29 @@ def adjust_logits(logits: Tensor, history: Tensor | None = None, length: Tensor 
         given["allowed"] = _tensor(allowed, "allowed", (DType.int32,), (batch, -(-vocab // 32)))
     _same_device(logits, *given.values())
     return _adjust(logits, *given.values(), which=tuple(given))
+
+
+def sample_tokens(logits: Tensor, uniform: Tensor, *, temperature: Tensor | None = None, top_k: Tensor | None = None, top_p: Tensor | None = None,
+                  min_p: Tensor | None = None) -> Tensor:
+    """The next token (batch,) int64 of each row of ``logits`` (batch, vocab), bf16 or fp32, drawn with the random number ``uniform`` (batch,) fp32 of [0, 1).
+
+    Tokens are ordered by their logits, equal ones by their ids; the weight of a token is exp((z - max z) / ``temperature``), those below 2^-44 are left
+    out. Of these, one filter behind the other keeps
+
+    * ``top_k`` (whole numbers; none where it is 0 or less): the first k;
+    * ``top_p`` (none from 1 on): those in front of which less than p of the weight that is left lies;
+    * ``min_p`` (none at 0): those with at least this weight;
+
+    and the first always. The token is the first one, in the order of ids, with which the sum of the weights that are left exceeds ``uniform`` of it. A
+    ``temperature`` of 0 takes the first in order (the lowest id of the largest logit). A row without a token (all are -inf or NaN) gives -1.
+    Each of the four is (batch,), fp32 but for ``top_k``, and may be left out. Weights are computed in 64 bits: the same row gives the same token."""
+    _tensor(logits, "logits", _FLOATS, (None, None))
+    batch, vocab = _shape(logits)
+    _need(1 <= vocab <= MOST_VOCAB, f"a vocabulary of {vocab}: 1 to {MOST_VOCAB} tokens")
+    _tensor(uniform, "uniform", (DType.float32,), (batch,))
+    given = {}
+    for name, t in (("temperature", temperature), ("top_k", top_k), ("top_p", top_p), ("min_p", min_p)):
+        if t is not None:
+            given[name] = _tensor(t, name, _WHOLE if name == "top_k" else (DType.float32,), (batch,))
+    _same_device(logits, uniform, *given.values())
+    return _sample(logits, uniform, *given.values(), which=tuple(given))
