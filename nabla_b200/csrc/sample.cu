@@ -10,15 +10,18 @@
 // Borders have to be met exactly, and sums must not depend on the order in which threads add: weights are whole multiples of 2^-43, computed in 64 bits (a draw
 // differs from one in exact arithmetic about once in 2^30), and their sums are sums of whole numbers. What the first k or a share p cut off is
 // found by selection, not by a sort: a histogram of the logits by their distance from the largest, in 2048 steps of a 45th of an octave of w, says where
-// the border lies, up to a step for p; a pass makes the sums there exact and checks it; what is left, some tens of tokens, is ranked in
-// shared memory. Where too many are left (equal logits, flat rows) steps are cut into 2048 finer ones of the order, down to single tokens.
+// the border lies, up to a step for p. Where all that is kept is some hundreds of tokens (a usual k) they are put into a list in shared memory, which is all
+// that the rest works on. Else a pass makes the sums exact and checks the border; the tokens of its steps, some tens, are ranked in a list, and another
+// pass makes the draw. Where too many are left (equal logits, flat rows) steps are cut into 2048 finer ones of the order, down to single tokens.
 //
-// One block of threads for each row; its warps own stretches of ids. The row is read four to six times, all but the first from the caches.
+// A row is read three to five times, all but the first from the caches, by one block of threads or by a cluster of up to eight, which exchange sums,
+// histograms and lists over distributed shared memory. Warps own stretches of ids.
+#include <cooperative_groups.h>
+
 #include "kv_cache.cuh"
 
 namespace nbc {
 using nb::follow_grid;
-using nb::launch_following;
 
 using u64 = unsigned long long;
 
@@ -27,10 +30,10 @@ struct SampleArgs {
   const float *uniform, *temperature, *top_p, *min_p;        // [batch], null: temperature 1, no filter
   Whole top_k;                   // p null: no filter
   long long* out;                // [batch]
-  int batch, vocab;
+  int vocab, blocks;             // blocks of a row
 };
 
-constexpr int SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32, BINS = 2048, LIST = SAMPLE_THREADS;
+constexpr int SAMPLE_THREADS = 512, SAMPLE_WARPS = SAMPLE_THREADS / 32, BINS = 2048, LIST = SAMPLE_THREADS, MOST_BLOCKS = 8;
 constexpr float FAR = 45.f;      // octaves that the histogram covers: weights end at 44
 constexpr double UNIT_WEIGHT = 8796093022208.0;              // 2^43
 
@@ -41,16 +44,17 @@ __device__ __forceinline__ uint32_t key_of(float z) {
 }
 __device__ __forceinline__ float number_of(uint32_t key) { return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu)); }
 __device__ __forceinline__ u64 order_of(float z, int v) { return z > -INFINITY ? (static_cast<u64>(key_of(z)) << 32) | (0xffffffffu - static_cast<uint32_t>(v)) : 0; }
+__device__ __forceinline__ int token_of(u64 order) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(order)); }
 
 struct Weigher {
   float top, per_octave;         // the largest logit; octaves of w for a unit of logit
   double rate;                   // 32 octaves
   const double* roots;           // 2^(-i / 32), in shared memory
 
-  // The step of the histogram that a logit falls into, BINS: behind its end. Monotone.
+  // The step of the histogram that a logit falls into, BINS: behind its end, or nowhere. Monotone.
   __device__ __forceinline__ int bin(float z) const {
     const float x = z == top ? 0.f : (top - z) * per_octave;
-    return x < FAR ? static_cast<int>(x * ((BINS - 1) / FAR)) : BINS;
+    return x < FAR ? __float_as_int(fmaf(x, (BINS - 1) / FAR, 8388608.f)) & 0xfff : BINS;        // + 2^23: the nearest whole number is in the low bits
   }
   __device__ __forceinline__ float about(float z) const { return z == top ? 1.f : exp2f((z - top) * per_octave); }
   // w, as a number and in multiples of 2^-43
@@ -77,10 +81,10 @@ template <typename T>
 struct LogitRow {
   const T* in;
   int vocab, shift, from, to;                                // groups of eight of this warp
-  __device__ __forceinline__ LogitRow(const T* p, int n) : in(p), vocab(n) {
+  __device__ __forceinline__ LogitRow(const T* p, int n, int rank, int blocks) : in(p), vocab(n) {
     shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) / sizeof(T) & 7);
-    const int groups = (vocab + shift + 7) / 8, each = ((groups + SAMPLE_WARPS - 1) / SAMPLE_WARPS + 31) / 32 * 32;
-    from = min(groups, static_cast<int>(threadIdx.x >> 5) * each), to = min(groups, from + each);
+    const int groups = (vocab + shift + 7) / 8, warps = blocks * SAMPLE_WARPS, each = ((groups + warps - 1) / warps + 31) / 32 * 32;
+    from = min(groups, (rank * SAMPLE_WARPS + static_cast<int>(threadIdx.x >> 5)) * each), to = min(groups, from + each);
   }
   __device__ __forceinline__ bool whole(int v) const { return v >= 0 && v + 8 <= vocab && NB_IN_BOUNDS(NB_SITE_LOGITS_TOKEN, v + 7, vocab); }
   // The eight logits from token v on, -inf where there is none
@@ -98,25 +102,34 @@ struct LogitRow {
       for (int e = 0; e < 8; ++e) z[e] = v + e >= 0 && v + e < vocab ? static_cast<float>(in[v + e]) : -INFINITY;
     }
   }
+  // f(token, logit) for all, two groups under way at once
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
-#pragma unroll 2
-    for (int g = from + (threadIdx.x & 31); g < to; g += 32) {
-      float z[8];
-      get(g * 8 - shift, z);
-      f(g * 8 - shift, z);
+#pragma unroll 1
+    for (int g = from + (threadIdx.x & 31); g < to; g += 64) {
+      float z[2][8];
+      const int v = g * 8 - shift;
+      get(v, z[0]);
+      const bool more = g + 32 < to;
+      if (more) get(v + 256, z[1]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f(v + e, z[0][e]);
+      if (more)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f(v + 256 + e, z[1][e]);
     }
   }
 };
 
 struct SampleShared {
   double roots[32];
-  uint32_t bins[BINS];
+  uint32_t bins[BINS], own_bins[BINS];     // of the row, of this block (blocks == 1: the row's are counted at once)
   u64 order[LIST], weights[LIST];
+  u64 own_order[LIST];                     // of this block's part of the row
+  u64 exchange[2][MOST_BLOCKS][3];         // what the blocks tell each other, in turn
   u64 joined[3][SAMPLE_WARPS];
   u64 edges[2];
-  int found, before, entries, total;
-  float mass;
+  int found, before, entries, total, turn;
 };
 
 __device__ __forceinline__ u64 over_warp_max(u64 x) {
@@ -124,40 +137,147 @@ __device__ __forceinline__ u64 over_warp_max(u64 x) {
   for (int w = 16; w; w >>= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, w));
   return x;
 }
-template <typename N>
-__device__ __forceinline__ N over_warp_sum(N x) {
+__device__ __forceinline__ u64 over_warp_sum(u64 x) {
 #pragma unroll
   for (int w = 16; w; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
   return x;
 }
-// All threads get the result.
-__device__ __forceinline__ u64 over_block_max(SampleShared& s, u64 x) {
+
+// The threads of a row: a block, or the blocks of a cluster.
+template <bool CLUSTER>
+struct Team {
+  SampleShared& s;
+  int rank, blocks;
+  int turn = 0;
+  __device__ __forceinline__ Team(SampleShared& shared, int n) : s(shared), rank(CLUSTER ? static_cast<int>(blockIdx.x) % n : 0), blocks(CLUSTER ? n : 1) {}
+  __device__ __forceinline__ void sync() const {
+    if constexpr (CLUSTER) cooperative_groups::this_cluster().sync(); else __syncthreads();
+  }
+  template <typename P>
+  __device__ __forceinline__ P* of(P* mine, int other) const { return cooperative_groups::this_cluster().map_shared_rank(mine, other); }
+
+  // Numbers that each block has, by rank: s.exchange[turn][rank][...]. All threads; `x` counts where threadIdx.x < N of every block
+  template <int N>
+  __device__ __forceinline__ const u64 (*told(u64 x))[3] {
+    turn ^= 1;
+    if constexpr (CLUSTER) {
+      if (threadIdx.x < N)
+        for (int r = 0; r < blocks; ++r) *of(&s.exchange[turn][rank][threadIdx.x], r) = x;
+    } else {
+      if (threadIdx.x < N) s.exchange[turn][0][threadIdx.x] = x;
+    }
+    sync();
+    return s.exchange[turn];
+  }
+  __device__ __forceinline__ u64 max_of(u64 x) {
+    x = over_warp_max(x);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.joined[0][threadIdx.x >> 5] = x;
+    __syncthreads();
+    const auto all = told<1>(over_warp_max(s.joined[0][threadIdx.x & (SAMPLE_WARPS - 1)]));
+    x = all[0][0];
+    for (int r = 1; r < blocks; ++r) x = max(x, all[r][0]);
+    return x;
+  }
+  __device__ __forceinline__ void sums_of(u64& x, u64& y, u64& z) {
+    x = over_warp_sum(x), y = over_warp_sum(y), z = over_warp_sum(z);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) s.joined[0][threadIdx.x >> 5] = x, s.joined[1][threadIdx.x >> 5] = y, s.joined[2][threadIdx.x >> 5] = z;
+    __syncthreads();
+    u64 part = 0;
+    if (threadIdx.x < 3)
+      for (int w = 0; w < SAMPLE_WARPS; ++w) part += s.joined[threadIdx.x][w];
+    const auto all = told<3>(part);
+    x = y = z = 0;
+    for (int r = 0; r < blocks; ++r) x += all[r][0], y += all[r][1], z += all[r][2];
+  }
+  // s.bins counts the tokens of the row for which `f` (token, logit) names a bin below BINS
+  template <typename T, typename F>
+  __device__ __forceinline__ void count(const LogitRow<T>& row, F&& f) {
+    uint32_t* bins = CLUSTER ? s.own_bins : s.bins;
+    sync();                                // (others have read the ones before)
+    for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) bins[i] = 0;
+    __syncthreads();
+    row.each([&](int v, float z) {
+      const int i = f(v, z);
+      if (i < BINS) atomicAdd(&bins[i], 1u);
+    });
+    sync();
+    if constexpr (CLUSTER) {
+      for (int i = threadIdx.x; i < BINS / 4; i += SAMPLE_THREADS) {
+        uint4 sum = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < MOST_BLOCKS; ++r)
+          if (r < blocks) {
+            const uint4 x = of(reinterpret_cast<uint4*>(s.own_bins), r)[i];
+            sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+          }
+        reinterpret_cast<uint4*>(s.bins)[i] = sum;
+      }
+      __syncthreads();
+    }
+  }
+  // s.order and s.weights (1 for `counted`) list the tokens of the row that `f` wants; their number. No more than LIST of them.
+  template <typename T, typename F>
+  __device__ __forceinline__ int list(const LogitRow<T>& row, const Weigher& weigh, bool counted, F&& f) {
+    u64* own = CLUSTER ? s.own_order : s.order;
+    sync();
+    if (threadIdx.x == 0) s.entries = 0;
+    __syncthreads();
+    row.each([&](int v, float z) {
+      if (!f(v, z)) return;
+      const int i = atomicAdd(&s.entries, 1);
+      if (i < LIST) own[i] = order_of(z, v);
+    });
+    __syncthreads();
+    int n = min(s.entries, LIST);
+    if constexpr (CLUSTER) {
+      const auto all = told<1>(static_cast<u64>(n));
+      n = 0;
+      for (int r = 0; r < blocks; ++r) {
+        const int m = static_cast<int>(all[r][0]);
+        const u64* from = of(s.own_order, r);
+        for (int i = threadIdx.x; i < m; i += SAMPLE_THREADS)
+          if (n + i < LIST) s.order[n + i] = from[i];
+        n = min(LIST, n + m);
+      }
+      __syncthreads();
+    }
+    if (static_cast<int>(threadIdx.x) < n) s.weights[threadIdx.x] = counted ? 1 : weigh.fixed(number_of(static_cast<uint32_t>(s.order[threadIdx.x] >> 32)));
+    __syncthreads();
+    return n;
+  }
+};
+// Over the threads of a block
+__device__ __forceinline__ u64 block_max(SampleShared& s, u64 x) {
   x = over_warp_max(x);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) s.joined[0][threadIdx.x >> 5] = x;
   __syncthreads();
   return over_warp_max(s.joined[0][threadIdx.x & (SAMPLE_WARPS - 1)]);
 }
-__device__ __forceinline__ void over_block_sums(SampleShared& s, u64& x, u64& y, u64& z) {
-  x = over_warp_sum(x), y = over_warp_sum(y), z = over_warp_sum(z);
+__device__ __forceinline__ u64 block_sum(SampleShared& s, u64 x) {
+  x = over_warp_sum(x);
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) s.joined[0][threadIdx.x >> 5] = x, s.joined[1][threadIdx.x >> 5] = y, s.joined[2][threadIdx.x >> 5] = z;
+  if ((threadIdx.x & 31) == 0) s.joined[0][threadIdx.x >> 5] = x;
   __syncthreads();
-  x = y = z = 0;
-#pragma unroll
-  for (int w = 0; w < SAMPLE_WARPS; ++w) x += s.joined[0][w], y += s.joined[1][w], z += s.joined[2][w];
+  x = threadIdx.x % 32 < SAMPLE_WARPS ? s.joined[0][threadIdx.x % 32] : 0;
+  return over_warp_sum(x);
 }
 
-// The last bin that holds a token and in front of which the sum of f(bin) (counts or weights) is below `want`: s.found (-1: none), s.before the tokens in
-// front of it; s.total: tokens of all bins, s.mass: the sum over all bins. All threads.
-template <typename N, typename F>
+// The last bin that holds a token and in front of which the sum of f(bin) (counts or weights) is below `want`, or below that share of all of it: s.found
+// (-1: none), s.before the tokens in front of it; s.total: tokens of all bins. All threads.
+template <typename N, bool SHARE, typename F>
 __device__ __forceinline__ void find_bin(SampleShared& s, N want, F&& f) {
   constexpr int PER = BINS / SAMPLE_THREADS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  N sum = 0;
-  int count = 0;
+  N part[PER], sum = 0;
+  int n[PER], count = 0;
 #pragma unroll
-  for (int i = 0; i < PER; ++i) sum += f(static_cast<int>(threadIdx.x) * PER + i), count += static_cast<int>(s.bins[threadIdx.x * PER + i]);
+  for (int i = 0; i < PER; ++i) {
+    n[i] = static_cast<int>(s.bins[threadIdx.x * PER + i]), part[i] = f(static_cast<int>(threadIdx.x) * PER + i);
+    sum += part[i], count += n[i];
+  }
 #pragma unroll
   for (int w = 1; w < 32; w <<= 1) {
     const N x = __shfl_up_sync(0xffffffffu, sum, w);
@@ -179,25 +299,24 @@ __device__ __forceinline__ void find_bin(SampleShared& s, N want, F&& f) {
     if (w == warp) x += all, y += all_count;                 // in front of this thread's bins
     all += sums[w], all_count += counts[w];
   }
+  if (SHARE) want *= all;
   int found = -1, before = 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
-    const int n = static_cast<int>(s.bins[threadIdx.x * PER + i]);
-    if (n > 0 && x < want) found = threadIdx.x * PER + i, before = y;
-    x += f(static_cast<int>(threadIdx.x) * PER + i), y += n;
+    if (n[i] > 0 && x < want) found = threadIdx.x * PER + i, before = y;
+    x += part[i], y += n[i];
   }
   if (found >= 0) atomicMax(&s.found, found);
-  if (threadIdx.x == 0) s.total = all_count, s.mass = static_cast<float>(all);
+  if (threadIdx.x == 0) s.total = all_count;
   __syncthreads();
   if (found >= 0 && found == s.found) s.before = before;
   __syncthreads();
 }
 // Tokens in bins [0, b). All threads.
 __device__ __forceinline__ int tokens_before(SampleShared& s, int b) {
-  u64 x = 0, y = 0, z = 0;
+  u64 x = 0;
   for (int i = threadIdx.x; i < b && i < BINS; i += SAMPLE_THREADS) x += s.bins[i];
-  over_block_sums(s, x, y, z);
-  return static_cast<int>(x);
+  return static_cast<int>(block_sum(s, x));
 }
 
 // A stretch of the order that holds a border: tokens with low <= order <= high, n of them at most, `sum` of weights (or tokens) in front.
@@ -207,23 +326,17 @@ struct Stretch {
 };
 
 // The place in the order of the last token in front of which less than `want` lies; the stretch holds it. COUNT: tokens are counted, not weighed.
-template <typename T, bool COUNT>
-__device__ __noinline__ u64 last_kept(SampleShared& s, const LogitRow<T>& row, const Weigher& weigh, Stretch at, double want) {
+template <typename T, bool CLUSTER, bool COUNT>
+__device__ __noinline__ u64 last_kept(Team<CLUSTER>& team, const LogitRow<T>& row, const Weigher& weigh, Stretch at, double want) {
+  SampleShared& s = team.s;
   for (int level = 0; at.n > LIST && level < 64; ++level) {   // (a few levels: each is at most 3 of some 2000 bins, or what is left beside them)
     // finer bins of the order
     const u64 range = at.high - at.low;
     const int shift = max(0, 64 - __clzll(static_cast<long long>(range)) - 11);
-    __syncthreads();
-    for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) s.bins[i] = 0;
-    __syncthreads();
-    row.each([&](int v, const float (&z)[8]) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const u64 q = order_of(z[e], v + e);
-        if (q >= at.low && q <= at.high) atomicAdd(&s.bins[(at.high - q) >> shift], 1u);
-      }
+    team.count(row, [&](int v, float z) {
+      const u64 q = order_of(z, v);
+      return q >= at.low && q <= at.high ? static_cast<int>((at.high - q) >> shift) : BINS;
     });
-    __syncthreads();
     const auto cut = [&](int first, int last) {              // the stretch of bins [first, last]
       Stretch x = at;
       x.high = at.high - (static_cast<u64>(first) << shift);
@@ -231,7 +344,7 @@ __device__ __noinline__ u64 last_kept(SampleShared& s, const LogitRow<T>& row, c
       return x;
     };
     if (COUNT) {
-      find_bin<int>(s, static_cast<int>(want) - static_cast<int>(at.sum), [&](int i) { return static_cast<int>(s.bins[i]); });
+      find_bin<int, false>(s, static_cast<int>(want) - static_cast<int>(at.sum), [&](int i) { return static_cast<int>(s.bins[i]); });
       const int c = s.found;
       Stretch x = cut(c, c);
       x.sum = at.sum + s.before, x.n = static_cast<int>(s.bins[c]);
@@ -239,23 +352,20 @@ __device__ __noinline__ u64 last_kept(SampleShared& s, const LogitRow<T>& row, c
       continue;
     }
     const float missing = static_cast<float>((want - static_cast<double>(at.sum)) / UNIT_WEIGHT);
-    find_bin<float>(s, missing, [&](int i) {
+    find_bin<float, false>(s, missing, [&](int i) {
       const u64 n = s.bins[i], middle = at.high - (static_cast<u64>(i) << shift) - (shift ? 1ull << (shift - 1) : 0);
       return n ? static_cast<float>(n) * weigh.about(number_of(static_cast<uint32_t>(middle >> 32))) : 0.f;
     });
     const int c = max(s.found, 0), first = max(c - 1, 0), last = min(c + 1, BINS - 1);
     Stretch x = cut(first, last);
     u64 above = 0, within = 0, none = 0;
-    row.each([&](int v, const float (&z)[8]) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const u64 q = order_of(z[e], v + e);
-        if (q > at.high || q < x.low) continue;
-        const u64 w = weigh.fixed(z[e]);
-        if (q > x.high) above += w; else within += w;
-      }
+    row.each([&](int v, float z) {
+      const u64 q = order_of(z, v);
+      if (q > at.high || q < x.low) return;
+      const u64 w = weigh.fixed(z);
+      if (q > x.high) above += w; else within += w;
     });
-    over_block_sums(s, above, within, none);
+    team.sums_of(above, within, none);
     above += at.sum;
     if (static_cast<double>(above) >= want) {                // it lies in front
       x = cut(0, first - 1);
@@ -268,20 +378,10 @@ __device__ __noinline__ u64 last_kept(SampleShared& s, const LogitRow<T>& row, c
     }
     at = x;
   }
-  __syncthreads();
-  if (threadIdx.x == 0) s.entries = 0;
-  __syncthreads();
-  row.each([&](int v, const float (&z)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const u64 q = order_of(z[e], v + e);
-      if (q < at.low || q > at.high) continue;
-      const int i = atomicAdd(&s.entries, 1);
-      if (i < LIST) s.order[i] = q, s.weights[i] = COUNT ? 1 : weigh.fixed(z[e]);
-    }
+  const int n = team.list(row, weigh, COUNT, [&](int v, float z) {
+    const u64 q = order_of(z, v);
+    return q >= at.low && q <= at.high && q != 0;
   });
-  __syncthreads();
-  const int n = min(s.entries, LIST);
   u64 kept = ~0ull;
   if (static_cast<int>(threadIdx.x) < n) {
     const u64 q = s.order[threadIdx.x];
@@ -289,56 +389,55 @@ __device__ __noinline__ u64 last_kept(SampleShared& s, const LogitRow<T>& row, c
     for (int j = 0; j < n; ++j) sum += s.order[j] > q ? s.weights[j] : 0;
     if (static_cast<double>(sum) < want) kept = q;
   }
-  return ~over_block_max(s, ~kept);
+  return ~block_max(s, ~kept);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs a) {
-  __shared__ SampleShared s;
+// The multiple of a weight's unit that the sum up to the drawn token exceeds: whole numbers exceed u * all where they exceed the whole part of that.
+__device__ __forceinline__ u64 target_of(float u, u64 all) {
+  const double to = u > 0.f ? static_cast<double>(u) * static_cast<double>(all) : 0.0;
+  return to < static_cast<double>(all) ? min(static_cast<u64>(to), all - 1) : all - 1;
+}
+
+template <typename T, bool CLUSTER>
+__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs a) {
+  __shared__ __align__(16) SampleShared s;
   if (threadIdx.x < 32) s.roots[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 32.0);
+  Team<CLUSTER> team(s, a.blocks);
+  if constexpr (CLUSTER) team.sync();      // every block of the cluster runs before another writes to it
   follow_grid();
-  const int b = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const LogitRow<T> row(static_cast<const T*>(a.in) + (long long)b * a.vocab, a.vocab);
-  u64 best = 0;
-  row.each([&](int v, const float (&z)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) best = max(best, order_of(z[e], v + e));
-  });
-  best = over_block_max(s, best);
-  const float temperature = a.temperature == nullptr ? 1.f : a.temperature[b];
+  const int b = CLUSTER ? blockIdx.x / a.blocks : blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const LogitRow<T> row(static_cast<const T*>(a.in) + (long long)b * a.vocab, a.vocab, team.rank, team.blocks);
+  const float temperature = a.temperature == nullptr ? 1.f : a.temperature[b], p = a.top_p == nullptr ? 1.f : a.top_p[b],
+              least = a.min_p == nullptr ? 0.f : a.min_p[b], u = a.uniform[b];
   const long long asked = a.top_k.p == nullptr ? 0 : a.top_k.at(b);
-  if (best == 0 || !(temperature > 0.f) || asked == 1) {
-    if (threadIdx.x == 0) a.out[b] = best == 0 ? -1ll : static_cast<long long>(0xffffffffu - static_cast<uint32_t>(best));
+  float largest = -INFINITY;
+  row.each([&](int v, float z) { largest = fmaxf(largest, z); });      // (passes over NaN)
+  const float top = number_of(static_cast<uint32_t>(team.max_of(key_of(largest))));
+  if (!(top > -INFINITY) || !(temperature > 0.f) || asked == 1) {
+    u64 first = 0;                         // the first in order
+    if (top > -INFINITY) {
+      row.each([&](int v, float z) { if (z == top) first = max(first, order_of(z, v)); });
+      first = team.max_of(first);
+    }
+    if (threadIdx.x == 0 && team.rank == 0) a.out[b] = first == 0 ? -1ll : token_of(first);
     return;
   }
-  const float p = a.top_p == nullptr ? 1.f : a.top_p[b], least = a.min_p == nullptr ? 0.f : a.min_p[b], u = a.uniform[b];
   const bool by_count = asked > 0 && asked < a.vocab, by_share = p < 1.f;
   const double rate = 46.166241308446828 / static_cast<double>(temperature);              // 32 log2(e)
-  const Weigher weigh = {number_of(static_cast<uint32_t>(best >> 32)), static_cast<float>(rate / 32.0), rate, s.roots};
+  const double floor_of = least > 0.f ? fmin(static_cast<double>(least), 1.0) : 0.0;
+  const Weigher weigh = {top, static_cast<float>(rate / 32.0), rate, s.roots};
   u64 last = 0;                            // of the order, the last that is kept
   if (by_count || by_share) {
-    const auto count_bins = [&] {
-      __syncthreads();
-      for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) s.bins[i] = 0;
-      __syncthreads();
-      row.each([&](int v, const float (&z)[8]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = z[e] > -INFINITY ? weigh.bin(z[e]) : BINS;
-          if (i < BINS) atomicAdd(&s.bins[i], 1u);
-        }
-      });
-      __syncthreads();
-    };
-    count_bins();
-    // the order of the first token of a bin is at most this: keys whose bin is below `b` begin there (bins fall as keys grow)
+    const auto in_bins = [&](int v, float z) { return weigh.bin(z); };
+    team.count(row, in_bins);
+    // keys whose bin is below `b` begin here (bins fall as keys grow)
     const auto edge = [&](int b) {
-      u64 lo = key_of(-INFINITY), hi = static_cast<u64>(key_of(weigh.top)) + 1;              // the least key in (lo, hi] with a bin below b
+      uint32_t lo = key_of(-INFINITY), hi = key_of(weigh.top) + 1;       // the least key in (lo, hi] with a bin below b
       while (hi - lo > 1) {
-        const u64 mid = (lo + hi) >> 1;
-        if (weigh.bin(number_of(static_cast<uint32_t>(mid))) < b) hi = mid; else lo = mid;
+        const uint32_t mid = lo + (hi - lo) / 2;
+        if (weigh.bin(number_of(mid)) < b) hi = mid; else lo = mid;
       }
-      return hi << 32;
+      return static_cast<u64>(hi) << 32;
     };
     const auto stretch = [&](int first, int last_bin) {      // of bins [first, last_bin]
       __syncthreads();
@@ -346,64 +445,90 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
       __syncthreads();
       return Stretch{s.edges[1], s.edges[0] - 1, 0, 0};
     };
-    const auto about = [&](int i) { return exp2f((static_cast<float>(i) + 0.5f) * (-FAR / (BINS - 1))); };
+    const auto about = [&](int i) { return exp2f(static_cast<float>(i) * (-FAR / (BINS - 1))); };
     int end = BINS, end_tokens = 0;        // the bin that top-k ends in, and how many of it are kept
-    if (by_count) {
-      find_bin<int>(s, static_cast<int>(asked), [&](int i) { return static_cast<int>(s.bins[i]); });
-      const int c = s.found, before = s.before;
-      if (s.total > asked) {
-        end = c, end_tokens = static_cast<int>(asked) - before;
-        Stretch x = stretch(c, c);
-        x.sum = before, x.n = static_cast<int>(s.bins[c]);
-        last = last_kept<T, true>(s, row, weigh, x, static_cast<double>(asked));
-        if (by_share && x.n > LIST) count_bins();              // finer bins took the histogram's place
+    find_bin<int, false>(s, by_count ? static_cast<int>(asked) : 0x7fffffff, [&](int i) { return static_cast<int>(s.bins[i]); });
+    const int c = s.found, before = s.before, total = s.total;
+    const bool cut = by_count && total > asked;
+    const int upto = before + static_cast<int>(s.bins[c]);   // tokens up to the bin that top-k ends in, or all of weight
+    if (upto <= LIST) {
+      // ---- all that may be kept is in a list, one entry for each thread
+      const int n = team.list(row, weigh, false, [&](int v, float z) { return weigh.bin(z) <= c; });
+      if constexpr (CLUSTER) {
+        team.sync();                       // (its lists have been read)
+        if (team.rank != 0) return;
       }
+      const bool mine = static_cast<int>(threadIdx.x) < n;
+      const u64 q = mine ? s.order[threadIdx.x] : 0, w = mine ? s.weights[threadIdx.x] : 0;
+      u64 sum = 0;
+      int place = 0;
+      if (mine)
+        for (int j = 0; j < n; ++j)
+          if (s.order[j] > q) ++place, sum += s.weights[j];
+      bool kept = mine && (!cut || place < asked);
+      if (by_share) {
+        const double want = static_cast<double>(p) * static_cast<double>(block_sum(s, kept ? w : 0));
+        kept = kept && (place == 0 || static_cast<double>(sum) < want);
+      }
+      kept = kept && weigh.weight(number_of(static_cast<uint32_t>(q >> 32))) >= floor_of;
+      const u64 all = block_sum(s, kept ? w : 0);            // (all threads are behind their reads of the weights)
+      if (mine) s.weights[threadIdx.x] = kept ? w : 0;
+      __syncthreads();
+      if (!kept || w == 0) return;
+      u64 front = 0;                       // of smaller ids
+      for (int j = 0; j < n; ++j) front += static_cast<uint32_t>(s.order[j]) > static_cast<uint32_t>(q) ? s.weights[j] : 0;
+      const u64 target = target_of(u, all);
+      if (target >= front && target < front + w) a.out[b] = token_of(q);
+      return;
+    }
+    if (cut) {
+      end = c, end_tokens = static_cast<int>(asked) - before;
+      Stretch x = stretch(c, c);
+      x.sum = before, x.n = static_cast<int>(s.bins[c]);
+      last = last_kept<T, CLUSTER, true>(team, row, weigh, x, static_cast<double>(asked));
+      if (by_share && x.n > LIST) team.count(row, in_bins);  // finer bins took the histogram's place
     }
     if (by_share) {
-      const auto mass = [&](int i) { return i > end ? 0.f : static_cast<float>(i == end ? end_tokens : static_cast<int>(s.bins[i])) * about(i); };
-      find_bin<float>(s, INFINITY, mass);
-      find_bin<float>(s, p * s.mass, mass);
-      const int c = max(s.found, 0), first = max(c - 1, 0), last_bin = min(c + 1, BINS - 1);
+      find_bin<float, true>(s, p, [&](int i) { return i > end ? 0.f : static_cast<float>(i == end ? end_tokens : static_cast<int>(s.bins[i])) * about(i); });
+      const int d = max(s.found, 0), first = max(d - 1, 0), last_bin = min(d + 1, BINS - 1);
       Stretch x = stretch(first, last_bin);
+      // the border of top-k as a number and an id, and the stretch as numbers (above the largest: no number, nothing is at least that)
+      const float z_last = last ? number_of(static_cast<uint32_t>(last >> 32)) : -INFINITY, z_low = number_of(static_cast<uint32_t>(x.low >> 32)),
+                  z_above = number_of(static_cast<uint32_t>(x.high >> 32) + 1);
+      const int v_last = last ? token_of(last) : -1;
       u64 all = 0, above = 0, within = 0;
-      row.each([&](int v, const float (&z)[8]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const u64 q = order_of(z[e], v + e);
-          if (q < last || q == 0) continue;
-          const u64 w = weigh.fixed(z[e]);
-          all += w;
-          if (q > x.high) above += w; else if (q >= x.low) within += w;
-        }
+      row.each([&](int v, float z) {
+        if (!(z > z_last || (z == z_last && v <= v_last))) return;
+        const u64 w = weigh.fixed(z);
+        all += w;
+        if (z >= z_above) above += w;
+        else if (z >= z_low) within += w;
       });
-      over_block_sums(s, all, above, within);
+      team.sums_of(all, above, within);
       const double want = fmax(static_cast<double>(p) * static_cast<double>(all), 0.5);     // (the first is kept)
       if (static_cast<double>(above) >= want) {
         x = stretch(0, first - 1);
         x.sum = 0, x.n = tokens_before(s, first);
       } else if (static_cast<double>(above + within) < want) {
         x = stretch(last_bin + 1, BINS - 1);
-        x.sum = above + within, x.n = tokens_before(s, BINS) - tokens_before(s, last_bin + 1);
+        x.sum = above + within, x.n = total - tokens_before(s, last_bin + 1);
       } else {
         x.sum = above, x.n = tokens_before(s, last_bin + 1) - tokens_before(s, first);
       }
       x.low = max(x.low, last);
-      last = last_kept<T, false>(s, row, weigh, x, want);
+      last = last_kept<T, CLUSTER, false>(team, row, weigh, x, want);
     }
   }
   // ---- the draw
-  const double floor_of = least > 0.f ? fmin(static_cast<double>(least), 1.0) : 0.0;
-  const auto drawn = [&](float z, int v) {
-    const u64 q = order_of(z, v);
-    if (q < last || q == 0) return 0ull;
+  const float z_last = last ? number_of(static_cast<uint32_t>(last >> 32)) : -INFINITY;
+  const int v_last = last ? token_of(last) : -1;
+  const auto drawn = [&](int v, float z) {
+    if (!(z > z_last || (z == z_last && v <= v_last))) return 0ull;
     const double w = weigh.weight(z);
     return w >= floor_of ? Weigher::whole(w) : 0ull;
   };
   u64 sum = 0;
-  row.each([&](int v, const float (&z)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) sum += drawn(z[e], v + e);
-  });
+  row.each([&](int v, float z) { sum += drawn(v, z); });
   sum = over_warp_sum(sum);
   __syncthreads();
   if (lane == 0) s.joined[0][warp] = sum;
@@ -413,17 +538,25 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
     if (w == warp) before = all;
     all += s.joined[0][w];
   }
-  // whole numbers: the sum with a token exceeds u * all where it is more than the whole part of that
-  const double to = u > 0.f ? static_cast<double>(u) * static_cast<double>(all) : 0.0;
-  const u64 target = to < static_cast<double>(all) ? min(static_cast<u64>(to), all - 1) : all - 1;
+  if constexpr (CLUSTER) {
+    const auto parts = team.template told<1>(all);
+    all = 0;
+    for (int r = 0; r < team.blocks; ++r) {
+      if (r == team.rank) before += all;
+      all += parts[r][0];
+    }
+    team.sync();                           // no block leaves while another still reads its bins or its list
+  }
+  const u64 target = target_of(u, all);
   if (target < before || target >= before + sum) return;
+#pragma unroll 1
   for (int g = row.from; g < row.to; g += 32) {              // the warp that holds it
     float z[8];
     u64 w[8], mine = 0;
     const int v = (g + lane) * 8 - row.shift;
     if (g + lane < row.to) row.get(v, z);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = g + lane < row.to ? drawn(z[e], v + e) : 0, mine += w[e];
+    for (int e = 0; e < 8; ++e) w[e] = g + lane < row.to ? drawn(v + e, z[e]) : 0, mine += w[e];
     u64 upto = mine;
 #pragma unroll
     for (int k = 1; k < 32; k <<= 1) {
@@ -448,19 +581,40 @@ __global__ void __launch_bounds__(SAMPLE_THREADS) sample_kernel(const SampleArgs
   }
 }
 
+template <typename T>
+static cudaError_t launch_sample(SampleArgs a, int batch, cudaStream_t stream) {
+  // blocks of a row: as many as the chip has room for twice over, each with 4096 tokens at least
+  a.blocks = 1;
+  while (a.blocks < MOST_BLOCKS && (long long)batch * a.blocks * 2 <= 296 && a.vocab > 4096 * a.blocks) a.blocks *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(static_cast<unsigned>(batch) * a.blocks);
+  cfg.blockDim = dim3(SAMPLE_THREADS);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  if (a.blocks > 1) {
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(a.blocks);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+  }
+  nb::set_following(cfg);
+  return cudaLaunchKernelEx(&cfg, a.blocks > 1 ? sample_kernel<T, true> : sample_kernel<T, false>, a);
+}
+
 }  // namespace nbc
 
 // wide: top_k holds 64-bit numbers. -1: more tokens than sums of weights have room for.
 extern "C" int nb_sample_tokens(const void* in, const float* uniform, const float* temperature, const void* top_k, const float* top_p, const float* min_p,
                                 void* out, int wide, int batch, int vocab, int fp32, void* stream) {
   using namespace nbc;
-  if (vocab < 1 || vocab > 1 << 20) return -1;
+  if (vocab < 1 || vocab > 1 << 20 || batch < 1) return -1;
   SampleArgs a = {};
   a.in = in, a.uniform = uniform, a.temperature = temperature, a.top_p = top_p, a.min_p = min_p;
   a.top_k = Whole{top_k, wide}, a.out = static_cast<long long*>(out);
-  a.batch = batch, a.vocab = vocab;
-  return launch_following(fp32 ? sample_kernel<float> : sample_kernel<__nv_bfloat16>, dim3(static_cast<unsigned>(batch)), dim3(SAMPLE_THREADS), 0,
-                          static_cast<cudaStream_t>(stream), a);
+  a.vocab = vocab;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return fp32 ? launch_sample<float>(a, batch, s) : launch_sample<__nv_bfloat16>(a, batch, s);
 }
 
 NB_DEBUG_DEFINE(sample)
