@@ -35,7 +35,8 @@ TARGETS: dict[str, tuple[list[str], list[str]]] = {
     "libnb_gemm.so": (["gemm_tcgen05.cu"], []),
     "libnb_kernels.so": (["fused_kernels.cu", "elementwise_kernels.cu"], []),
     "libnb_attention.so": (["attention_tcgen05.cu"], []),
-    "libnb_serving.so": (["kv_cache.cu", "cached_attention.cu", "cached_attention_tcgen05.cu", "logits.cu", "sample.cu"], []),
+    "libnb_serving.so": (["kv_cache.cu", "cached_attention.cu", "cached_attention_tcgen05.cu", "logits.cu"], []),
+    "libnb_answers.so": (["sample.cu", "shared_prefix.cu", "cached_attention_tcgen05.cu"], ["-DNB_SHARED_PREFIX"]),
     "libnb_heads.so": (["norm_rotary.cu"], []),
     "libnb_comm.so": (["peer_collectives.cu"], []),
     "libnb_runtime.so": (["plan_runtime.cpp"], []),

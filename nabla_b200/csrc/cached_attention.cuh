@@ -4,6 +4,10 @@
 
 namespace nbc {
 
+// What a call of the kernels is: all there is of an attention; or, of one over a prefix that a batch shares (shared_prefix.cu), the keys of the prefix, whose
+// parts are left for the other, or the keys of each sequence's own, which are joined with them.
+enum Role { ALONE, FIRST, SECOND };
+
 struct AttendArgs {
   const void* q;                 // [batch][new][heads][D]
   long long q_sb, q_st, q_sh;        // its strides in elements
@@ -19,6 +23,11 @@ struct AttendArgs {
   // fp32 results of parts, and log2 of the sum of their weights: [splits][batch][kv_heads][new * group] rows, or two tiles of rows for each block
   float *part_o, *part_w;
   int* lines;                    // see attend_few_kernel
+  // FIRST: how many keys the prefix has. (Its rows are those of all sequences, one behind the other, of a batch of one.)
+  Whole limit;
+  // SECOND: parts of the rows, [first_parts][kv_heads][batch * new * group]
+  const float *first_o, *first_w;
+  int first_parts;
 };
 
 // Few rows: a block's warps take steps of STEP keys of its range in turn. The keys of a range, and the row of its block at which the loads of 16 keys start,
@@ -57,6 +66,31 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, int b, int h, int
     __nv_bfloat162 u = __floats2bfloat162_rn(x.x, x.y), w = __floats2bfloat162_rn(x.z, x.w);
     *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<uint32_t*>(&u), *reinterpret_cast<uint32_t*>(&w));
   }
+}
+
+// The result x of a row over its own keys, with log2 of the sum of its weights, joined with what the row has of a shared prefix, in the order of its parts.
+template <typename T, int D, Role ROLE>
+__device__ __forceinline__ void store_result(const AttendArgs& a, int b, int h, int r, int c, float4 x, float weight, bool live) {
+  if constexpr (ROLE == SECOND) {
+    if (live) {
+      const long long rows = (long long)a.fresh * (a.heads / a.kv_heads), at = h * a.batch * rows + b * rows + r, stride = a.kv_heads * a.batch * rows;
+      float top = weight;
+      for (int s = 0; s < a.first_parts; ++s) top = fmaxf(top, a.first_w[at + s * stride]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      float f = exp2f(weight - ref), sum = f;
+      x.x *= f, x.y *= f, x.z *= f, x.w *= f;
+#pragma unroll 4
+      for (int s = 0; s < a.first_parts; ++s) {
+        const float4 y = reinterpret_cast<const float4*>(a.first_o)[(at + s * stride) * (D / 4) + c];
+        f = exp2f(a.first_w[at + s * stride] - ref);
+        sum += f;
+        x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+      }
+      const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // NaN stays
+      x.x *= inverse, x.y *= inverse, x.z *= inverse, x.w *= inverse;
+    }
+  }
+  store_out<T, D>(a, b, h, r, c, x);
 }
 
 template <int D>
@@ -98,7 +132,7 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 __device__ __forceinline__ uint32_t widen(uint32_t biased, uint32_t sel) { return __byte_perm(biased, 0x64646464u, sel); }
 constexpr uint32_t BIAS2 = 0x64806480u;      // 1152 twice
 // Many rows: tiles of 128 rows on the tensor cores (cached_attention_tcgen05.cu), bf16 only.
-template <int D>
+template <int D, Role ROLE>
 cudaError_t launch_many(const AttendArgs& a, int* status, cudaStream_t stream);
 
 }  // namespace nbc

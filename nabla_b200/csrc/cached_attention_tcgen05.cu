@@ -90,7 +90,7 @@ __device__ __forceinline__ float top3(float a, float b, float c) {
   return r;
 }
 
-template <int D>
+template <int D, Role ROLE>
 __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const ManyArgs args) {
   using L = ManySmem<D>;
   const AttendArgs& a = args.a;
@@ -141,9 +141,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
   const int sp = at_ % a.splits;
   at_ /= a.splits;
   const int h = at_ % a.kv_heads, b = at_ / a.kv_heads;
-  const int room = a.table.columns << a.block_log, past = clamp_tokens(a.past.at(b), room);
-  const int count = clamp_tokens(a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
-  const int all_keys = min(room, past + count);
+  const int room = a.table.columns << a.block_log, past = ROLE == FIRST ? 0 : clamp_tokens(a.past.at(b), room);
+  const int count = clamp_tokens(ROLE == FIRST || a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
+  const int all_keys = ROLE == FIRST ? clamp_tokens(a.limit.at(0), room) : min(room, past + count);
   const int row0 = qt * args.q_tiles * BT;
   int n_t[2], first_t[2];          // key tiles of a row tile, the last key that its first row sees
 #pragma unroll
@@ -496,10 +496,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           float4 x = make_float4(__uint_as_float(v[4 * i]) * inverse, __uint_as_float(v[4 * i + 1]) * inverse, __uint_as_float(v[4 * i + 2]) * inverse,
                                  __uint_as_float(v[4 * i + 3]) * inverse);
           if (none) x = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (a.splits > 1) {
+          if (ROLE == FIRST || a.splits > 1) {
             store_part<D>(a, sp, b, h, row, 8 * c + i, x, none ? -INFINITY : m - ROOM + __log2f(l));
           } else {
-            store_out<__nv_bfloat16, D>(a, b, h, row, 8 * c + i, x);
+            store_result<__nv_bfloat16, D, ROLE>(a, b, h, row, 8 * c + i, x, none ? -INFINITY : m - ROOM + __log2f(l), live);
           }
         }
       }
@@ -513,19 +513,27 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
   }
 }
 
-template <int D>
+template <int D, Role ROLE>
 cudaError_t launch_many(const AttendArgs& a, int* status, cudaStream_t stream) {
   ManyArgs args = {a, 2, status};
   const long long rows = (long long)a.fresh * (a.heads / a.kv_heads), pairs = (long long)a.batch * a.kv_heads * a.splits;
   if ((rows + 255) / 256 * pairs < 148) args.q_tiles = 1;
   const long long grid = (rows + args.q_tiles * BT - 1) / (args.q_tiles * BT) * pairs;
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  const cudaError_t e = cudaFuncSetAttribute(attend_many_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ManySmem<D>::TOTAL);
+  const cudaError_t e = cudaFuncSetAttribute(attend_many_kernel<D, ROLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, ManySmem<D>::TOTAL);
   if (e != cudaSuccess) return e;
-  return launch_following(attend_many_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(MANY_THREADS), ManySmem<D>::TOTAL, stream, args);
+  return launch_following(attend_many_kernel<D, ROLE>, dim3(static_cast<unsigned>(grid)), dim3(MANY_THREADS), ManySmem<D>::TOTAL, stream, args);
 }
-template cudaError_t launch_many<64>(const AttendArgs&, int*, cudaStream_t);
-template cudaError_t launch_many<128>(const AttendArgs&, int*, cudaStream_t);
+
+#ifdef NB_SHARED_PREFIX          // built once more for the library that has shared_prefix.cu
+template cudaError_t launch_many<64, FIRST>(const AttendArgs&, int*, cudaStream_t);
+template cudaError_t launch_many<128, FIRST>(const AttendArgs&, int*, cudaStream_t);
+template cudaError_t launch_many<64, SECOND>(const AttendArgs&, int*, cudaStream_t);
+template cudaError_t launch_many<128, SECOND>(const AttendArgs&, int*, cudaStream_t);
+#else
+template cudaError_t launch_many<64, ALONE>(const AttendArgs&, int*, cudaStream_t);
+template cudaError_t launch_many<128, ALONE>(const AttendArgs&, int*, cudaStream_t);
+#endif
 
 }  // namespace nbc
 

@@ -1,4 +1,5 @@
-"""Python wrappers of the serving kernels (``csrc/kv_cache.cu``, ``csrc/cached_attention.cu``, ``csrc/logits.cu``, ``csrc/sample.cu``).
+"""Python wrappers of the serving kernels (``csrc/kv_cache.cu``, ``csrc/cached_attention.cu``, ``csrc/shared_prefix.cu``,
+``csrc/logits.cu``, ``csrc/sample.cu``).
 
 Arguments are torch CUDA tensors whose shapes and types ``ops/serving.py`` has checked; scratch comes from torch's caching allocator.
 ``launch_count`` counts kernel launches issued from here.
@@ -12,31 +13,37 @@ import torch
 
 from . import load, ptr, recorder, status_word, stream_ptr
 
-_lib = None
+_libs: dict = {}
 launch_count = 0
 c_int, c_ll, c_f, c_vp = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
+# of each library: (result, arguments)
+_FUNCTIONS = {
+    "libnb_serving.so": {
+        "nb_kv_write": (c_int, [c_vp] * 9 + [c_int] * 8 + [c_ll] * 6 + [c_int, c_vp]),
+        "nb_kv_read": (c_int, [c_vp] * 9 + [c_int] * 9 + [c_vp]),
+        "nb_cached_attention": (c_int, [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_vp, c_int, c_vp, c_vp]),
+        "nb_cached_attention_scratch": (c_ll, [c_int] * 8),
+        "nb_adjust_logits": (c_int, [c_vp] * 9 + [c_ll, c_vp] + [c_int] * 6 + [c_vp]),
+    },
+    "libnb_answers.so": {
+        "nb_shared_prefix_attention": (c_int, [c_vp] * 11 + [c_int] * 10 + [c_ll] * 3 + [c_f, c_int, c_vp, c_int, c_vp, c_vp]),
+        "nb_shared_prefix_scratch": (c_ll, [c_int] * 9),
+        "nb_shared_prefix_launches": (c_int, [c_int] * 8),
+        "nb_sample_tokens": (c_int, [c_vp] * 7 + [c_int] * 4 + [c_vp]),
+    },
+}
 
 
-def _L():
-    global _lib
-    if _lib is None:
-        lib = load("libnb_serving.so")
-        sig = {
-            "nb_kv_write": [c_vp] * 9 + [c_int] * 8 + [c_ll] * 6 + [c_int, c_vp],
-            "nb_kv_read": [c_vp] * 9 + [c_int] * 9 + [c_vp],
-            "nb_cached_attention": [c_vp] * 9 + [c_int] * 9 + [c_ll] * 3 + [c_f, c_int, c_vp, c_int, c_vp, c_vp],
-            "nb_sample_tokens": [c_vp] * 7 + [c_int] * 4 + [c_vp],
-            "nb_adjust_logits": [c_vp] * 9 + [c_ll, c_vp] + [c_int] * 6 + [c_vp],
-        }
-        for name, args in sig.items():
-            fn = getattr(lib, name)
-            fn.argtypes = args
-            fn.restype = c_int
-        lib.nb_cached_attention_scratch.argtypes = [c_int] * 8
-        lib.nb_cached_attention_scratch.restype = c_ll
-        _lib = lib
+def _L(name: str = "libnb_serving.so"):
+    lib = _libs.get(name)
+    if lib is None:
+        lib = load(name)
+        for f, (result, args) in _FUNCTIONS[name].items():
+            fn = getattr(lib, f)
+            fn.restype, fn.argtypes = result, args
+        _libs[name] = lib
     r = recorder()
-    return _lib if r is None else r.library(_lib)
+    return lib if r is None else r.library(lib)
 
 
 def _ok(rc: int, what: str, launches: int = 1) -> None:
@@ -108,6 +115,33 @@ def _scratch(*sizes: int) -> int:
     return _L().nb_cached_attention_scratch(*sizes)
 
 
+def shared_prefix_attention(q, k_codes, k_scale, v_codes, v_scale, prefix_table, prefix_length, table, past, count, causal: bool, scale: float):
+    _dense(k_codes, k_scale, v_codes, v_scale)
+    q = _rows(q)
+    b, t, hq, d = q.shape
+    if b > 1 and t > 1 and q.stride(0) != t * q.stride(1):          # the rows of a batch are those of one sequence
+        q = q.contiguous()
+    prefix_table, prefix_length, table, past = prefix_table.contiguous(), prefix_length.contiguous(), table.contiguous(), past.contiguous()
+    count = count.contiguous() if count is not None else None
+    blocks, h, n, _ = k_codes.shape
+    out = torch.empty((b, t, hq, d), dtype=q.dtype, device=q.device)
+    fp32 = int(q.dtype == torch.float32)
+    floats, launches = _prefix_scratch(b, t, hq, h, d, n, prefix_table.shape[0], table.shape[1], fp32)
+    part = torch.empty(floats, dtype=torch.float32, device=q.device)
+    _ok(_L("libnb_answers.so").nb_shared_prefix_attention(ptr(q), ptr(k_codes), ptr(k_scale), ptr(v_codes), ptr(v_scale), ptr(out), ptr(prefix_table), ptr(prefix_length),
+                                        ptr(table), ptr(past), ptr(count), _wide(prefix_table, prefix_length, table, past, count), b, t, hq, h, d, n, blocks,
+                                        prefix_table.shape[0], table.shape[1], *q.stride()[:3], float(scale), int(causal), ptr(part), fp32,
+                                        ptr(status_word(q.device)), stream_ptr()), "shared_prefix_attention", launches)
+    return out
+
+
+@functools.lru_cache(1024)
+def _prefix_scratch(b, t, hq, h, d, n, prefix_columns, columns, fp32):
+    """Floats of scratch and launches, functions of the sizes alone."""
+    floats = _L("libnb_answers.so").nb_shared_prefix_scratch(b, t, hq, h, d, n, prefix_columns, columns, fp32)
+    return floats, _L("libnb_answers.so").nb_shared_prefix_launches(b, t, hq, h, d, n, columns, fp32)
+
+
 def adjust_logits(logits, history, length, prompt, repetition, presence, frequency, bias, allowed):
     vocab = logits.shape[-1]
     x = logits.contiguous()
@@ -130,6 +164,6 @@ def sample_tokens(logits, uniform, temperature, top_k, top_p, min_p):
     x = logits if logits.is_contiguous() else logits.contiguous()
     uniform, temperature, top_k, top_p, min_p = (t.contiguous() if t is not None else None for t in (uniform, temperature, top_k, top_p, min_p))
     out = torch.empty(x.shape[0], dtype=torch.int64, device=x.device)
-    _ok(_L().nb_sample_tokens(ptr(x), ptr(uniform), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), ptr(out), _wide(top_k), x.shape[0], x.shape[1],
+    _ok(_L("libnb_answers.so").nb_sample_tokens(ptr(x), ptr(uniform), ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), ptr(out), _wide(top_k), x.shape[0], x.shape[1],
                               int(x.dtype == torch.float32), stream_ptr()), "sample_tokens")
     return out

@@ -6,8 +6,8 @@ columns) of whole numbers: position t of sequence b lies in row ``t % block_size
 no block (negative, or not below the number of blocks) is a place without tokens: writes to it are dropped, reads give zeros, attention
 sees no key there. Sequences may share blocks that are only read; a block that a call writes belongs to one sequence.
 
-Each is one ``Operation`` with hand-written kernels on CUDA (``csrc/kv_cache.cu``, ``cached_attention.cu``, ``logits.cu``,
-``sample.cu``) and an equivalent torch expression on the CPU. They have no derivatives. On a mesh the heads of the cache may be split as those of the model are.
+Each is one ``Operation`` with hand-written kernels on CUDA (``csrc/kv_cache.cu``, ``cached_attention.cu``, ``shared_prefix.cu``,
+``logits.cu``, ``sample.cu``) and an equivalent torch expression on the CPU. They have no derivatives. On a mesh the heads of the cache may be split as those of the model are.
 """
 from __future__ import annotations
 
@@ -133,6 +133,24 @@ class KVCacheReadOp(Operation):
 
 
 # ================================================================ attention
+def _softmax_over(q, k, v, seen, scale: float):
+    """softmax(scale * q k^T) v over the keys that are seen (batch, new, keys), zeros where there are none."""
+    b, t, hq, d = q.shape
+    h = k.shape[2]
+    s = torch.einsum("bthgd,bkhd->bhgtk", q.float().reshape(b, t, h, hq // h, d), k) * scale
+    s = torch.where(seen[:, None, None], s, float("-inf"))
+    top = s.amax(-1, keepdim=True)
+    p = torch.exp(s - torch.where(top == float("-inf"), 0.0, top))
+    p = torch.where(seen[:, None, None], p, 0.0)
+    total = p.sum(-1, keepdim=True)
+    # what a row does not see may be anything, what it sees and is not finite (all that a block holds for a head) makes it NaN
+    fine = torch.isfinite(v).all(-1)
+    o = torch.einsum("bhgtk,bkhd->bthgd", p / torch.where(total == 0, 1.0, total), torch.where(fine[..., None], v, 0.0))
+    reached = torch.einsum("btk,bkh->bth", seen.float(), (~fine).float()) > 0
+    o = torch.where(reached[..., None, None], float("nan"), o)
+    return o.reshape(b, t, hq, d).to(q.dtype)
+
+
 class CachedAttentionOp(Operation):
     """softmax(scale * q k^T) v over the keys and values of a cache, (batch, new, heads, head_dim) as ``q``."""
 
@@ -154,18 +172,7 @@ class CachedAttentionOp(Operation):
         i = torch.arange(t, device=q.device)
         last = past[:, None] + i if causal else (past + count - 1)[:, None].expand(b, t)
         seen = (torch.arange(k.shape[1], device=q.device) <= last[..., None]) & (i < count[:, None])[..., None] & there[:, None]
-        s = torch.einsum("bthgd,bkhd->bhgtk", q.float().reshape(b, t, h, hq // h, d), k) * scale
-        s = torch.where(seen[:, None, None], s, float("-inf"))
-        top = s.amax(-1, keepdim=True)
-        p = torch.exp(s - torch.where(top == float("-inf"), 0.0, top))
-        p = torch.where(seen[:, None, None], p, 0.0)
-        total = p.sum(-1, keepdim=True)
-        # what a row does not see may be anything, what it sees and is not finite (all that a block holds for a head) makes it NaN
-        fine = torch.isfinite(v).all(-1)
-        o = torch.einsum("bhgtk,bkhd->bthgd", p / torch.where(total == 0, 1.0, total), torch.where(fine[..., None], v, 0.0))
-        reached = torch.einsum("btk,bkh->bth", seen.float(), (~fine).float()) > 0
-        o = torch.where(reached[..., None, None], float("nan"), o)
-        return o.reshape(b, t, hq, d).to(q.dtype)
+        return _softmax_over(q, k, v, seen, scale)
 
     def sharding_rule(self, input_shapes, output_shapes, **kw):
         codes, scale = {0: ["bcast_blocks"], 1: ["h"], 2: ["bcast_n"], 3: ["bcast_d"]}, {0: ["bcast_blocks"], 1: ["h"]}
@@ -176,6 +183,39 @@ class CachedAttentionOp(Operation):
     def compute_cost(self, input_shapes, output_shapes) -> float:
         b, t, h, d = (int(n) for n in input_shapes[0])
         return 4.0 * b * t * h * d * int(input_shapes[5][1]) * int(input_shapes[1][2])
+
+
+class SharedPrefixAttentionOp(Operation):
+    """``CachedAttentionOp`` over sequences that all begin with the tokens of one prefix, (batch, new, heads, head_dim) as ``q``."""
+
+    def kernel(self, q, k_codes, k_scale, v_codes, v_scale, prefix_table, prefix_length, table, past, count=None, *, causal: bool = True, scale: float):
+        if q.device.type == "meta" or not q.numel():
+            return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if _runs_native(q):
+            from ..native import serving
+
+            return serving.shared_prefix_attention(q, k_codes, k_scale, v_codes, v_scale, prefix_table, prefix_length, table, past, count, causal, scale)
+        b, t, hq, d = q.shape
+        blocks, h, n, _ = k_codes.shape
+        shared, own = prefix_table.shape[0] * n, table.shape[1] * n
+        tables = torch.cat([prefix_table.long().expand(b, -1), table.long()], 1)
+        at, there = _blocks_of(tables, torch.arange(tables.shape[1], device=q.device).expand(b, -1), blocks)
+        k, v = ((c[at].float() * s[at][..., None, None]).transpose(2, 3).reshape(b, -1, h, d) for c, s in ((k_codes, k_scale), (v_codes, v_scale)))
+        there = there.repeat_interleave(n, 1)
+        past = past.long().clamp(0, own)
+        count = _live(count, t, past)
+        i = torch.arange(t, device=q.device)
+        last = past[:, None] + i if causal else (past + count - 1)[:, None].expand(b, t)
+        seen = torch.cat([(torch.arange(shared, device=q.device) < prefix_length.long()).expand(b, t, shared),
+                          torch.arange(own, device=q.device) <= last[..., None]], -1)
+        return _softmax_over(q, k, v, seen & (i < count[:, None])[..., None] & there[:, None], scale)
+
+    def sharding_rule(self, input_shapes, output_shapes, **kw):
+        return _attend.sharding_rule(input_shapes, output_shapes)
+
+    def compute_cost(self, input_shapes, output_shapes) -> float:
+        b, t, h, d = (int(n) for n in input_shapes[0])
+        return 4.0 * b * t * h * d * (int(input_shapes[5][0]) + int(input_shapes[7][1])) * int(input_shapes[1][2])
 
 
 # ================================================================ logits
@@ -274,7 +314,8 @@ class SampleTokensOp(Operation):
         return OpShardingRule([{0: ["b"], 1: ["bcast_v"]}] + [{0: ["b"]} for _ in input_shapes[1:]], [{0: ["b"]}])
 
 
-_write, _read, _attend, _adjust, _sample = KVCacheWriteOp(), KVCacheReadOp(), CachedAttentionOp(), AdjustLogitsOp(), SampleTokensOp()
+_write, _read, _attend, _prefixed = KVCacheWriteOp(), KVCacheReadOp(), CachedAttentionOp(), SharedPrefixAttentionOp()
+_adjust, _sample = AdjustLogitsOp(), SampleTokensOp()
 
 
 # ---------------------------------------------------------------- checks of arguments
@@ -411,6 +452,31 @@ def cached_attention(q: Tensor, cache: dict[str, Tensor], block_table: Tensor, p
     more = () if count is None else (count,)
     _same_device(q, *parts, block_table, past, *more)
     return _now((_attend(q, *parts, block_table, past, *more, causal=bool(causal), scale=scale),))[0]
+
+
+def shared_prefix_attention(q: Tensor, cache: dict[str, Tensor], prefix_table: Tensor, prefix_length: Tensor, block_table: Tensor, past: Tensor,
+                            count: Tensor | None = None, *, causal: bool = True, scale: float | None = None) -> Tensor:
+    """``cached_attention`` for a batch whose sequences all begin with the same tokens, which lie in the cache once and are read once for all.
+
+    ``prefix_table`` (columns,) names the blocks of the prefix, ``prefix_length`` (1,) says how many tokens it has: every query sees all of them, with or
+    without ``causal``. ``block_table`` (batch, columns), ``past`` and ``count`` describe what each sequence has behind the prefix, as ``kv_cache_write``
+    and ``cached_attention`` take them: token ``past + i`` of a sequence is the ``prefix_length + past + i``-th of the text. The prefix need not end with
+    a block. Queries from ``count`` on are zeros, a prefix of no tokens leaves what ``cached_attention`` gives."""
+    parts, (blocks, heads, n, d) = _cache(cache)
+    _tensor(q, "q", _FLOATS, (None, None, None, d))
+    batch, new, hq, _ = _shape(q)
+    _need(hq >= heads and hq % heads == 0, f"{hq} query heads cannot share {heads} heads of the cache evenly")
+    _need(batch * new * hq < 1 << 31, "fewer than 2^31 rows of queries")
+    _tensor(prefix_table, "prefix_table", _WHOLE, (None,))
+    _need(_shape(prefix_table)[0] >= 1, "prefix_table has no columns")
+    _need(_shape(prefix_table)[0] * n < 1 << 30, "a prefix has fewer than 2^30 positions")
+    _tensor(prefix_length, "prefix_length", _WHOLE, (1,))
+    _places(block_table, past, count, batch, "past", n)
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    _need(scale > 0 and math.isfinite(scale), "scale has to be positive")
+    more = () if count is None else (count,)
+    _same_device(q, *parts, prefix_table, prefix_length, block_table, past, *more)
+    return _now((_prefixed(q, *parts, prefix_table, prefix_length, block_table, past, *more, causal=bool(causal), scale=scale),))[0]
 
 
 def adjust_logits(logits: Tensor, history: Tensor | None = None, length: Tensor | None = None, prompt_length: Tensor | None = None, *,

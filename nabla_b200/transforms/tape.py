@@ -25,10 +25,11 @@ LAUNCHES = frozenset("""nb_gemm_bf16 nb_gemm_dual_bf16 nb_attn_fwd nb_attn_bwd n
     nb_lse_pick_fwd nb_lse_pick_bwd nb_adamw nb_adamw_group nb_adam_hyper nb_mean_diff nb_sgd nb_embedding_gather nb_embedding_scatter_add
     nb_cast nb_activation nb_nf4_dequant nb_nf4_dequant_codes nb_pool2d_fwd nb_pool2d_bwd nb_pool2d_select nb_conv2d_direct nb_conv_flip
     nb_conv2d_wgrad_direct nb_sgemm nb_sum_slices nb_binary nb_unary nb_reduce nb_cumsum nb_kv_write nb_kv_read nb_cached_attention
-    nb_adjust_logits nb_sample_tokens nb_norm_rotary""".split())
+    nb_adjust_logits nb_sample_tokens nb_shared_prefix_attention nb_norm_rotary""".split())
 # functions of sizes alone
 QUERIES = frozenset("""nb_layernorm_bwd_nblocks nb_colsum_nparts nb_conv2d_wgrad_slices nb_sgemm_slices nb_reduce_splits
-    nb_embedding_scatter_work nb_cached_attention_scratch nb_norm_rotary_scratch""".split())
+    nb_embedding_scatter_work nb_cached_attention_scratch nb_norm_rotary_scratch
+    nb_shared_prefix_scratch nb_shared_prefix_launches""".split())
 # switches that the wrappers read on every call
 ENVIRONMENT = ("NABLA_B200_DISABLE_NATIVE", "NABLA_B200_ATTENTION", "NABLA_B200_ATTENTION_BWD", "NABLA_B200_ELEMENTWISE", "NABLA_B200_LN_BWD",
                "NABLA_B200_OPTIMIZER_STREAM", "NABLA_B200_TAPE")
