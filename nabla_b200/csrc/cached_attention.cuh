@@ -68,23 +68,45 @@ __device__ __forceinline__ void store_out(const AttendArgs& a, int b, int h, int
   }
 }
 
-// The result x of a row over its own keys, with log2 of the sum of its weights, joined with what the row has of a shared prefix, in the order of its parts.
+// Numbers that the launch ahead has left: read when the program says so, neither earlier nor one after the other.
+__device__ __forceinline__ float4 left4(const float* p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+// The result x of a row over its own keys, with log2 of the sum of its weights, joined with what the row has of a shared prefix: its parts in their order,
+// sixteen under way at once, against the largest weight of the sixteens so far.
 template <typename T, int D, Role ROLE>
 __device__ __forceinline__ void store_result(const AttendArgs& a, int b, int h, int r, int c, float4 x, float weight, bool live) {
   if constexpr (ROLE == SECOND) {
     if (live) {
+      constexpr int AHEAD = 16;
       const long long rows = (long long)a.fresh * (a.heads / a.kv_heads), at = h * a.batch * rows + b * rows + r, stride = a.kv_heads * a.batch * rows;
-      float top = weight;
-      for (int s = 0; s < a.first_parts; ++s) top = fmaxf(top, a.first_w[at + s * stride]);
-      const float ref = top == -INFINITY ? 0.f : top;
-      float f = exp2f(weight - ref), sum = f;
-      x.x *= f, x.y *= f, x.z *= f, x.w *= f;
-#pragma unroll 4
-      for (int s = 0; s < a.first_parts; ++s) {
-        const float4 y = reinterpret_cast<const float4*>(a.first_o)[(at + s * stride) * (D / 4) + c];
-        f = exp2f(a.first_w[at + s * stride] - ref);
-        sum += f;
-        x.x = fmaf(f, y.x, x.x), x.y = fmaf(f, y.y, x.y), x.z = fmaf(f, y.z, x.z), x.w = fmaf(f, y.w, x.w);
+      float top = weight, sum = weight == -INFINITY ? 0.f : 1.f;
+      for (int s0 = 0; s0 < a.first_parts; s0 += AHEAD) {
+        float w[AHEAD];
+        float4 y[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          // (those behind the last are the last again, without a weight: loads have no condition)
+          const long long from = at + min(s0 + k, a.first_parts - 1) * stride;
+          w[k] = scale_at(a.first_w, from), y[k] = left4(a.first_o + (from * (D / 4) + c) * 4);
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+          if (s0 + k >= a.first_parts) w[k] = -INFINITY, y[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        float now = top;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) now = fmaxf(now, w[k]);
+        const float ref = now == -INFINITY ? 0.f : now, f = exp2f(top - ref);
+        if (top != -INFINITY) sum *= f, x.x *= f, x.y *= f, x.z *= f, x.w *= f;
+        top = now;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const float e = exp2f(w[k] - ref);
+          sum += e;
+          x.x = fmaf(e, y[k].x, x.x), x.y = fmaf(e, y[k].y, x.y), x.z = fmaf(e, y[k].z, x.z), x.w = fmaf(e, y[k].w, x.w);
+        }
       }
       const float inverse = sum == 0.f ? 0.f : 1.f / sum;      // NaN stays
       x.x *= inverse, x.y *= inverse, x.z *= inverse, x.w *= inverse;
@@ -93,9 +115,12 @@ __device__ __forceinline__ void store_result(const AttendArgs& a, int b, int h, 
   store_out<T, D>(a, b, h, r, c, x);
 }
 
+__device__ __forceinline__ long long part_of(const AttendArgs& a, int part, int b, int h, int r) {
+  return (((long long)part * a.batch + b) * a.kv_heads + h) * a.fresh * (a.heads / a.kv_heads) + r;
+}
 template <int D>
 __device__ __forceinline__ void store_part(const AttendArgs& a, int part, int b, int h, int r, int c, float4 x, float weight) {
-  const long long at = (((long long)part * a.batch + b) * a.kv_heads + h) * a.fresh * (a.heads / a.kv_heads) + r;
+  const long long at = part_of(a, part, b, h, r);
   reinterpret_cast<float4*>(a.part_o)[at * (D / 4) + c] = x;
   if (c == 0) a.part_w[at] = weight;
 }

@@ -280,34 +280,51 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
     float row_mul = 0.f, offset = 0.f;
     if (n > 0) {
       // the row as 16-bit floats, its largest brought to [2^8, 2^9) by a power of two; its 128 bytes of 64 numbers lie in turned 16-byte pieces
-      const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + b * a.q_sb + (long long)token * a.q_st + (long long)(h * group + row % group) * a.q_sh;
-      float top = 0.f;
-      if (live)
+      // D / 8 lanes read a row together (a lane for each row costs an access 32 lines); then every thread sums its own row up
+      constexpr int LANES = D / 8, ROWS = 32 / LANES;
+      // (dead rows read the call's first: loads have no condition, behind one each would be waited for)
+      const long long from = live ? b * a.q_sb + (long long)token * a.q_st + (long long)(h * group + row % group) * a.q_sh : 0;
+      const uint32_t lives = __ballot_sync(0xffffffffu, live);
+      const uint32_t tile = smem_u32(smem + L::Q + t * L::TILE);
+      const int piece = lane % LANES;
+      Eight<__nv_bfloat16> x[LANES];
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          float x[8];
-          load8(q + 8 * c, x);
+      for (int j = 0; j < LANES; ++j) {
+        const long long at = __shfl_sync(0xffffffffu, from, ROWS * j + lane / LANES);
+        x[j].load(static_cast<const __nv_bfloat16*>(a.q) + at + 8 * piece);
+      }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
-        }
-      int ex = static_cast<int>(__float_as_uint(top) >> 23) - 127;
-      ex = ex == 128 || top == 0.f ? 8 : max(ex, -110);
-      const float up = __uint_as_float(static_cast<uint32_t>(127 + (8 - ex)) << 23);
-      row_mul = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - (8 - ex)) << 23);
-      const uint32_t to = smem_u32(smem + L::Q + t * L::TILE) + r * 128;
-      float sum = 0.f;
+      for (int j = 0; j < LANES; ++j) {
+        if (!(lives >> (ROWS * j + lane / LANES) & 1)) x[j].clear();
+        uint32_t most = x[j].top();
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (live) load8(q + 8 * c, x);
+        for (int w = 1; w < LANES; w <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, w));
+        const float top = __uint_as_float(most);
+        int ex = static_cast<int>(most >> 23) - 127;
+        ex = ex == 128 || top == 0.f ? 8 : max(ex, -110);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + (8 - ex)) << 23);
+        const float back = __shfl_sync(0xffffffffu, a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - (8 - ex)) << 23), lane % ROWS * LANES);
+        if (lane / ROWS == j) row_mul = back;
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          w[e] = pack_half2(x[2 * e] * up, x[2 * e + 1] * up);
+          const float2 y = x[j].pair(e);
+          w[e] = pack_half2(y.x * up, y.y * up);
+        }
+        const int i = wq * 32 + ROWS * j + lane / LANES;
+        sts16(tile + (piece >> 3) * (BT * 128) + i * 128 + (((piece & 7) ^ (i & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
+      }
+      __syncwarp();
+      float sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const uint4 y = *reinterpret_cast<const uint4*>(smem + L::Q + t * L::TILE + (c >> 3) * (BT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+        const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
           const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
           sum += f.x + f.y;
         }
-        sts16(to + (c >> 3) * (BT * 128) + (((c & 7) ^ (r & 7)) << 4), make_uint4(w[0], w[1], w[2], w[3]));
       }
       offset = 1152.f * sum;
       fence_proxy_async_smem();
@@ -469,6 +486,18 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
       tc_fence_before();
       mbar_arrive(&p_full[t]);
     }
+    // SECOND: the row's parts of the prefix join here. The first part's first columns are on their way while the last product is waited for
+    const bool joins = ROLE == SECOND && a.splits == 1, none = l == 0.f || !live;
+    const int first = row - lane + (lane >> 3);                // of the rows that this lane stores, eight lanes to a row: first, first + 4, ...
+    const long long row_parts = (long long)a.kv_heads * a.batch * rows, part = (long long)h * a.batch * rows + (long long)b * rows;
+    const int left_rows = min(rows, count * group) - first;    // (those from there on read the call's first row: loads have no condition)
+    const float* left = a.first_o + (left_rows > 0 ? part + first : 0) * D + 4 * (lane & 7);
+    float4 y[8];
+    auto get = [&](int s, int c) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = left4(left + s * row_parts * D + 32 * c + (4 * j < left_rows ? 4 * j : 0) * D);
+    };
+    if (joins && t < args.q_tiles) get(0, 0);
     if (ok && n > 0) {
       if (!mbar_wait(&o_done[t], 0)) {
         atomicExch(args.status, NB_ERR_TIMEOUT_EPILOGUE);
@@ -478,31 +507,73 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
     }
     if (ok && t < args.q_tiles) {
       tc_fence_after();
-      const bool none = l == 0.f || !live;
-      const float inverse = none ? 0.f : 1.f / l;
+      const float weight = none ? -INFINITY : m - ROOM + __log2f(l);
+      float inverse = none ? 0.f : 1.f / l, ref = 0.f, over = 1.f, share = 0.f;        // joins: the reference of all, one over the sum of all weights
+      if (joins && live) {
+        float top = weight;
+        for (int s = 0; s < a.first_parts; ++s) top = fmaxf(top, scale_at(a.first_w, part + row + s * row_parts));
+        ref = top == -INFINITY ? 0.f : top;
+        const float own = exp2f(weight - ref);
+        float sum = own;
+        for (int s = 0; s < a.first_parts; ++s) sum += exp2f(scale_at(a.first_w, part + row + s * row_parts) - ref);
+        over = sum == 0.f ? 0.f : 1.f / sum;          // NaN stays
+        inverse *= own * over;
+        share = exp2f(scale_at(a.first_w, part + row) - ref) * over;
+      }
+      // 32 columns at a time, turned in shared memory (the group's queries have been read for the last time) so that eight lanes read and write a row's
+      // 128 bytes together
+      float4* turned = reinterpret_cast<float4*>(smem + L::Q + t * L::TILE) + wq * 256;
+      const long long out_at = row < rows ? ((((long long)b * a.fresh + token) * a.heads + h * group + row % group) * D) : 0;
+      long long outs[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) outs[j] = __shfl_sync(0xffffffffu, out_at, 4 * j + (lane >> 3)) + 4 * (lane & 7);
+      float4* parts = reinterpret_cast<float4*>(a.part_o) + part_of(a, sp, b, h, first) * (D / 4) + (lane & 7);
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t v[32];
         if (n > 0) {
           tmem_ld_32x32(t_o + c * 32, v);
           tmem_ld_wait_regs(v);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0;
         }
-        if (row >= rows) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float4 x = make_float4(__uint_as_float(v[4 * i]) * inverse, __uint_as_float(v[4 * i + 1]) * inverse, __uint_as_float(v[4 * i + 2]) * inverse,
-                                 __uint_as_float(v[4 * i + 3]) * inverse);
-          if (none) x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < 8; ++i)
+          turned[lane * 8 + (i ^ (lane & 7))] = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                     : make_float4(__uint_as_float(v[4 * i]) * inverse, __uint_as_float(v[4 * i + 1]) * inverse,
+                                                                   __uint_as_float(v[4 * i + 2]) * inverse, __uint_as_float(v[4 * i + 3]) * inverse);
+        __syncwarp();
+        float4 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = turned[(4 * j + (lane >> 3)) * 8 + ((lane ^ (4 * j + (lane >> 3))) & 7)];
+        __syncwarp();
+        if (joins) {
+          for (int s = 0; s < a.first_parts; ++s) {
+            float mine = share;
+            if (s > 0) {
+              get(s, c);
+              mine = live ? exp2f(scale_at(a.first_w, part + row + s * row_parts) - ref) * over : 0.f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float f = __shfl_sync(0xffffffffu, mine, 4 * j + (lane >> 3));
+              if (4 * j >= left_rows) continue;
+              x[j].x = fmaf(f, y[j].x, x[j].x), x[j].y = fmaf(f, y[j].y, x[j].y), x[j].z = fmaf(f, y[j].z, x[j].z), x[j].w = fmaf(f, y[j].w, x[j].w);
+            }
+          }
+          if (c + 1 < D / 32) get(0, c + 1);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (first + 4 * j >= rows || !NB_IN_BOUNDS(NB_SITE_CACHE_ROW, first + 4 * j, a.fresh * group)) continue;
           if (ROLE == FIRST || a.splits > 1) {
-            store_part<D>(a, sp, b, h, row, 8 * c + i, x, none ? -INFINITY : m - ROOM + __log2f(l));
+            parts[j * D + 8 * c] = x[j];
           } else {
-            store_result<__nv_bfloat16, D, ROLE>(a, b, h, row, 8 * c + i, x, none ? -INFINITY : m - ROOM + __log2f(l), live);
+            const __nv_bfloat162 u = __floats2bfloat162_rn(x[j].x, x[j].y), w = __floats2bfloat162_rn(x[j].z, x[j].w);
+            *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + outs[j] + 32 * c) =
+                make_uint2(*reinterpret_cast<const uint32_t*>(&u), *reinterpret_cast<const uint32_t*>(&w));
           }
         }
       }
+      if ((ROLE == FIRST || a.splits > 1) && row < rows) a.part_w[part_of(a, sp, b, h, row)] = weight;
     }
   }
   tc_fence_before();
