@@ -52,14 +52,15 @@ enum Share { ONE, CLUSTER, FLAT };
 constexpr int UNIT = FEW_WARPS * STEP, FLAT_BATCH = 1024;      // keys that a line is cut in multiples of; sequences that FLAT takes
 
 // lines[b] = units of sequences in front of b, for b up to the batch, in shared memory. All threads.
+template <bool PAST>
 __device__ __forceinline__ void number_lines(const AttendArgs& a, int tiles, int* lines) {
   __shared__ int sums[FEW_WARPS];
   const int each = (a.batch + 32 * FEW_WARPS - 1) / (32 * FEW_WARPS), b0 = min(a.batch, static_cast<int>(threadIdx.x) * each), b1 = min(a.batch, b0 + each);
   const int room = a.table.columns << a.block_log;
   int own = 0;
   for (int b = b0; b < b1; ++b) {
-    const int count = clamp_tokens(a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
-    const int keys = count == 0 ? 0 : min(room, clamp_tokens(a.past.at(b), room) + count);
+    const int count = clamp_tokens(a.count.p == nullptr ? a.fresh : a.count.at<PAST>(b), a.fresh);
+    const int keys = count == 0 ? 0 : min(room, clamp_tokens(a.past.at<PAST>(b), room) + count);
     const int units = (keys + UNIT - 1) / UNIT * a.kv_heads * tiles;
     lines[b + 1] = units;
     own += units;
@@ -85,13 +86,15 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   constexpr bool EXACT = sizeof(T) == 4;              // fp32: two parts, codes less their offset before the product
   constexpr int PARTS = EXACT ? 2 : 1, KSTEPS = D / 16, PIECES = D / 64, MT = D / 16, ROWS = 8 * RT;
   extern __shared__ __align__(16) uint8_t smem[];
-  follow_grid();
+  // SECOND works while the prefix is still being worked on, and waits before it stores (launch.cuh says on what grounds): what it reads until then goes past L1
+  constexpr bool PAST = ROLE == SECOND;
+  if (!PAST) follow_grid();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int group = a.heads / a.kv_heads, tiles = (a.fresh * group + ROWS - 1) / ROWS;
   int sp = 0, h = 0, tile = 0, b = 0, line_from = 0, line_to = 0, line = 0;
   int* lines = reinterpret_cast<int*>(smem) + Few<D, RT>::SMEM / 4;
   if (SHARE == FLAT) {
-    number_lines(a, tiles, lines);
+    number_lines<PAST>(a, tiles, lines);
     const int all = lines[a.batch];
     // no more blocks than units, so that each has one: the joining kernel reads what every block between a line's first and last has written
     const int blocks = min(static_cast<int>(gridDim.x), all), c = blockIdx.x;
@@ -119,8 +122,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
     slot = piece == units ? -1 : 2 * static_cast<int>(blockIdx.x) + (unit0 == 0 ? 1 : 0);
     line += piece;
   }
-  const int room = a.table.columns << a.block_log, past = ROLE == FIRST ? 0 : clamp_tokens(a.past.at(b), room);
-  const int count = clamp_tokens(ROLE == FIRST || a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
+  const int room = a.table.columns << a.block_log, past = ROLE == FIRST ? 0 : clamp_tokens(a.past.at<PAST>(b), room);
+  const int count = clamp_tokens(ROLE == FIRST || a.count.p == nullptr ? a.fresh : a.count.at<PAST>(b), a.fresh);
   const int row0 = tile * ROWS, rows = min(ROWS, a.fresh * group - row0);       // row r: token r / group, head r % group
   const int live = min(rows, count * group - row0);                             // rows from here on are zero
   // keys that the last row sees
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   struct Place { int id[2], there; };
   auto find = [&](int step) {
     const int at = key_of(range, warp, mine, step);
-    const int x = a.table.block(b, min(at, last_key) >> a.block_log), y = n == 16 ? a.table.block(b, min(at + 16, last_key) >> a.block_log) : x;
+    const int x = a.table.block<PAST>(b, min(at, last_key) >> a.block_log), y = n == 16 ? a.table.block<PAST>(b, min(at + 16, last_key) >> a.block_log) : x;
     const Place p = {{max(x, 0), max(y, 0)}, (x >= 0 ? 1 : 0) | (y >= 0 && at + 16 < k1 ? 2 : 0)};
     return p;
   };
@@ -154,8 +157,8 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int c = 0; c < PIECES; ++c) kr[i][u][c] = ldg16(at + u * 8 * D + c * 64);
-      ks[i] = scale_at(a.scales[0], unit(p, i));
+        for (int c = 0; c < PIECES; ++c) kr[i][u][c] = ldg16<PAST>(at + u * 8 * D + c * 64);
+      ks[i] = scale_at<PAST>(a.scales[0], unit(p, i));
     }
   };
   auto get_values = [&](const Place& p, int step) {
@@ -167,9 +170,9 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
       for (int r = 0; r < 4; ++r) {
         const int8_t* codes = at + ((r & 1) + 8 * (r >> 1)) * D;
         if (D == 128) {
-          vr[i][r] = ldg16(codes);
+          vr[i][r] = ldg16<PAST>(codes);
         } else {
-          const uint2 x = ldg8(codes);
+          const uint2 x = ldg8<PAST>(codes);
           vr[i][r].x = x.x, vr[i][r].y = x.y;
         }
       }
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   get_values(now, 0);
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    vs[i] = scale_at(a.scales[1], unit(now, i));
+    vs[i] = scale_at<PAST>(a.scales[1], unit(now, i));
   Place next = find(1);
 
   // ---- queries as the small operand: lane (g, t) holds dims 16 (t + 4 p) + 4 s + {0, 1} and {2, 3} of row g for k-step 4 p + s
@@ -197,7 +200,9 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         float y[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (8 * u + g < live) load8(q + 16 * (t + 4 * p) + 8 * w, y);
+        if (8 * u + g < live) {
+          if constexpr (PAST) load8_past(q + 16 * (t + 4 * p) + 8 * w, y); else load8(q + 16 * (t + 4 * p) + 8 * w, y);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[4 * p + 2 * w + e / 4][e % 4] = y[e], top = fmaxf(top, fabsf(y[e]));
       }
@@ -375,7 +380,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
     get_values(next, step + 1);
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      vs[i] = scale_at(a.scales[1], unit(next, i));
+      vs[i] = scale_at<PAST>(a.scales[1], unit(next, i));
     now = next;
     next = find(step + 2);
   }
@@ -403,6 +408,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
           so[warp * ROWS * (D / 4) + out_at<D>(row, g * (D / 32) + c)] =
               make_float4(o[u][2 * c][r], o[u][2 * c][2 + r], o[u][2 * c + 1][r], o[u][2 * c + 1][2 + r]);
     }
+  if (PAST) follow_grid();
   __syncthreads();
   constexpr int PER = ROWS * (D / 4) / (32 * FEW_WARPS);
 #pragma unroll
@@ -463,6 +469,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   if (SHARE != FLAT) break;
   __syncthreads();                                    // before the next piece's results
   }
+  if (PAST && SHARE == FLAT) follow_grid();             // also of a block that has no share
 }
 
 // Joins the parts of each row in their order: those of ranges of keys (tiles of 128 rows), or of the pieces of a line (FLAT). One block per row; side s of its

@@ -21,9 +21,19 @@ constexpr float LEAST_SCALE = 7.888609052210118e-31f;      // 2^-100: its recipr
 struct Whole {
   const void* p;
   int wide;
+  // PAST: past L1, for a kernel that reads before it has waited for the grid ahead (launch.cuh)
+  template <bool PAST = false>
   __device__ __forceinline__ long long at(long long i) const {
     long long v;
     int w;
+    if (PAST) {
+      if (wide) {
+        asm volatile("ld.global.cg.s64 %0, [%1];" : "=l"(v) : "l"(static_cast<const long long*>(p) + i));
+        return v;
+      }
+      asm volatile("ld.global.cg.s32 %0, [%1];" : "=r"(w) : "l"(static_cast<const int*>(p) + i));
+      return w;
+    }
     if (wide) {
       asm volatile("ld.global.s64 %0, [%1];" : "=l"(v) : "l"(static_cast<const long long*>(p) + i));      // volatile: behind the wait for the grid ahead
       return v;
@@ -52,8 +62,13 @@ __device__ __forceinline__ void several(const Whole& w, long long base, int i, i
     }
   }
 }
+template <bool PAST = false>
 __device__ __forceinline__ float scale_at(const float* p, long long i) {
   float v;
+  if (PAST) {
+    asm volatile("ld.global.cg.f32 %0, [%1];" : "=f"(v) : "l"(p + i));
+    return v;
+  }
   asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p + i));
   return v;
 }
@@ -62,9 +77,10 @@ struct Table {
   Whole ids;          // [batch][columns]
   int columns;
   int blocks;         // of the cache
+  template <bool PAST = false>
   __device__ __forceinline__ int block(int b, int column) const {      // -1: none
     if (column >= columns || column < 0) return -1;
-    const long long id = ids.at((long long)b * columns + column);
+    const long long id = ids.at<PAST>((long long)b * columns + column);
     return id >= 0 && id < blocks ? static_cast<int>(id) : -1;
   }
 };
@@ -89,15 +105,29 @@ __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, flo
     x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
   }
 }
+template <typename T>
+__device__ __forceinline__ void load8_past(const T* p, float (&x)[8]) {          // past L1
+  constexpr int WORDS = 2 * static_cast<int>(sizeof(T));
+  uint32_t w[WORDS];
+#pragma unroll
+  for (int i = 0; i < WORDS; i += 4)
+    asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "l"(reinterpret_cast<const uint32_t*>(p) + i));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(sizeof(T) == 4 ? w[i & (WORDS - 1)] : i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+}
 // Codes are read once by a block, past L1. (The address comes from the table, so these cannot move ahead of the wait for the grid ahead.)
+template <bool PAST = false>
 __device__ __forceinline__ uint4 ldg16(const void* p) {
   uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  if (PAST) asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  else asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
+template <bool PAST = false>
 __device__ __forceinline__ uint2 ldg8(const void* p) {
   uint2 v;
-  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  if (PAST) asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  else asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
 

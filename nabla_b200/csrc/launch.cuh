@@ -16,7 +16,7 @@
 //  - only then does it let the next launch begin, so no more than two grids of a stream are on the chip. A kernel that takes
 //    tensor memory has it by then: a waiting block may wait for the tensor memory of a running one, never the other way.
 //  - a kernel without follow_grid() is launched with <<< >>> and waits for the end of all that is ahead of it, as before.
-// Two exceptions, and what they rest on:
+// Three exceptions, and what they rest on:
 //  - kernels with bounded waits look at the device's status word while they set up, half a microsecond that a launch would otherwise
 //    pay behind its wait. They see it as of then: the launch right behind one whose wait ran out may still start, and meets the limits
 //    of its own waits; the one behind it leaves. Nothing else follows from the word on the device.
@@ -24,6 +24,9 @@
 //    writes nothing that it reads and reads nothing that it writes, and begins it only behind its own wait, so all that came before is
 //    complete; what it reads goes past L1; and its blocks wait before they end, so whoever waits for it has dK and dV too. Three grids
 //    are on the chip then. A second kernel of this kind directly behind it would not have that ground to stand on.
+//  - attend_few_kernel as SECOND, the own keys of sequences behind a shared prefix, works before it has waited for the kernel of the prefix, which is
+//    always the launch ahead of it, writes nothing but parts, and begins it only behind its own wait. What SECOND reads until its wait goes past L1, so
+//    no line is older than that; all its blocks wait before they read a part, store a result or end, and only then let the next launch begin.
 #pragma once
 #include <cuda_runtime.h>
 

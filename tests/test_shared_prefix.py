@@ -306,3 +306,44 @@ def test_refusals():
     for kw in ({"count": whole(2)}, {"scale": 0.0}, {"scale": math.inf}):
         with pytest.raises(ValueError):
             F.shared_prefix_attention(*ok, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,hq,h,columns,dtype", [(5, 8, 2, 4, "bf16"), (40, 16, 4, 20, "bf16"), (6, 4, 2, 40, "bf16"), (64, 16, 4, 16, "fp32"), (3, 4, 4, 300, "bf16")])
+def test_steps_in_a_row_see_what_was_just_written(b, hq, h, columns, dtype):
+    """Tokens are written and attended to, one kernel directly behind the other, at the same addresses in every step: lengths and tables grow in place. Each
+    step's result is that of the same step alone."""
+    g = gen("cuda", 17)
+    n, d, shared, steps = 16, 64, 40, 12
+    dtype = torch.bfloat16 if dtype == "bf16" else torch.float32
+    blocks = shared + b * columns
+    cache0 = new_cache(g, "cuda", blocks, h, n, d)
+    ids = torch.randperm(blocks, generator=g, device="cuda").to(torch.int32)
+    prefix_table, all_table = ids[:shared].clone(), ids[shared:].view(b, columns)
+    prefix = torch.tensor([shared * n - 3], device="cuda")
+    start = torch.randint(0, columns * n - steps, (b,), generator=g, device="cuda", dtype=torch.int32)
+    kv = torch.randn((steps, 3, b, 1, hq, d), generator=g, device="cuda").to(dtype)
+
+    def run(wait):
+        cache = {k: v.clone() for k, v in cache0.items()}
+        past, table, q = start.clone(), torch.full_like(all_table, -1), torch.empty_like(kv[0, 0])
+        length = torch.zeros_like(prefix)
+        call = nb.compile(lambda c, k, v, q, t, p, pt, pl: (lambda c: (F.shared_prefix_attention(q, c, pt, pl, t, p), c))(F.kv_cache_write(c, k, v, t, p)))
+        c, tensors, out = wrap(cache), [T(x) for x in (q, table, past, prefix_table, length)], []
+        for i in range(steps):
+            # everything that the call reads is written directly in front of it
+            q.copy_(kv[i, 0])
+            length.copy_(prefix - i)
+            table.copy_(torch.where(torch.arange(columns, device="cuda") <= past[:, None] // n, all_table, -1))
+            if wait:
+                torch.cuda.synchronize()
+            o, c = call(c, T(kv[i, 1][:, :, :h]), T(kv[i, 2][:, :, :h]), *tensors)
+            if wait:
+                torch.cuda.synchronize()
+            out.append(o.to_torch().clone())
+            past += 1
+        return out
+
+    want = run(True)
+    for _ in range(3):
+        assert all(torch.equal(x, y) for x, y in zip(run(False), want))
