@@ -157,7 +157,8 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 __device__ __forceinline__ uint32_t widen(uint32_t biased, uint32_t sel) { return __byte_perm(biased, 0x64646464u, sel); }
 constexpr uint32_t BIAS2 = 0x64806480u;      // 1152 twice
 // Many rows: tiles of 128 rows on the tensor cores (cached_attention_tcgen05.cu), bf16 only.
+// q_tiles: tiles of a block, 0: two where the grid then still has a block for every SM.
 template <int D, Role ROLE>
-cudaError_t launch_many(const AttendArgs& a, int* status, cudaStream_t stream);
+cudaError_t launch_many(const AttendArgs& a, int q_tiles, int* status, cudaStream_t stream);
 
 }  // namespace nbc

@@ -647,7 +647,7 @@ static cudaError_t launch_few(const AttendArgs& a, const Cut& c, cudaStream_t st
 template <typename T, int D, Role ROLE>
 static cudaError_t launch_attend(const AttendArgs& a, const Cut& c, int* status, cudaStream_t stream) {
   if (c.rows == 128) {
-    const cudaError_t e = launch_many<D, ROLE>(a, status, stream);
+    const cudaError_t e = launch_many<D, ROLE>(a, 0, status, stream);
     return e != cudaSuccess || c.splits == 1 ? e : join<T, D, false, ROLE>(a, stream);
   }
   return c.rows == 8 ? launch_few<T, D, 1, ROLE>(a, c, stream) : launch_few<T, D, 2, ROLE>(a, c, stream);

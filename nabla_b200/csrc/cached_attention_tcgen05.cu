@@ -585,10 +585,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
 }
 
 template <int D, Role ROLE>
-cudaError_t launch_many(const AttendArgs& a, int* status, cudaStream_t stream) {
-  ManyArgs args = {a, 2, status};
+cudaError_t launch_many(const AttendArgs& a, int q_tiles, int* status, cudaStream_t stream) {
+  ManyArgs args = {a, q_tiles, status};
   const long long rows = (long long)a.fresh * (a.heads / a.kv_heads), pairs = (long long)a.batch * a.kv_heads * a.splits;
-  if ((rows + 255) / 256 * pairs < 148) args.q_tiles = 1;
+  if (q_tiles == 0) args.q_tiles = (rows + 255) / 256 * pairs < 148 ? 1 : 2;
   const long long grid = (rows + args.q_tiles * BT - 1) / (args.q_tiles * BT) * pairs;
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
   const cudaError_t e = cudaFuncSetAttribute(attend_many_kernel<D, ROLE>, cudaFuncAttributeMaxDynamicSharedMemorySize, ManySmem<D>::TOTAL);
@@ -597,13 +597,13 @@ cudaError_t launch_many(const AttendArgs& a, int* status, cudaStream_t stream) {
 }
 
 #ifdef NB_SHARED_PREFIX          // built once more for the library that has shared_prefix.cu
-template cudaError_t launch_many<64, FIRST>(const AttendArgs&, int*, cudaStream_t);
-template cudaError_t launch_many<128, FIRST>(const AttendArgs&, int*, cudaStream_t);
-template cudaError_t launch_many<64, SECOND>(const AttendArgs&, int*, cudaStream_t);
-template cudaError_t launch_many<128, SECOND>(const AttendArgs&, int*, cudaStream_t);
+template cudaError_t launch_many<64, FIRST>(const AttendArgs&, int, int*, cudaStream_t);
+template cudaError_t launch_many<128, FIRST>(const AttendArgs&, int, int*, cudaStream_t);
+template cudaError_t launch_many<64, SECOND>(const AttendArgs&, int, int*, cudaStream_t);
+template cudaError_t launch_many<128, SECOND>(const AttendArgs&, int, int*, cudaStream_t);
 #else
-template cudaError_t launch_many<64, ALONE>(const AttendArgs&, int*, cudaStream_t);
-template cudaError_t launch_many<128, ALONE>(const AttendArgs&, int*, cudaStream_t);
+template cudaError_t launch_many<64, ALONE>(const AttendArgs&, int, int*, cudaStream_t);
+template cudaError_t launch_many<128, ALONE>(const AttendArgs&, int, int*, cudaStream_t);
 #endif
 
 }  // namespace nbc

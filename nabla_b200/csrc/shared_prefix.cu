@@ -11,17 +11,38 @@
 
 namespace nbc {
 
-// How the prefix is cut: rows of a tile, ranges of its keys.
+// How the prefix is cut: rows of a tile, tiles of 128 rows to a block, ranges of its keys.
 struct FirstCut {
-  int rows, splits;
+  int rows, q_tiles, splits;
 };
-static FirstCut cut_first(int rows, int kv_heads, long long room, int fp32) {
-  const bool wide = !fp32 && rows > 32;
-  FirstCut c = {wide ? 128 : few_rows(rows), 1};
-  const long long units = (long long)kv_heads * ((rows + c.rows - 1) / c.rows), blocks = wide ? 148 : 148 * (c.rows == 8 ? 3 : 2);
-  const long long least = wide ? 512 : UNIT, most = (room + least - 1) / least, want = blocks / units;
-  c.splits = static_cast<int>(want < 2 || most < 2 ? 1 : want < most ? want : most);
-  return c;
+// `c`: how the own keys are cut, in lines of at most `room` keys.
+static FirstCut cut_first(int rows, int kv_heads, long long prefix_room, int fp32, const Cut& c, int batch, int own_rows, long long room) {
+  // Tiles of 128 rows start late and are soon quicker. us, tiles of 16 and of 128, behind 500, 2001 and 8001 tokens: 2 heads with 40 rows 10.8 and 15.6, 11.3 and
+  // 16.0, 20.0 and 17.1, with 128 rows 9.2 and 14.8, 15.3 and 15.0, 20.0 and 16.6; 4 heads with 96 rows 9.5 and 14.6, 17.3 and 15.0, 22.6 and 19.3; 16 heads with
+  // 64 rows 16.7 and 15.1, 21.5 and 22.3, 38.9 and 33.2.
+  const bool wide = !fp32 && rows > 32 && (rows > 128 || (long long)kv_heads * ((rows + 15) / 16) * prefix_room > 32768);
+  FirstCut f = {wide ? 128 : few_rows(rows), wide && rows > 128 ? 2 : 1, 1};
+  const long long units = (long long)kv_heads * ((rows + f.rows * f.q_tiles - 1) / (f.rows * f.q_tiles)), least = wide ? 256 : UNIT,
+                  most = (prefix_room + least - 1) / least;
+  long long want = (wide ? 148 : 148 * (f.rows == 8 ? 3 : 2)) / units;
+  if (wide && c.rows != 128) {
+    // Blocks of 128-row tiles take an SM each, those of the own keys a third or half of one. Either the prefix has the chip for itself and the own keys follow, or it
+    // takes the SMs that the own keys leave when all of their blocks run at once. us of the parts, measured: 7 for a block's start and end and 3.3 for a
+    // tile of 128 keys with 256 rows, 2.2 with 128; 9 and 1.6 for each step of 128 keys of a line of own keys; 0.08 to join a part. Both together, behind 8001
+    // tokens 64 sequences of up to 1000 with 16 heads over 4 27.2 beside each other (64 blocks) and 35.8 after each other (148), with up to 60 26.4 and 24.3; 16 of
+    // up to 2000 with 16 heads over 2 behind 60001 49.5 and 41.1; 32 of up to 1000 behind 16001 26.7 (120 blocks) and 38.4.
+    const long long lines = (long long)batch * kv_heads * ((own_rows + c.rows - 1) / c.rows);
+    const long long blocks = c.share == FLAT ? c.splits : lines * c.splits, left = 148 - (blocks + (c.rows == 8 ? 2 : 1)) / (c.rows == 8 ? 3 : 2);
+    const auto splits = [&](long long n) { return n / units < 1 ? 1 : n / units < most ? n / units : most; };
+    const auto time = [&](long long n) {
+      const long long tiles = (prefix_room + 127) / 128;
+      return 7.0 + (f.q_tiles == 2 ? 3.3 : 2.2) * static_cast<double>((tiles + splits(n) - 1) / splits(n)) * static_cast<double>((units * splits(n) + n - 1) / n);
+    };
+    const double own = 9.0 + 1.6 * static_cast<double>(room) / UNIT / (c.share == ONE ? 1.0 : c.share == CLUSTER ? c.splits : static_cast<double>(c.splits) / lines);
+    if (left >= units && left >= 16 && (time(left) > own ? time(left) : own) + 3.0 + 0.08 * splits(left) < time(148) + own + 0.08 * splits(148)) want = left / units;
+  }
+  f.splits = static_cast<int>(want < 2 || most < 2 ? 1 : want < most ? want : most);
+  return f;
 }
 
 template <typename T, int D, int RT>
@@ -32,15 +53,22 @@ static cudaError_t first_few(const AttendArgs& a, cudaStream_t stream) {
 }
 template <typename T, int D>
 static cudaError_t launch_both(const AttendArgs& first, const FirstCut& f, const AttendArgs& second, const Cut& c, int* status, cudaStream_t stream) {
-  const cudaError_t e = f.rows == 128 ? launch_many<D, FIRST>(first, status, stream)
+  const cudaError_t e = f.rows == 128 ? launch_many<D, FIRST>(first, f.q_tiles, status, stream)
                       : f.rows == 8 ? first_few<T, D, 1>(first, stream) : first_few<T, D, 2>(first, stream);
   return e != cudaSuccess ? e : launch_attend<T, D, SECOND>(second, c, status, stream);
 }
 
 // Floats of the parts; what follows them starts on a boundary of 16 bytes.
 static long long first_floats(long long rows, int splits, int head_dim) { return (rows * splits * (head_dim + 1) + 3) / 4 * 4; }
-static Cut cut_second(int batch, int fresh, int heads, int kv_heads, int head_dim, long long room, int fp32) {
-  return cut(batch, fresh * (heads / kv_heads), (long long)batch * fresh * heads, kv_heads, head_dim, room, fp32);
+struct Cuts {
+  FirstCut first;
+  Cut second;
+};
+static Cuts cut_both(int batch, int fresh, int heads, int kv_heads, int head_dim, long long prefix_room, long long room, int fp32) {
+  const long long rows = (long long)batch * fresh * heads;
+  const int own_rows = fresh * (heads / kv_heads);
+  const Cut c = cut(batch, own_rows, rows, kv_heads, head_dim, room, fp32);
+  return Cuts{cut_first(static_cast<int>(rows / kv_heads), kv_heads, prefix_room, fp32, c, batch, own_rows, room), c};
 }
 }  // namespace nbc
 
@@ -49,12 +77,12 @@ extern "C" long long nb_shared_prefix_scratch(int batch, int fresh, int heads, i
   using namespace nbc;
   const long long rows = (long long)batch * fresh * heads;
   if (rows > 0x7fffffffll) return -1;
-  return first_floats(rows, cut_first(static_cast<int>(rows / kv_heads), kv_heads, (long long)prefix_columns * block, fp32).splits, head_dim)
-         + cut_second(batch, fresh, heads, kv_heads, head_dim, (long long)columns * block, fp32).scratch;
+  const Cuts c = cut_both(batch, fresh, heads, kv_heads, head_dim, (long long)prefix_columns * block, (long long)columns * block, fp32);
+  return first_floats(rows, c.first.splits, head_dim) + c.second.scratch;
 }
 // Kernels that a call launches.
 extern "C" int nb_shared_prefix_launches(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int columns, int fp32) {
-  return nbc::cut_second(batch, fresh, heads, kv_heads, head_dim, (long long)columns * block, fp32).scratch > 0 ? 3 : 2;
+  return nbc::cut(batch, fresh * (heads / kv_heads), (long long)batch * fresh * heads, kv_heads, head_dim, (long long)columns * block, fp32).scratch > 0 ? 3 : 2;
 }
 
 // Strides of q as the rows of one sequence: q_sb = fresh * q_st, or fresh is 1. wide: bit 0 prefix_table, 1 prefix_length, 2 table, 3 past, 4 count are
@@ -76,7 +104,9 @@ extern "C" int nb_shared_prefix_attention(const void* q, const void* k_codes, co
   const long long rows = (long long)batch * fresh * heads;
   if (a.block_log < 0 || (head_dim != 64 && head_dim != 128) || rows > 0x7fffffffll || scratch == nullptr) return -1;
   if (batch > 1 && fresh > 1 && q_sb != fresh * q_st) return -1;
-  const FirstCut f = cut_first(static_cast<int>(rows / kv_heads), kv_heads, (long long)prefix_columns * block, fp32);
+  const Cuts cuts = cut_both(batch, fresh, heads, kv_heads, head_dim, (long long)prefix_columns * block, (long long)columns * block, fp32);
+  const FirstCut& f = cuts.first;
+  const Cut& c = cuts.second;
   AttendArgs first = a;
   first.table = Table{Whole{prefix_table, wide & 1}, prefix_columns, blocks};
   first.limit = Whole{prefix_length, wide >> 1 & 1};
@@ -84,7 +114,6 @@ extern "C" int nb_shared_prefix_attention(const void* q, const void* k_codes, co
   first.q_st = fresh == 1 ? q_sb : q_st;
   first.splits = f.splits, first.tile_rows = f.rows;
   first.part_o = scratch, first.part_w = scratch + rows * f.splits * head_dim;
-  const Cut c = cut_second(batch, fresh, heads, kv_heads, head_dim, (long long)columns * block, fp32);
   scratch += first_floats(rows, f.splits, head_dim);
   a.table = Table{Whole{table, wide >> 2 & 1}, columns, blocks};
   a.past = Whole{past, wide >> 3 & 1}, a.count = Whole{count, wide >> 4 & 1};
