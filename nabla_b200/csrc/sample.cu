@@ -48,42 +48,47 @@ __device__ __forceinline__ int token_of(u64 order) { return static_cast<int>(0xf
 
 struct Weigher {
   float top, per_octave;         // the largest logit; octaves of w for a unit of logit
-  double rate;                   // 32 octaves
+  double top64, rate;            // 32 octaves
   const double* roots;           // 2^(-i / 32), in shared memory
+  bool alone;                    // the largest logit, or what a unit of logit is worth, is infinite: only tokens with that logit have a weight
 
+  __device__ __forceinline__ Weigher(float largest, float temperature, const double* table) : top(largest), top64(largest), roots(table) {
+    rate = 46.166241308446828 / static_cast<double>(temperature);                        // 32 log2(e)
+    per_octave = static_cast<float>(rate / 32.0);
+    alone = top == INFINITY || per_octave == INFINITY;
+  }
   // The step of the histogram that a logit falls into, BINS: behind its end, or nowhere. Monotone.
   __device__ __forceinline__ int bin(float z) const {
-    const float x = z == top ? 0.f : (top - z) * per_octave;
+    if (alone) return z == top ? 0 : BINS;
+    const float x = (top - z) * per_octave;
     return x < FAR ? __float_as_int(fmaf(x, (BINS - 1) / FAR, 8388608.f)) & 0xfff : BINS;        // + 2^23: the nearest whole number is in the low bits
   }
-  __device__ __forceinline__ float about(float z) const { return z == top ? 1.f : exp2f((z - top) * per_octave); }
-  // w, as a number and in multiples of 2^-43
-  __device__ __forceinline__ double weight(float z) const {
-    if (z == top) return 1.0;
-    const double t = (static_cast<double>(top) - static_cast<double>(z)) * rate;             // 32nds of octaves
-    if (!(t <= 32.0 * 44.0)) return 0.0;
-    const double whole = t + 6755399441055744.0;             // 1.5 * 2^52: the nearest whole number is in the low bits
+  __device__ __forceinline__ float about(float z) const { return alone ? (z == top ? 1.f : 0.f) : exp2f((z - top) * per_octave); }
+  // w in multiples of 2^-43. With t in 32nds of octaves and n the whole number next to it: exp(-(t - n) ln 2 / 32) by its series (the term behind the last is
+  // below 2^-48), times a root of 2, put where its last bit is 2^-43 by adding 2^52. A logit of -inf and NaN have none.
+  __device__ __forceinline__ u64 fixed(float z) const {
+    if (alone) return z == top ? 1ull << 43 : 0;
+    const double t = (top64 - static_cast<double>(z)) * rate, whole = t + 6755399441055744.0;       // 1.5 * 2^52
     const int n = __double2loint(whole);
-    const double r = (t - (whole - 6755399441055744.0)) * -0.021660849392498290;            // ln 2 / 32
-    double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);              // exp(r) for |r| <= ln 2 / 64: the next term is below 2^-48
-    e = fma(r, e, 1.0 / 6.0), e = fma(r, e, 0.5), e = fma(r, e, 1.0), e = fma(r, e, 1.0);
-    e *= roots[n & 31];
-    return __hiloint2double(__double2hiint(e) - ((n >> 5) << 20), __double2loint(e));
+    const double x = t - (whole - 6755399441055744.0);
+    constexpr double U = -0.021660849392498290;              // -ln 2 / 32
+    double e = fma(x, U * U * U * U * U / 120.0, U * U * U * U / 24.0);
+    e = fma(x, e, U * U * U / 6.0), e = fma(x, e, U * U / 2.0), e = fma(x, e, U), e = fma(x, e, 1.0);
+    const double unit = __hiloint2double((1023 + 43 - (n >> 5)) << 20, 0);                 // 2^(43 - n / 32)
+    const double w = fma(e * roots[n & 31], unit, 4503599627370496.0);
+    return t <= 32.0 * 44.0 ? static_cast<u64>(__double_as_longlong(w)) & 0xfffffffffffffull : 0;
   }
-  static __device__ __forceinline__ u64 whole(double w) {
-    return static_cast<u64>(__double_as_longlong(fma(w, UNIT_WEIGHT, 4503599627370496.0))) & 0xfffffffffffffull;      // + 2^52
-  }
-  __device__ __forceinline__ u64 fixed(float z) const { return whole(weight(z)); }
 };
 
 // A row, eight tokens at a time from where memory is aligned; each warp has a stretch of ids.
 template <typename T>
 struct LogitRow {
   const T* in;
-  int vocab, shift, from, to;                                // groups of eight of this warp
+  int vocab, shift, from, to, per_warp;                      // groups of eight of this warp, of each
   __device__ __forceinline__ LogitRow(const T* p, int n, int rank, int blocks) : in(p), vocab(n) {
     shift = static_cast<int>(reinterpret_cast<uintptr_t>(p) / sizeof(T) & 7);
     const int groups = (vocab + shift + 7) / 8, warps = blocks * SAMPLE_WARPS, each = ((groups + warps - 1) / warps + 31) / 32 * 32;
+    per_warp = each;
     from = min(groups, (rank * SAMPLE_WARPS + static_cast<int>(threadIdx.x >> 5)) * each), to = min(groups, from + each);
   }
   __device__ __forceinline__ bool whole(int v) const { return v >= 0 && v + 8 <= vocab && NB_IN_BOUNDS(NB_SITE_LOGITS_TOKEN, v + 7, vocab); }
@@ -102,23 +107,33 @@ struct LogitRow {
       for (int e = 0; e < 8; ++e) z[e] = v + e >= 0 && v + e < vocab ? static_cast<float>(in[v + e]) : -INFINITY;
     }
   }
-  // f(token, logit) for all, two groups under way at once
+  // f(token, logit) for all, the next group under way while one is worked on
   template <typename F>
   __device__ __forceinline__ void each(F&& f) const {
+    int g = from + static_cast<int>(threadIdx.x & 31);
+    Eight<T> next;
+    if (g < to && whole(g * 8 - shift)) next.load(in + g * 8 - shift);
 #pragma unroll 1
-    for (int g = from + (threadIdx.x & 31); g < to; g += 64) {
-      float z[2][8];
-      const int v = g * 8 - shift;
-      get(v, z[0]);
-      const bool more = g + 32 < to;
-      if (more) get(v + 256, z[1]);
+    for (; g < to; g += 32) {
+      const Eight<T> now = next;
+      const int v = g * 8 - shift, w = v + 256;
+      if (g + 32 < to && whole(w)) next.load(in + w);
+      float z[8];
+      if (whole(v)) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f(v + e, z[0][e]);
-      if (more)
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = now.pair(e);
+          z[2 * e] = x.x, z[2 * e + 1] = x.y;
+        }
+      } else {
+        get(v, z);
+      }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f(v + 256 + e, z[1][e]);
+      for (int e = 0; e < 8; ++e) f(v + e, z[e]);
     }
   }
+  // The warp of the row's that owns token v
+  __device__ __forceinline__ int warp_of(int v) const { return (v + shift) / 8 / per_warp; }
 };
 
 struct SampleShared {
@@ -191,13 +206,19 @@ struct Team {
     x = y = z = 0;
     for (int r = 0; r < blocks; ++r) x += all[r][0], y += all[r][1], z += all[r][2];
   }
+  __device__ __forceinline__ void clear() const {
+    uint4* bins = reinterpret_cast<uint4*>(CLUSTER ? s.own_bins : s.bins);
+    for (int i = threadIdx.x; i < BINS / 4; i += SAMPLE_THREADS) bins[i] = make_uint4(0, 0, 0, 0);
+  }
   // s.bins counts the tokens of the row for which `f` (token, logit) names a bin below BINS
   template <typename T, typename F>
-  __device__ __forceinline__ void count(const LogitRow<T>& row, F&& f) {
+  __device__ __forceinline__ void count(const LogitRow<T>& row, F&& f, bool again = true) {
     uint32_t* bins = CLUSTER ? s.own_bins : s.bins;
-    sync();                                // (others have read the ones before)
-    for (int i = threadIdx.x; i < BINS; i += SAMPLE_THREADS) bins[i] = 0;
-    __syncthreads();
+    if (again) {
+      sync();                              // (others have read the ones before)
+      clear();
+      __syncthreads();
+    }
     row.each([&](int v, float z) {
       const int i = f(v, z);
       if (i < BINS) atomicAdd(&bins[i], 1u);
@@ -326,10 +347,12 @@ struct Stretch {
 };
 
 // The place in the order of the last token in front of which less than `want` lies; the stretch holds it. COUNT: tokens are counted, not weighed.
+// `entries`: the tokens of the stretch, which are in the list then; -1 where it was cut finer first.
 template <typename T, bool CLUSTER, bool COUNT>
-__device__ __noinline__ u64 last_kept(Team<CLUSTER>& team, const LogitRow<T>& row, const Weigher& weigh, Stretch at, double want) {
+__device__ __noinline__ u64 last_kept(Team<CLUSTER>& team, const LogitRow<T>& row, const Weigher& weigh, Stretch at, double want, int& entries) {
   SampleShared& s = team.s;
-  for (int level = 0; at.n > LIST && level < 64; ++level) {   // (a few levels: each is at most 3 of some 2000 bins, or what is left beside them)
+  const bool whole = at.n <= LIST;
+  for (int level = 0; at.n > LIST && level < 64; ++level) {   // (a few levels: each is one of some 2000 bins, or what is left beside it)
     // finer bins of the order
     const u64 range = at.high - at.low;
     const int shift = max(0, 64 - __clzll(static_cast<long long>(range)) - 11);
@@ -356,7 +379,7 @@ __device__ __noinline__ u64 last_kept(Team<CLUSTER>& team, const LogitRow<T>& ro
       const u64 n = s.bins[i], middle = at.high - (static_cast<u64>(i) << shift) - (shift ? 1ull << (shift - 1) : 0);
       return n ? static_cast<float>(n) * weigh.about(number_of(static_cast<uint32_t>(middle >> 32))) : 0.f;
     });
-    const int c = max(s.found, 0), first = max(c - 1, 0), last = min(c + 1, BINS - 1);
+    const int first = max(s.found, 0), last = first;          // (the estimate is seldom off by a bin: what it names is checked)
     Stretch x = cut(first, last);
     u64 above = 0, within = 0, none = 0;
     row.each([&](int v, float z) {
@@ -378,10 +401,14 @@ __device__ __noinline__ u64 last_kept(Team<CLUSTER>& team, const LogitRow<T>& ro
     }
     at = x;
   }
+  // (as numbers first: above the largest there is no number, nothing is at least that)
+  const float z_low = number_of(static_cast<uint32_t>(at.low >> 32)), z_above = number_of(static_cast<uint32_t>(at.high >> 32) + 1);
   const int n = team.list(row, weigh, COUNT, [&](int v, float z) {
+    if (!(z >= z_low) || z >= z_above) return false;
     const u64 q = order_of(z, v);
-    return q >= at.low && q <= at.high && q != 0;
+    return q >= at.low && q <= at.high;
   });
+  entries = whole ? n : -1;
   u64 kept = ~0ull;
   if (static_cast<int>(threadIdx.x) < n) {
     const u64 q = s.order[threadIdx.x];
@@ -403,6 +430,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
   __shared__ __align__(16) SampleShared s;
   if (threadIdx.x < 32) s.roots[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 32.0);
   Team<CLUSTER> team(s, a.blocks);
+  team.clear();
   if constexpr (CLUSTER) team.sync();      // every block of the cluster runs before another writes to it
   follow_grid();
   const int b = CLUSTER ? blockIdx.x / a.blocks : blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -423,25 +451,33 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     return;
   }
   const bool by_count = asked > 0 && asked < a.vocab, by_share = p < 1.f;
-  const double rate = 46.166241308446828 / static_cast<double>(temperature);              // 32 log2(e)
-  const double floor_of = least > 0.f ? fmin(static_cast<double>(least), 1.0) : 0.0;
-  const Weigher weigh = {top, static_cast<float>(rate / 32.0), rate, s.roots};
+  const Weigher weigh(top, temperature, s.roots);
+  // the least weight that min-p keeps: w >= m where the whole number of w is at least that of m, rounded up (m is no whole number but by chance)
+  const u64 least_kept = least > 0.f ? static_cast<u64>(ceil(fmin(static_cast<double>(least), 1.0) * UNIT_WEIGHT)) : 0;
   u64 last = 0;                            // of the order, the last that is kept
+  u64 above_mine = 0;                      // top-p alone: what this warp has above the steps that hold the border, and how many tokens of these are in the list
+  int listed = -1;
   if (by_count || by_share) {
     const auto in_bins = [&](int v, float z) { return weigh.bin(z); };
-    team.count(row, in_bins);
-    // keys whose bin is below `b` begin here (bins fall as keys grow)
+    team.count(row, in_bins, false);
+    // the least key whose bin is below `b`: bins fall as keys grow. A warp tries 31 keys at once
     const auto edge = [&](int b) {
-      uint32_t lo = key_of(-INFINITY), hi = key_of(weigh.top) + 1;       // the least key in (lo, hi] with a bin below b
+      uint32_t lo = key_of(-INFINITY), hi = key_of(weigh.top) + 1;       // in (lo, hi]
       while (hi - lo > 1) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        if (weigh.bin(number_of(mid)) < b) hi = mid; else lo = mid;
+        const uint32_t step = (hi - lo + 31) / 32, mid = lo + min(hi - lo, step * (lane + 1));
+        const uint32_t below = __ballot_sync(0xffffffffu, mid >= hi || weigh.bin(number_of(mid)) < b);
+        const int k = __ffs(static_cast<int>(below)) - 1;                // the first of them (the last is at hi)
+        const uint32_t top_key = lo + min(hi - lo, step * (k + 1));
+        lo += step * k, hi = top_key;
       }
       return static_cast<u64>(hi) << 32;
     };
     const auto stretch = [&](int first, int last_bin) {      // of bins [first, last_bin]
       __syncthreads();
-      if (warp == 0 && lane < 2) s.edges[lane] = edge(lane ? last_bin + 1 : first);
+      if (warp < 2) {
+        const u64 at = edge(warp ? last_bin + 1 : first);
+        if (lane == 0) s.edges[warp] = at;
+      }
       __syncthreads();
       return Stretch{s.edges[1], s.edges[0] - 1, 0, 0};
     };
@@ -470,7 +506,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         const double want = static_cast<double>(p) * static_cast<double>(block_sum(s, kept ? w : 0));
         kept = kept && (place == 0 || static_cast<double>(sum) < want);
       }
-      kept = kept && weigh.weight(number_of(static_cast<uint32_t>(q >> 32))) >= floor_of;
+      kept = kept && w >= least_kept;
       const u64 all = block_sum(s, kept ? w : 0);            // (all threads are behind their reads of the weights)
       if (mine) s.weights[threadIdx.x] = kept ? w : 0;
       __syncthreads();
@@ -485,12 +521,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
       end = c, end_tokens = static_cast<int>(asked) - before;
       Stretch x = stretch(c, c);
       x.sum = before, x.n = static_cast<int>(s.bins[c]);
-      last = last_kept<T, CLUSTER, true>(team, row, weigh, x, static_cast<double>(asked));
+      int entries;
+      last = last_kept<T, CLUSTER, true>(team, row, weigh, x, static_cast<double>(asked), entries);
       if (by_share && x.n > LIST) team.count(row, in_bins);  // finer bins took the histogram's place
     }
     if (by_share) {
       find_bin<float, true>(s, p, [&](int i) { return i > end ? 0.f : static_cast<float>(i == end ? end_tokens : static_cast<int>(s.bins[i])) * about(i); });
-      const int d = max(s.found, 0), first = max(d - 1, 0), last_bin = min(d + 1, BINS - 1);
+      const int first = max(s.found, 0), last_bin = first;     // (the estimate is seldom off by a bin: what it names is checked)
       Stretch x = stretch(first, last_bin);
       // the border of top-k as a number and an id, and the stretch as numbers (above the largest: no number, nothing is at least that)
       const float z_last = last ? number_of(static_cast<uint32_t>(last >> 32)) : -INFINITY, z_low = number_of(static_cast<uint32_t>(x.low >> 32)),
@@ -504,8 +541,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         if (z >= z_above) above += w;
         else if (z >= z_low) within += w;
       });
+      above_mine = over_warp_sum(above);
       team.sums_of(all, above, within);
       const double want = fmax(static_cast<double>(p) * static_cast<double>(all), 0.5);     // (the first is kept)
+      bool here = false;
       if (static_cast<double>(above) >= want) {
         x = stretch(0, first - 1);
         x.sum = 0, x.n = tokens_before(s, first);
@@ -514,9 +553,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
         x.sum = above + within, x.n = total - tokens_before(s, last_bin + 1);
       } else {
         x.sum = above, x.n = tokens_before(s, last_bin + 1) - tokens_before(s, first);
+        here = true;
       }
       x.low = max(x.low, last);
-      last = last_kept<T, CLUSTER, false>(team, row, weigh, x, want);
+      last = last_kept<T, CLUSTER, false>(team, row, weigh, x, want, listed);
+      if (!here) listed = -1;
     }
   }
   // ---- the draw
@@ -524,12 +565,21 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
   const int v_last = last ? token_of(last) : -1;
   const auto drawn = [&](int v, float z) {
     if (!(z > z_last || (z == z_last && v <= v_last))) return 0ull;
-    const double w = weigh.weight(z);
-    return w >= floor_of ? Weigher::whole(w) : 0ull;
+    const u64 w = weigh.fixed(z);
+    return w >= least_kept ? w : 0ull;
   };
   u64 sum = 0;
-  row.each([&](int v, float z) { sum += drawn(v, z); });
-  sum = over_warp_sum(sum);
+  if (listed >= 0 && least_kept == 0) {    // the sums are known: those above the steps of the border, and in these what the list has up to it
+    const int me = team.rank * SAMPLE_WARPS + warp;
+    for (int i = lane; i < listed; i += 32) {
+      const u64 q = s.order[i];
+      if (q >= last && row.warp_of(token_of(q)) == me) sum += s.weights[i];
+    }
+    sum = over_warp_sum(sum) + above_mine;
+  } else {
+    row.each([&](int v, float z) { sum += drawn(v, z); });
+    sum = over_warp_sum(sum);
+  }
   __syncthreads();
   if (lane == 0) s.joined[0][warp] = sum;
   __syncthreads();
@@ -583,9 +633,11 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
 
 template <typename T>
 static cudaError_t launch_sample(SampleArgs a, int batch, cudaStream_t stream) {
-  // blocks of a row: as many as the chip has room for twice over, each with 4096 tokens at least
+  // Blocks of a row: as many as the chip has room for twice over, of 8192 tokens each (a cluster's exchanges cost 3 us). us with 1, 2, 4, 8 blocks: one row of
+  // 32000 19.0, 16.9, 14.2, 14.9, of 8192 9.5, 11.7, 12.4, 14.0; 64 rows of 32001 82, 66, 55, 57; 128 rows 51, 44, 54, 96; 256 rows 62, 64, 85, 168; 32 rows of
+  // 131072 158, 97, 70, 59.
   a.blocks = 1;
-  while (a.blocks < MOST_BLOCKS && (long long)batch * a.blocks * 2 <= 296 && a.vocab > 4096 * a.blocks) a.blocks *= 2;
+  while (a.blocks < MOST_BLOCKS && (long long)batch * a.blocks * 2 <= 296 && a.vocab > 8192 * a.blocks) a.blocks *= 2;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(static_cast<unsigned>(batch) * a.blocks);
