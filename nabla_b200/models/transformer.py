@@ -11,6 +11,9 @@ parallel axis as well (activations ``P('dp', 'tp', None)``): the row-parallel pr
 a reduce-scatter instead of an all-reduce, the column-parallel ones start with an all-gather,
 and no elementwise work is replicated over the tensor-parallel group. Both collectives fuse
 with their GEMM (``csrc/gemm_tcgen05.cu``).
+
+With ``rotary_base`` queries and keys are turned by their positions and there is no position embedding; with ``qk_norm`` as well they are normed for each
+head first (``F.packed_norm_rotary``).
 """
 from __future__ import annotations
 
@@ -36,6 +39,12 @@ class TransformerConfig:
     max_seq: int = 2048
     dtype: DType = DType.bfloat16
     init_std: float = 0.02
+    rotary_base: float | None = None      # rotations in place of the position embedding
+    qk_norm: bool = False                 # with rotations: norms of the heads of queries and keys, with gains
+
+    def __post_init__(self) -> None:
+        if self.qk_norm and self.rotary_base is None:
+            raise ValueError("qk_norm goes with rotary_base")
 
     @property
     def head_dim(self) -> int:
@@ -43,8 +52,8 @@ class TransformerConfig:
 
     def num_params(self) -> int:
         d, f, v = self.d_model, self.d_ff, self.vocab
-        per_layer = 4 * d * d + 4 * d + 2 * d * f + f + d + 4 * d
-        return self.n_layers * per_layer + 2 * v * d + self.max_seq * d + 2 * d
+        per_layer = 4 * d * d + 4 * d + 2 * d * f + f + d + 4 * d + (2 * self.head_dim if self.qk_norm else 0)
+        return self.n_layers * per_layer + 2 * v * d + (self.max_seq * d if self.rotary_base is None else 0) + 2 * d
 
     def flops_per_token(self, seq: int) -> float:
         """Training FLOPs per token: 6 x matmul parameters + causal attention."""
@@ -98,9 +107,10 @@ def init_params(cfg: TransformerConfig, mesh=None, tp_axis: str | None = "tp", d
             "ln2_g": rep(ones((d,), dtype=dt, device=device)), "ln2_b": rep(zeros((d,), dtype=dt, device=device)),
             "w1": col(w((d, f))), "b1": vec_col(zeros((f,), dtype=dt, device=device)),
             "w2": row(w((f, d), out_std)), "b2": rep(zeros((d,), dtype=dt, device=device)),
+            **({name: rep(ones((cfg.head_dim,), dtype=dt, device=device)) for name in ("q_gain", "k_gain")} if cfg.qk_norm else {}),
         })
     return {
-        "tok_emb": rep(w((v, d))), "pos_emb": rep(w((cfg.max_seq, d))),
+        "tok_emb": rep(w((v, d))), **({"pos_emb": rep(w((cfg.max_seq, d)))} if cfg.rotary_base is None else {}),
         "layers": layers,
         "lnf_g": rep(ones((d,), dtype=dt, device=device)), "lnf_b": rep(zeros((d,), dtype=dt, device=device)),
         "lm_head": col(w((d, v))),
@@ -133,12 +143,21 @@ def _lora_linear(x: Tensor, w: Tensor, b: Tensor | None, ad: dict[str, Tensor] |
     return y + ((x @ A) @ B) * (alpha / float(int(A.shape[1])))
 
 
+def _attend(qkv: Tensor, p: dict[str, Tensor], cfg: TransformerConfig, positions: Tensor | None) -> Tensor:
+    """Causal self-attention on the packed projection, its queries and keys turned by ``positions`` (S,) first (0 ... S - 1 by default)."""
+    if cfg.rotary_base is not None:
+        if positions is None:
+            positions = arange(0, int(qkv.shape[1]), 1, dtype=DType.int32, device=qkv.device)
+        qkv = F.packed_norm_rotary(qkv, cfg.head_dim, positions, p.get("q_gain"), p.get("k_gain"), base=cfg.rotary_base)
+    return fused.packed_self_attention(qkv, cfg.head_dim, causal=True)
+
+
 def block(x: Tensor, p: dict[str, Tensor], cfg: TransformerConfig, sp: SeqParallel | None = None,
-          lora: dict[str, Any] | None = None, lora_alpha: float = 16.0) -> Tensor:
+          lora: dict[str, Any] | None = None, lora_alpha: float = 16.0, positions: Tensor | None = None) -> Tensor:
     if lora is not None:
         h = F.layer_norm(x, p["ln1_g"], p["ln1_b"])
         qkv = _lora_linear(h, p["wqkv"], p["bqkv"], lora["qkv"], lora_alpha)
-        a = fused.packed_self_attention(qkv, cfg.head_dim, causal=True)
+        a = _attend(qkv, p, cfg, positions)
         x = x + _lora_linear(a, p["wo"], p["bo"], lora["o"], lora_alpha)
         h = F.layer_norm(x, p["ln2_g"], p["ln2_b"])
         m = F.linear(h, p["w1"], p["b1"], activation="gelu")
@@ -146,7 +165,7 @@ def block(x: Tensor, p: dict[str, Tensor], cfg: TransformerConfig, sp: SeqParall
     if sp is None:
         h = F.layer_norm(x, p["ln1_g"], p["ln1_b"])
         qkv = F.linear(h, p["wqkv"], p["bqkv"])
-        a = fused.packed_self_attention(qkv, cfg.head_dim, causal=True)
+        a = _attend(qkv, p, cfg, positions)
         x = x + F.linear(a, p["wo"], p["bo"])
         h = F.layer_norm(x, p["ln2_g"], p["ln2_b"])
         m = F.linear(h, p["w1"], p["b1"], activation="gelu")
@@ -154,7 +173,7 @@ def block(x: Tensor, p: dict[str, Tensor], cfg: TransformerConfig, sp: SeqParall
     # tokens split over tp outside the projections: gather -> column-parallel -> row-parallel -> scatter
     h = sp.tokens_whole(F.layer_norm(x, p["ln1_g"], p["ln1_b"]))
     qkv = F.linear(h, p["wqkv"], p["bqkv"])
-    a = fused.packed_self_attention(qkv, cfg.head_dim, causal=True)
+    a = _attend(qkv, p, cfg, positions)
     x = x + (sp.tokens_split(F.linear(a, p["wo"])) + p["bo"])
     h = sp.tokens_whole(F.layer_norm(x, p["ln2_g"], p["ln2_b"]))
     m = F.linear(h, p["w1"], p["b1"], activation="gelu")
@@ -166,14 +185,18 @@ def forward(params: dict[str, Any], tokens: Tensor, cfg: TransformerConfig, sp: 
     """tokens (B, S) int64 -> logits (B, S, vocab)."""
     S = int(tokens.shape[1])
     x = gather(params["tok_emb"], tokens, axis=0)
-    pos = params["pos_emb"]
-    if int(pos.shape[0]) != S:
-        pos = pos[:S]
-    x = x + pos
+    positions = None
+    if cfg.rotary_base is not None:
+        positions = arange(0, S, 1, dtype=DType.int32, device=tokens.device)
+    else:
+        pos = params["pos_emb"]
+        if int(pos.shape[0]) != S:
+            pos = pos[:S]
+        x = x + pos
     if sp is not None:
         x = sp.tokens_split(x)
     for li, p in enumerate(params["layers"]):
-        x = block(x, p, cfg, sp, lora[li] if lora is not None else None)
+        x = block(x, p, cfg, sp, lora[li] if lora is not None else None, positions=positions)
     x = F.layer_norm(x, params["lnf_g"], params["lnf_b"])
     if sp is not None:
         x = sp.tokens_whole(x)
@@ -211,13 +234,25 @@ def torch_reference_forward(params: dict[str, Any], tokens, cfg: TransformerConf
     def t(x):
         return torch.from_numpy(x.to_numpy()).float()
 
-    x = t(params["tok_emb"])[tokens] + t(params["pos_emb"])[: tokens.shape[1]]
+    x = t(params["tok_emb"])[tokens]
+    if cfg.rotary_base is None:
+        x = x + t(params["pos_emb"])[: tokens.shape[1]]
     B, S, d = x.shape
     H, hd = cfg.n_heads, cfg.head_dim
+
+    def turned(y, gain):                 # (B, H, S, hd)
+        if gain is not None:
+            y = y * torch.rsqrt((y * y).mean(-1, keepdim=True) + 1e-6) * t(gain)
+        angle = torch.arange(S, dtype=torch.float64)[:, None] * cfg.rotary_base ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd)
+        c, s, (a, b) = angle.cos().float(), angle.sin().float(), y.chunk(2, -1)
+        return torch.cat([a * c - b * s, a * s + b * c], -1)
+
     for p in params["layers"]:
         h = TF.layer_norm(x, (d,), t(p["ln1_g"]), t(p["ln1_b"]))
         qkv = (h @ t(p["wqkv"]) + t(p["bqkv"])).view(B, S, H, 3, hd)
         q, k, v = (qkv[:, :, :, i].transpose(1, 2) for i in range(3))
+        if cfg.rotary_base is not None:
+            q, k = turned(q, p.get("q_gain")), turned(k, p.get("k_gain"))
         a = TF.scaled_dot_product_attention(q, k, v, is_causal=True).transpose(1, 2).reshape(B, S, d)
         x = x + a @ t(p["wo"]) + t(p["bo"])
         h = TF.layer_norm(x, (d,), t(p["ln2_g"]), t(p["ln2_b"]))
