@@ -347,3 +347,60 @@ def test_steps_in_a_row_see_what_was_just_written(b, hq, h, columns, dtype):
     want = run(True)
     for _ in range(3):
         assert all(torch.equal(x, y) for x, y in zip(run(False), want))
+
+
+_CHECKED = """
+import torch
+import nabla_b200 as nb
+from nabla_b200 import native
+from nabla_b200.nn import functional as F
+T = nb.Tensor.from_torch
+g = torch.Generator("cuda").manual_seed(0)
+rand = lambda *s: torch.randn(s, generator=g, device="cuda")
+for d, n in ((64, 16), (128, 64)):
+    for b, new, hq, h, prefix, dtype in ((3, 1, 8, 2, 37, torch.bfloat16), (70, 1, 8, 2, 300, torch.bfloat16), (5, 40, 4, 2, 200, torch.bfloat16), (4, 3, 4, 4, 50, torch.float32)):
+        cache = F.init_kv_cache(64 + b * 4, h, d, n, device=nb.Accelerator(0))
+        shared = -(-prefix // n) + 1
+        ids = torch.randperm(64 + b * 4, generator=g, device="cuda").to(torch.int32)
+        table = ids[shared:shared + b * 4].view(b, 4).clone()
+        past = torch.randint(0, 4 * n, (b,), generator=g, device="cuda", dtype=torch.int32)
+        count = torch.randint(0, new + 1, (b,), generator=g, device="cuda", dtype=torch.int32)
+        table[0, 3], table[-1, 0] = -1, 1 << 30
+        for length in (prefix, 0, 1 << 40, -5):
+            F.shared_prefix_attention(T(rand(b, new, hq, d).to(dtype)), cache, T(ids[:shared]), T(torch.tensor([length], device="cuda")), T(table), T(past), T(count)).to_torch()
+for v, b in ((1, 2), (333, 7), (40001, 3), (40001, 300)):
+    for dtype in (torch.bfloat16, torch.float32):
+        z, u = rand(b, v).to(dtype), torch.rand(b, generator=g, device="cuda")
+        k, p = torch.randint(-1, v + 2, (b,), generator=g, device="cuda"), torch.rand(b, generator=g, device="cuda")
+        for kw in ({}, {"top_k": T(k)}, {"top_p": T(p)}, {"top_k": T(k), "top_p": T(p), "min_p": T(p * 0.1), "temperature": T(p * 2)}):
+            for x in (z, z * 0, z * 1e-3):
+                F.sample_tokens(T(x), T(u), **kw).to_torch()
+for d, rotary, b, t in ((64, 32, 2, 5), (80, 80, 3, 1), (256, 256, 1, 700), (128, 128, 5, 999)):
+    q, k, pos = rand(b, t, 5, d).bfloat16(), rand(b, t, 3, d).bfloat16(), torch.arange(t, device="cuda")
+    gain = rand(d).bfloat16()
+    y, pull = nb.vjp(lambda q, k, c: F.norm_rotary(q, k, T(pos), c, c, rotary_dim=rotary), T(q), T(k), T(gain), create_graph=False)
+    [x.to_torch() for x in pull((T(q), T(k)))]
+torch.cuda.synchronize()
+native.check_status()
+native.debug_check()
+for name, units in (("libnb_answers.so", 3), ("libnb_heads.so", 1)):
+    native.debug_selftest(name, 12, 8, 64, 16)
+    print("FAILED CHECKS", name, native.debug_report()["count"] == units)
+"""
+
+
+@pytest.mark.gpu
+def test_the_checked_build_finds_every_access_in_bounds():
+    import os
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    from nabla_b200.csrc import build
+
+    build.build_all(debug=True)
+    root = Path(__file__).resolve().parent.parent
+    env = dict(os.environ, NABLA_B200_DEBUG_KERNELS="1", PYTHONPATH=str(root))
+    r = subprocess.run([sys.executable, "-c", _CHECKED], capture_output=True, text=True, env=env, timeout=600, cwd=root)
+    assert r.returncode == 0, r.stdout[-2000:] + r.stderr[-4000:]
+    assert r.stdout.count("True") == 2
