@@ -5,8 +5,8 @@
 namespace nbc {
 
 // What a call of the kernels is: all there is of an attention; or, of one over a prefix that a batch shares (shared_prefix.cu), the keys of the prefix, whose
-// parts are left for the other, or the keys of each sequence's own, which are joined with them.
-enum Role { ALONE, FIRST, SECOND };
+// parts are left for the other, or the keys of each sequence's own, which are joined with them, or both one behind the other.
+enum Role { ALONE, FIRST, SECOND, WHOLE };
 
 struct AttendArgs {
   const void* q;                 // [batch][new][heads][D]
@@ -23,8 +23,9 @@ struct AttendArgs {
   // fp32 results of parts, and log2 of the sum of their weights: [splits][batch][kv_heads][new * group] rows, or two tiles of rows for each block
   float *part_o, *part_w;
   int* lines;                    // see attend_few_kernel
-  // FIRST: how many keys the prefix has. (Its rows are those of all sequences, one behind the other, of a batch of one.)
+  // FIRST, WHOLE: how many keys the prefix has. (FIRST: its rows are those of all sequences, one behind the other, of a batch of one.)
   Whole limit;
+  Table first_table;             // WHOLE: the blocks of the prefix
   // SECOND: parts of the rows, [first_parts][kv_heads][batch * new * group]
   const float *first_o, *first_w;
   int first_parts;

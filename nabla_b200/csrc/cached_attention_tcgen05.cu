@@ -144,6 +144,8 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
   const int room = a.table.columns << a.block_log, past = ROLE == FIRST ? 0 : clamp_tokens(a.past.at(b), room);
   const int count = clamp_tokens(ROLE == FIRST || a.count.p == nullptr ? a.fresh : a.count.at(b), a.fresh);
   const int all_keys = ROLE == FIRST ? clamp_tokens(a.limit.at(0), room) : min(room, past + count);
+  // WHOLE: the tiles of the prefix come first, then those of the own keys, which begin a tile
+  const int prefix = ROLE == WHOLE ? clamp_tokens(a.limit.at(0), a.first_table.columns << a.block_log) : 0, n_pre = (prefix + BT - 1) / BT;
   const int row0 = qt * args.q_tiles * BT;
   int n_t[2], first_t[2];          // key tiles of a row tile, the last key that its first row sees
 #pragma unroll
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
     const int r0 = row0 + t * BT, r1 = min(min(r0 + BT, rows), count * group);        // rows [r0, r1) are live
     const bool any = t < args.q_tiles && r0 < r1;
     const int keys = !any ? 0 : a.causal ? min(room, past + (r1 - 1) / group + 1) : all_keys;
-    n_t[t] = (keys + BT - 1) / BT;
+    n_t[t] = !any ? 0 : n_pre + (keys + BT - 1) / BT;
     first_t[t] = a.causal ? min(all_keys - 1, past + r0 / group) : all_keys - 1;
   }
   const int per = (max(n_t[0], n_t[1]) + a.splits - 1) / a.splits, kt0 = sp * per;       // this block's key tiles: [kt0, kt0 + n_t[t])
@@ -168,8 +170,9 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
     // would be waited for where the paths meet)
     struct Place { long long codes, unit; bool there, in; };
     auto find = [&](int j) {
-      const int at = (kt0 + j) * BT + 16 * (lane & 7);
-      const int id = j < n_max && at < all_keys ? a.table.block(b, at >> a.block_log) : -1;
+      const bool pre = ROLE == WHOLE && kt0 + j < n_pre;
+      const int at = (kt0 + j - (pre ? 0 : n_pre)) * BT + 16 * (lane & 7);
+      const int id = j < n_max && at < (pre ? prefix : all_keys) ? (pre ? a.first_table.block(0, at >> a.block_log) : a.table.block(b, at >> a.block_log)) : -1;
       const long long unit = (long long)max(id, 0) * a.kv_heads + h;
       return Place{((unit << a.block_log) + (at & (n - 1))) * D, unit, id >= 0, holds_keys(a, unit, at & (n - 1))};
     };
@@ -332,9 +335,10 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
     }
     float m = -INFINITY, l = 0.f;
     bool ok = true;
-    const int last = a.causal ? min(all_keys - 1, past + token) : all_keys - 1;      // this row's last visible key
+    const int own_last = a.causal ? min(all_keys - 1, past + token) : all_keys - 1;  // this row's last visible key
     for (int j = 0; j < n; ++j) {
-      const int kv0 = (kt0 + j) * BT;
+      const bool pre = ROLE == WHOLE && kt0 + j < n_pre;
+      const int kv0 = (kt0 + j - (pre ? 0 : n_pre)) * BT, last = pre ? prefix - 1 : own_last, first_last = pre ? prefix - 1 : first_t[t];
       if (!mbar_wait(&s_full[t], j & 1)) {
         atomicExch(args.status, NB_ERR_TIMEOUT_EPILOGUE);
         ok = false;
@@ -343,7 +347,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
       if (!ok) break;
       tc_fence_after();
       uint32_t va[32], vb[32];
-      if (kv0 + BT - 1 > first_t[t]) {
+      if (kv0 + BT - 1 > first_last) {
         // a tile on the diagonal or the last one: scores of hidden keys are put out of sight, so that the passes below know nothing of them
 #pragma unroll 1
         for (int c = 0; c < BT / 32; ++c) {
@@ -379,7 +383,7 @@ __global__ void __launch_bounds__(MANY_THREADS, 1) attend_many_kernel(const Many
           gt[2 * c + k] = fmaf(fmaxf(x, y), fs[2 * c + k], adds[2 * c + k]);
         }
       }
-      if (kv0 + BT - 1 > first_t[t]) {     // the scale of 16 keys that a row does not see may be NaN
+      if (kv0 + BT - 1 > first_last) {     // the scale of 16 keys that a row does not see may be NaN
 #pragma unroll
         for (int k = 0; k < GROUPS; ++k)
           if (kv0 + 16 * k > last) fs[k] = 1.f, adds[k] = 0.f, gt[k] = -INFINITY;
@@ -601,6 +605,8 @@ template cudaError_t launch_many<64, FIRST>(const AttendArgs&, int, int*, cudaSt
 template cudaError_t launch_many<128, FIRST>(const AttendArgs&, int, int*, cudaStream_t);
 template cudaError_t launch_many<64, SECOND>(const AttendArgs&, int, int*, cudaStream_t);
 template cudaError_t launch_many<128, SECOND>(const AttendArgs&, int, int*, cudaStream_t);
+template cudaError_t launch_many<64, WHOLE>(const AttendArgs&, int, int*, cudaStream_t);
+template cudaError_t launch_many<128, WHOLE>(const AttendArgs&, int, int*, cudaStream_t);
 #else
 template cudaError_t launch_many<64, ALONE>(const AttendArgs&, int, int*, cudaStream_t);
 template cudaError_t launch_many<128, ALONE>(const AttendArgs&, int, int*, cudaStream_t);

@@ -6,7 +6,8 @@
 // sequences: their queries are the rows of one problem (FIRST), 128 to a tile of the tensor cores or 8 or 16 to a tile of the form for few rows, whose keys
 // are cut into ranges so that the chip is full. A row's result over a range, and log2 of the sum of its weights, is a part. The own keys follow as in
 // cached_attention (SECOND), and where a row's result is stored it is joined with the row's parts, in their order: a sum of numbers of a few ranges
-// each, in fp32, that does not depend on which block was first.
+// each, in fp32, that does not depend on which block was first. Where sequences have so many rows that tiles of 128 are full with each alone, a
+// block walks over the keys of the prefix and then over the own ones (WHOLE), and there are no parts.
 #include "cached_attention_few.cuh"
 
 namespace nbc {
@@ -53,6 +54,10 @@ static cudaError_t first_few(const AttendArgs& a, cudaStream_t stream) {
 }
 template <typename T, int D>
 static cudaError_t launch_both(const AttendArgs& first, const FirstCut& f, const AttendArgs& second, const Cut& c, int* status, cudaStream_t stream) {
+  if (f.splits == 0) {                     // WHOLE
+    const cudaError_t e = launch_many<D, WHOLE>(second, 0, status, stream);
+    return e != cudaSuccess || c.splits == 1 ? e : join<T, D, false, ALONE>(second, stream);
+  }
   const cudaError_t e = f.rows == 128 ? launch_many<D, FIRST>(first, f.q_tiles, status, stream)
                       : f.rows == 8 ? first_few<T, D, 1>(first, stream) : first_few<T, D, 2>(first, stream);
   return e != cudaSuccess ? e : launch_attend<T, D, SECOND>(second, c, status, stream);
@@ -61,18 +66,28 @@ static cudaError_t launch_both(const AttendArgs& first, const FirstCut& f, const
 // Floats of the parts; what follows them starts on a boundary of 16 bytes.
 static long long first_floats(long long rows, int splits, int head_dim) { return (rows * splits * (head_dim + 1) + 3) / 4 * 4; }
 struct Cuts {
+  bool whole;
   FirstCut first;
-  Cut second;
+  Cut second;                    // whole: of all keys
 };
 static Cuts cut_both(int batch, int fresh, int heads, int kv_heads, int head_dim, long long prefix_room, long long room, int fp32) {
   const long long rows = (long long)batch * fresh * heads;
   const int own_rows = fresh * (heads / kv_heads);
   const Cut c = cut(batch, own_rows, rows, kv_heads, head_dim, room, fp32);
-  return Cuts{cut_first(static_cast<int>(rows / kv_heads), kv_heads, prefix_room, fp32, c, batch, own_rows, room), c};
+  const Cuts both = {false, cut_first(static_cast<int>(rows / kv_heads), kv_heads, prefix_room, fp32, c, batch, own_rows, room), c};
+  if (c.rows != 128 || both.first.rows != 128) return both;
+  // Two kernels pack the rows of all sequences densely for the prefix; one does not leave and join parts, and starts its blocks once. SM * us for each head and
+  // sequence, from the times at cut_first: blocks of 256 rows, the last of 128 or fewer.
+  const double tiles = static_cast<double>((prefix_room + 127) / 128), own = static_cast<double>((room + 127) / 128);
+  const int full = own_rows / 256, left = (own_rows - full * 256 + 127) / 128;
+  const double for_tile = 3.3 * full + (left == 2 ? 3.3 : left == 1 ? 2.2 : 0.0), blocks = full + (left > 0);
+  const double two = own_rows / 256.0 * (3.3 * tiles + 9.0) + for_tile * own + 13.0 * blocks, one = for_tile * (tiles + own) + 9.0 * blocks;
+  if (two <= one) return both;
+  return Cuts{true, FirstCut{128, 0, 0}, cut(batch, own_rows, rows, kv_heads, head_dim, prefix_room + room, fp32)};
 }
 }  // namespace nbc
 
-// Scratch of a call with these sizes, in floats.
+// Scratch of a call with these sizes, in floats (0: none).
 extern "C" long long nb_shared_prefix_scratch(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int prefix_columns, int columns, int fp32) {
   using namespace nbc;
   const long long rows = (long long)batch * fresh * heads;
@@ -81,8 +96,10 @@ extern "C" long long nb_shared_prefix_scratch(int batch, int fresh, int heads, i
   return first_floats(rows, c.first.splits, head_dim) + c.second.scratch;
 }
 // Kernels that a call launches.
-extern "C" int nb_shared_prefix_launches(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int columns, int fp32) {
-  return nbc::cut(batch, fresh * (heads / kv_heads), (long long)batch * fresh * heads, kv_heads, head_dim, (long long)columns * block, fp32).scratch > 0 ? 3 : 2;
+extern "C" int nb_shared_prefix_launches(int batch, int fresh, int heads, int kv_heads, int head_dim, int block, int prefix_columns, int columns, int fp32) {
+  using namespace nbc;
+  const Cuts c = cut_both(batch, fresh, heads, kv_heads, head_dim, (long long)prefix_columns * block, (long long)columns * block, fp32);
+  return (c.whole ? 1 : 2) + (c.second.scratch > 0);
 }
 
 // Strides of q as the rows of one sequence: q_sb = fresh * q_st, or fresh is 1. wide: bit 0 prefix_table, 1 prefix_length, 2 table, 3 past, 4 count are
@@ -102,11 +119,12 @@ extern "C" int nb_shared_prefix_attention(const void* q, const void* k_codes, co
   a.block_log = block == 16 ? 4 : block == 32 ? 5 : block == 64 ? 6 : block == 128 ? 7 : -1;
   a.scale_log2 = scale * 1.4426950408889634f;
   const long long rows = (long long)batch * fresh * heads;
-  if (a.block_log < 0 || (head_dim != 64 && head_dim != 128) || rows > 0x7fffffffll || scratch == nullptr) return -1;
+  if (a.block_log < 0 || (head_dim != 64 && head_dim != 128) || rows > 0x7fffffffll) return -1;
   if (batch > 1 && fresh > 1 && q_sb != fresh * q_st) return -1;
   const Cuts cuts = cut_both(batch, fresh, heads, kv_heads, head_dim, (long long)prefix_columns * block, (long long)columns * block, fp32);
   const FirstCut& f = cuts.first;
   const Cut& c = cuts.second;
+  if ((f.splits > 0 || c.scratch > 0) && scratch == nullptr) return -1;
   AttendArgs first = a;
   first.table = Table{Whole{prefix_table, wide & 1}, prefix_columns, blocks};
   first.limit = Whole{prefix_length, wide >> 1 & 1};
@@ -119,6 +137,7 @@ extern "C" int nb_shared_prefix_attention(const void* q, const void* k_codes, co
   a.past = Whole{past, wide >> 3 & 1}, a.count = Whole{count, wide >> 4 & 1};
   a.batch = batch, a.fresh = fresh, a.causal = causal;
   a.first_o = first.part_o, a.first_w = first.part_w, a.first_parts = f.splits;
+  a.limit = first.limit, a.first_table = first.table;
   set_parts(a, c, scratch, head_dim);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (fp32) return head_dim == 64 ? launch_both<float, 64>(first, f, a, c, status, s) : launch_both<float, 128>(first, f, a, c, status, s);

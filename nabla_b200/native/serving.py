@@ -28,7 +28,7 @@ _FUNCTIONS = {
     "libnb_answers.so": {
         "nb_shared_prefix_attention": (c_int, [c_vp] * 11 + [c_int] * 10 + [c_ll] * 3 + [c_f, c_int, c_vp, c_int, c_vp, c_vp]),
         "nb_shared_prefix_scratch": (c_ll, [c_int] * 9),
-        "nb_shared_prefix_launches": (c_int, [c_int] * 8),
+        "nb_shared_prefix_launches": (c_int, [c_int] * 9),
         "nb_sample_tokens": (c_int, [c_vp] * 7 + [c_int] * 4 + [c_vp]),
     },
 }
@@ -127,7 +127,7 @@ def shared_prefix_attention(q, k_codes, k_scale, v_codes, v_scale, prefix_table,
     out = torch.empty((b, t, hq, d), dtype=q.dtype, device=q.device)
     fp32 = int(q.dtype == torch.float32)
     floats, launches = _prefix_scratch(b, t, hq, h, d, n, prefix_table.shape[0], table.shape[1], fp32)
-    part = torch.empty(floats, dtype=torch.float32, device=q.device)
+    part = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     _ok(_L("libnb_answers.so").nb_shared_prefix_attention(ptr(q), ptr(k_codes), ptr(k_scale), ptr(v_codes), ptr(v_scale), ptr(out), ptr(prefix_table), ptr(prefix_length),
                                         ptr(table), ptr(past), ptr(count), _wide(prefix_table, prefix_length, table, past, count), b, t, hq, h, d, n, blocks,
                                         prefix_table.shape[0], table.shape[1], *q.stride()[:3], float(scale), int(causal), ptr(part), fp32,
@@ -139,7 +139,7 @@ def shared_prefix_attention(q, k_codes, k_scale, v_codes, v_scale, prefix_table,
 def _prefix_scratch(b, t, hq, h, d, n, prefix_columns, columns, fp32):
     """Floats of scratch and launches, functions of the sizes alone."""
     floats = _L("libnb_answers.so").nb_shared_prefix_scratch(b, t, hq, h, d, n, prefix_columns, columns, fp32)
-    return floats, _L("libnb_answers.so").nb_shared_prefix_launches(b, t, hq, h, d, n, columns, fp32)
+    return floats, _L("libnb_answers.so").nb_shared_prefix_launches(b, t, hq, h, d, n, prefix_columns, columns, fp32)
 
 
 def adjust_logits(logits, history, length, prompt, repetition, presence, frequency, bias, allowed):

@@ -199,6 +199,8 @@ def test_missing_blocks_far_scales_and_undefined_ones(new, device):
     (64, 1, 16, 4, 64, 8001, 900, "bf16"), (16, 1, 16, 2, 128, 20001, 700, "bf16"), (4, 1, 16, 16, 64, 1000, 200, "bf16"), (200, 1, 8, 8, 64, 3000, 60, "bf16"),
     (1030, 1, 4, 2, 64, 500, 90, "bf16"), (3, 1, 4, 1, 64, 9000, 30, "bf16"), (8, 5, 12, 4, 16, 1501, 300, "fp32"), (50, 1, 8, 2, 64, 3000, 500, "fp32"),
     (12, 64, 8, 2, 64, 700, 100, "bf16"), (2, 700, 8, 2, 64, 1111, 50, "bf16"), (5, 40, 4, 2, 32, 900, 2000, "bf16"), (3, 50, 8, 1, 64, 600, 80, "fp32"),
+    # both sides of where one kernel walks over the prefix and the own keys: rows of a sequence that fill tiles of 128 badly and well, few tiles in all
+    (9, 70, 8, 2, 64, 1500, 300, "bf16"), (24, 33, 16, 4, 16, 777, 20, "bf16"), (1, 300, 4, 2, 32, 5000, 10, "bf16"), (2, 520, 4, 4, 64, 129, 0, "bf16"),
 ])
 def test_ragged_batches(b, new, hq, h, n, prefix, longest, dtype, d):
     """Idle sequences and short counts; scratch that holds garbage; the same bits every time, in a graph too."""
