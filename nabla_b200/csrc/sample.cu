@@ -207,8 +207,10 @@ struct Team {
     for (int r = 0; r < blocks; ++r) x += all[r][0], y += all[r][1], z += all[r][2];
   }
   __device__ __forceinline__ void clear() const {
-    uint4* bins = reinterpret_cast<uint4*>(CLUSTER ? s.own_bins : s.bins);
-    for (int i = threadIdx.x; i < BINS / 4; i += SAMPLE_THREADS) bins[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < BINS / 4; i += SAMPLE_THREADS) {
+      reinterpret_cast<uint4*>(s.bins)[i] = make_uint4(0, 0, 0, 0);
+      if (CLUSTER) reinterpret_cast<uint4*>(s.own_bins)[i] = make_uint4(0, 0, 0, 0);
+    }
   }
   // s.bins counts the tokens of the row for which `f` (token, logit) names a bin below BINS
   template <typename T, typename F>
@@ -238,7 +240,7 @@ struct Team {
       __syncthreads();
     }
   }
-  // s.order and s.weights (1 for `counted`) list the tokens of the row that `f` wants; their number. No more than LIST of them.
+  // s.order and s.weights (1 for `counted`) list the tokens of the row that `f` wants; their number. Where that is more than LIST, some LIST of them.
   template <typename T, typename F>
   __device__ __forceinline__ int list(const LogitRow<T>& row, const Weigher& weigh, bool counted, F&& f) {
     u64* own = CLUSTER ? s.own_order : s.order;
@@ -251,16 +253,15 @@ struct Team {
       if (i < LIST) own[i] = order_of(z, v);
     });
     __syncthreads();
-    int n = min(s.entries, LIST);
+    int n = s.entries;
     if constexpr (CLUSTER) {
       const auto all = told<1>(static_cast<u64>(n));
       n = 0;
       for (int r = 0; r < blocks; ++r) {
         const int m = static_cast<int>(all[r][0]);
         const u64* from = of(s.own_order, r);
-        for (int i = threadIdx.x; i < m; i += SAMPLE_THREADS)
-          if (n + i < LIST) s.order[n + i] = from[i];
-        n = min(LIST, n + m);
+        for (int i = threadIdx.x; i < m && n + i < LIST; i += SAMPLE_THREADS) s.order[n + i] = from[i];
+        n += m;
       }
       __syncthreads();
     }
@@ -403,12 +404,13 @@ __device__ __noinline__ u64 last_kept(Team<CLUSTER>& team, const LogitRow<T>& ro
   }
   // (as numbers first: above the largest there is no number, nothing is at least that)
   const float z_low = number_of(static_cast<uint32_t>(at.low >> 32)), z_above = number_of(static_cast<uint32_t>(at.high >> 32) + 1);
-  const int n = team.list(row, weigh, COUNT, [&](int v, float z) {
+  const int listed = team.list(row, weigh, COUNT, [&](int v, float z) {
     if (!(z >= z_low) || z >= z_above) return false;
     const u64 q = order_of(z, v);
     return q >= at.low && q <= at.high;
   });
-  entries = whole ? n : -1;
+  const int n = min(listed, LIST);         // (more only where the levels ran out)
+  entries = whole && listed <= LIST ? n : -1;
   u64 kept = ~0ull;
   if (static_cast<int>(threadIdx.x) < n) {
     const u64 q = s.order[threadIdx.x];
@@ -425,12 +427,13 @@ __device__ __forceinline__ u64 target_of(float u, u64 all) {
   return to < static_cast<double>(all) ? min(static_cast<u64>(to), all - 1) : all - 1;
 }
 
-template <typename T, bool CLUSTER>
-__global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleArgs a) {
+// FILTERED: with top-k or top-p.
+template <typename T, bool CLUSTER, bool FILTERED>
+__global__ void __launch_bounds__(SAMPLE_THREADS, FILTERED ? 2 : 3) sample_kernel(const SampleArgs a) {
   __shared__ __align__(16) SampleShared s;
   if (threadIdx.x < 32) s.roots[threadIdx.x] = exp2(-static_cast<double>(threadIdx.x) / 32.0);
   Team<CLUSTER> team(s, a.blocks);
-  team.clear();
+  if (FILTERED) team.clear();
   if constexpr (CLUSTER) team.sync();      // every block of the cluster runs before another writes to it
   follow_grid();
   const int b = CLUSTER ? blockIdx.x / a.blocks : blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -450,46 +453,40 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
     if (threadIdx.x == 0 && team.rank == 0) a.out[b] = first == 0 ? -1ll : token_of(first);
     return;
   }
-  const bool by_count = asked > 0 && asked < a.vocab, by_share = p < 1.f;
+  const bool by_count = FILTERED && asked > 0 && asked < a.vocab, by_share = FILTERED && p < 1.f;
   const Weigher weigh(top, temperature, s.roots);
-  // the least weight that min-p keeps: w >= m where the whole number of w is at least that of m, rounded up (m is no whole number but by chance)
+  // the least key in (lo, hi] for which `good` holds, which holds from some key on and at hi. A warp tries 32 keys at once
+  const auto least_key = [&](uint32_t lo, uint32_t hi, auto&& good) {
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo + 31) / 32, mid = lo + min(hi - lo, step * (lane + 1));
+      const int k = __ffs(static_cast<int>(__ballot_sync(0xffffffffu, mid >= hi || good(number_of(mid))))) - 1;      // (the last lane is at hi)
+      hi = lo + min(hi - lo, step * (k + 1));
+      lo += step * k;
+    }
+    return static_cast<u64>(hi) << 32;
+  };
+  // min-p: a whole number of w counts as w >= m where it is at least that of m, rounded up (m is no whole number but by chance). Its border in the order:
   const u64 least_kept = least > 0.f ? static_cast<u64>(ceil(fmin(static_cast<double>(least), 1.0) * UNIT_WEIGHT)) : 0;
+  const auto least_border = [&] {
+    if (least_kept == 0) return 0ull;
+    __syncthreads();
+    if (warp == 0) {
+      const u64 at = least_key(key_of(-INFINITY), key_of(top), [&](float z) { return weigh.fixed(z) >= least_kept; });
+      if (lane == 0) s.edges[0] = at;
+    }
+    __syncthreads();
+    return s.edges[0];
+  };
   u64 last = 0;                            // of the order, the last that is kept
-  u64 above_mine = 0;                      // top-p alone: what this warp has above the steps that hold the border, and how many tokens of these are in the list
+  // top-p: what this warp has above the bin that holds the border, where that begins, how many tokens of it are in the list (-1: not known); what it has up to the
+  // border of min-p
+  u64 above_mine = 0, least_mine = 0, bin_high = 0;
   int listed = -1;
-  if (by_count || by_share) {
+  u64 least_order = 0;
+  if (FILTERED && (by_count || by_share)) {
     const auto in_bins = [&](int v, float z) { return weigh.bin(z); };
-    team.count(row, in_bins, false);
-    // the least key whose bin is below `b`: bins fall as keys grow. A warp tries 31 keys at once
-    const auto edge = [&](int b) {
-      uint32_t lo = key_of(-INFINITY), hi = key_of(weigh.top) + 1;       // in (lo, hi]
-      while (hi - lo > 1) {
-        const uint32_t step = (hi - lo + 31) / 32, mid = lo + min(hi - lo, step * (lane + 1));
-        const uint32_t below = __ballot_sync(0xffffffffu, mid >= hi || weigh.bin(number_of(mid)) < b);
-        const int k = __ffs(static_cast<int>(below)) - 1;                // the first of them (the last is at hi)
-        const uint32_t top_key = lo + min(hi - lo, step * (k + 1));
-        lo += step * k, hi = top_key;
-      }
-      return static_cast<u64>(hi) << 32;
-    };
-    const auto stretch = [&](int first, int last_bin) {      // of bins [first, last_bin]
-      __syncthreads();
-      if (warp < 2) {
-        const u64 at = edge(warp ? last_bin + 1 : first);
-        if (lane == 0) s.edges[warp] = at;
-      }
-      __syncthreads();
-      return Stretch{s.edges[1], s.edges[0] - 1, 0, 0};
-    };
-    const auto about = [&](int i) { return exp2f(static_cast<float>(i) * (-FAR / (BINS - 1))); };
-    int end = BINS, end_tokens = 0;        // the bin that top-k ends in, and how many of it are kept
-    find_bin<int, false>(s, by_count ? static_cast<int>(asked) : 0x7fffffff, [&](int i) { return static_cast<int>(s.bins[i]); });
-    const int c = s.found, before = s.before, total = s.total;
-    const bool cut = by_count && total > asked;
-    const int upto = before + static_cast<int>(s.bins[c]);   // tokens up to the bin that top-k ends in, or all of weight
-    if (upto <= LIST) {
-      // ---- all that may be kept is in a list, one entry for each thread
-      const int n = team.list(row, weigh, false, [&](int v, float z) { return weigh.bin(z) <= c; });
+    // ---- all that may be kept is in the list, one entry for each thread: the first `asked` of these, all where that is 0
+    const auto finish = [&](int n, long long asked) {
       if constexpr (CLUSTER) {
         team.sync();                       // (its lists have been read)
         if (team.rank != 0) return;
@@ -501,7 +498,7 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
       if (mine)
         for (int j = 0; j < n; ++j)
           if (s.order[j] > q) ++place, sum += s.weights[j];
-      bool kept = mine && (!cut || place < asked);
+      bool kept = mine && (asked == 0 || place < asked);
       if (by_share) {
         const double want = static_cast<double>(p) * static_cast<double>(block_sum(s, kept ? w : 0));
         kept = kept && (place == 0 || static_cast<double>(sum) < want);
@@ -515,8 +512,27 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
       for (int j = 0; j < n; ++j) front += static_cast<uint32_t>(s.order[j]) > static_cast<uint32_t>(q) ? s.weights[j] : 0;
       const u64 target = target_of(u, all);
       if (target >= front && target < front + w) a.out[b] = token_of(q);
-      return;
-    }
+    };
+    const auto bin_count = [&](int i) { return static_cast<int>(s.bins[i]); };
+    team.count(row, in_bins, false);
+    // how far the first k, or all of weight, reach
+    find_bin<int, false>(s, by_count ? static_cast<int>(asked) : 0x7fffffff, bin_count);
+    const int c = s.found, before = s.before, total = s.total;
+    const bool cut = by_count && total > asked;
+    if (before + static_cast<int>(s.bins[c]) <= LIST)
+      return finish(team.list(row, weigh, false, [&](int v, float z) { return weigh.bin(z) <= c; }), cut ? asked : 0);
+    const auto stretch = [&](int first, int last_bin) {      // of bins [first, last_bin]: bins fall as keys grow
+      __syncthreads();
+      if (warp < 2) {
+        const int b = warp ? last_bin + 1 : first;
+        const u64 at = least_key(key_of(-INFINITY), key_of(top) + 1, [&](float z) { return weigh.bin(z) < b; });
+        if (lane == 0) s.edges[warp] = at;
+      }
+      __syncthreads();
+      return Stretch{s.edges[1], s.edges[0] - 1, 0, 0};
+    };
+    const auto about = [&](int i) { return exp2f(static_cast<float>(i) * (-FAR / (BINS - 1))); };
+    int end = BINS, end_tokens = 0;        // the bin that top-k ends in, and how many of it are kept
     if (cut) {
       end = c, end_tokens = static_cast<int>(asked) - before;
       Stretch x = stretch(c, c);
@@ -529,19 +545,22 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
       find_bin<float, true>(s, p, [&](int i) { return i > end ? 0.f : static_cast<float>(i == end ? end_tokens : static_cast<int>(s.bins[i])) * about(i); });
       const int first = max(s.found, 0), last_bin = first;     // (the estimate is seldom off by a bin: what it names is checked)
       Stretch x = stretch(first, last_bin);
+      least_order = least_border();
       // the border of top-k as a number and an id, and the stretch as numbers (above the largest: no number, nothing is at least that)
       const float z_last = last ? number_of(static_cast<uint32_t>(last >> 32)) : -INFINITY, z_low = number_of(static_cast<uint32_t>(x.low >> 32)),
-                  z_above = number_of(static_cast<uint32_t>(x.high >> 32) + 1);
+                  z_above = number_of(static_cast<uint32_t>(x.high >> 32) + 1), z_least = least_order ? number_of(static_cast<uint32_t>(least_order >> 32)) : INFINITY;
+      bin_high = x.high;
       const int v_last = last ? token_of(last) : -1;
       u64 all = 0, above = 0, within = 0;
       row.each([&](int v, float z) {
         if (!(z > z_last || (z == z_last && v <= v_last))) return;
         const u64 w = weigh.fixed(z);
         all += w;
+        if (z >= z_least) least_mine += w;
         if (z >= z_above) above += w;
         else if (z >= z_low) within += w;
       });
-      above_mine = over_warp_sum(above);
+      above_mine = over_warp_sum(above), least_mine = over_warp_sum(least_mine);
       team.sums_of(all, above, within);
       const double want = fmax(static_cast<double>(p) * static_cast<double>(all), 0.5);     // (the first is kept)
       bool here = false;
@@ -557,19 +576,20 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, 2) sample_kernel(const SampleA
       }
       x.low = max(x.low, last);
       last = last_kept<T, CLUSTER, false>(team, row, weigh, x, want, listed);
-      if (!here) listed = -1;
+      if (!here) listed = -1, bin_high = 0;
     }
   }
   // ---- the draw
+  if (!by_share) least_order = least_border();
+  const u64 border = last;
+  last = max(last, least_order);
   const float z_last = last ? number_of(static_cast<uint32_t>(last >> 32)) : -INFINITY;
-  const int v_last = last ? token_of(last) : -1;
-  const auto drawn = [&](int v, float z) {
-    if (!(z > z_last || (z == z_last && v <= v_last))) return 0ull;
-    const u64 w = weigh.fixed(z);
-    return w >= least_kept ? w : 0ull;
-  };
+  const int v_last = last ? (last > border ? 0x7fffffff : token_of(last)) : -1;      // (min-p keeps all with the logit of its border)
+  const auto drawn = [&](int v, float z) { return z > z_last || (z == z_last && v <= v_last) ? weigh.fixed(z) : 0ull; };
   u64 sum = 0;
-  if (listed >= 0 && least_kept == 0) {    // the sums are known: those above the steps of the border, and in these what the list has up to it
+  if (FILTERED && bin_high && last > bin_high) {             // the sums are known: up to the border of min-p,
+    sum = least_mine;
+  } else if (FILTERED && listed >= 0) {    // or those above the bin of the border and what the list has of that
     const int me = team.rank * SAMPLE_WARPS + warp;
     for (int i = lane; i < listed; i += 32) {
       const u64 q = s.order[i];
@@ -651,7 +671,8 @@ static cudaError_t launch_sample(SampleArgs a, int batch, cudaStream_t stream) {
     cfg.numAttrs = 1;
   }
   nb::set_following(cfg);
-  return cudaLaunchKernelEx(&cfg, a.blocks > 1 ? sample_kernel<T, true> : sample_kernel<T, false>, a);
+  if (a.top_k.p == nullptr && a.top_p == nullptr) return cudaLaunchKernelEx(&cfg, a.blocks > 1 ? sample_kernel<T, true, false> : sample_kernel<T, false, false>, a);
+  return cudaLaunchKernelEx(&cfg, a.blocks > 1 ? sample_kernel<T, true, true> : sample_kernel<T, false, true>, a);
 }
 
 }  // namespace nbc
