@@ -10,6 +10,10 @@
 // puts their cosines and sines into shared memory first. An angle is taken in turns, in 64 bits, and only what is left of a whole turn goes into
 // 32 (a position of 10^6 would be off by 0.06 in 32 bits); that remainder is carried in two parts, so cosines and sines are off by about a unit in
 // the last place.
+//
+// Bound by memory: 8 x 2048 tokens of 16 heads of 128 with their values in bf16 take 73 us forward, 403 MB, 5.5 TB/s, and 103 us backward, 537 MB, 5.2 TB/s (a plain
+// copy 6.5); 4 x 2048 tokens of 16 + 16 heads in fp32 54 and 83, 4.9 TB/s. Before the ring, with 2 or 4 tokens in registers, 90 to 108 and 165 to 378 (spilled). Three
+// to eight stages of the ring are alike. Small calls are bound by the start of the launches, 6 us each way on the device.
 #include "kv_cache.cuh"
 
 namespace nbc {

@@ -243,7 +243,8 @@ def _unpacked(qkv: torch.Tensor, head_dim: int):
     b, t, w = qkv.shape
     if qkv.stride(2) != 1:
         qkv = qkv.contiguous()
-    return torch.unbind(qkv.view(b, t, w // (3 * head_dim), 3, head_dim), 3)
+    parts = qkv.view(b, t, w // (3 * head_dim), 3, head_dim)
+    return tuple(parts[:, :, :, i] for i in range(3))           # (selections: a call with other views is not written down)
 
 
 _op, _bwd, _packed, _packed_bwd = NormRotaryOp(), NormRotaryBwdOp(), PackedNormRotaryOp(), PackedNormRotaryBwdOp()

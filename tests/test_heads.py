@@ -339,3 +339,21 @@ def test_refusals():
     with pytest.raises(ValueError):
         F.packed_norm_rotary(q, 64, pos)
     assert heads.MOST_DIM == 256
+
+
+@pytest.mark.gpu
+def test_compiled_calls_are_written_down():
+    """Forward and backward of both forms are replayed without Python: recorded at the second call of a signature."""
+    from nabla_b200.transforms import tape
+
+    if tape.module() is None:
+        pytest.skip("libnb_replay.so is not built here")
+    q, k, cq, ck, gq, gk, pos = make(CASES[8], "cuda")
+    b, t, h, d = q.shape
+    qkv = torch.stack([q, k, q], 3).reshape(b, t, -1)
+    f = nb.compile(lambda q, k, p, a, b, cq, ck: (lambda y, pull: (y, pull((cq, ck))))(*nb.vjp(lambda *x: F.norm_rotary(x[0], x[1], p, *x[2:]), q, k, a, b, create_graph=False)))
+    g = nb.compile(lambda x, p, a, b, c: (lambda y, pull: (y, pull(c)))(*nb.vjp(lambda *z: F.packed_norm_rotary(z[0], d, p, *z[1:]), x, a, b, create_graph=False)))
+    for call, args in ((f, (q, k, pos, gq, gk, cq, ck)), (g, (qkv, pos, gq, gk, qkv.clone()))):       # (arguments that share memory are not taken)
+        for _ in range(4):
+            call(*(T(x) for x in args))
+        assert call._taped is not None and bool(call._taped[0]), call.tape_refused

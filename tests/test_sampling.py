@@ -258,3 +258,16 @@ def test_refusals():
             F.sample_tokens(*args, **kw)
     with pytest.raises(ValueError):
         nb.vmap(lambda x: F.sample_tokens(x, u))(T(torch.zeros(3, 2, 5)))
+
+
+@pytest.mark.gpu
+def test_a_compiled_draw_is_written_down():
+    from nabla_b200.transforms import tape
+
+    if tape.module() is None:
+        pytest.skip("libnb_replay.so is not built here")
+    z, u, kw = rows("cuda", 6, 9, 2000, 3.0, torch.float32)
+    f = nb.compile(lambda z, u, *x: F.sample_tokens(z, u, **dict(zip(kw, x))))
+    for _ in range(4):
+        f(*[T(x) for x in (z, u, *kw.values())])
+    assert f._taped is not None and bool(f._taped[0]), f.tape_refused

@@ -351,6 +351,21 @@ def test_steps_in_a_row_see_what_was_just_written(b, hq, h, columns, dtype):
         assert all(torch.equal(x, y) for x, y in zip(run(False), want))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [CASES[1], CASES[3], CASES[10], CASES[12]])
+def test_a_compiled_call_is_written_down(case):
+    from nabla_b200.transforms import tape
+
+    if tape.module() is None:
+        pytest.skip("libnb_replay.so is not built here")
+    q, cache, *rest = make(case, "cuda")
+    rest = [x for x in rest if x is not None]
+    f = nb.compile(lambda q, c, *x: F.shared_prefix_attention(q, c, *x))
+    for _ in range(4):
+        f(T(q), wrap(cache), *(T(x) for x in rest))
+    assert f._taped is not None and bool(f._taped[0]), f.tape_refused
+
+
 _CHECKED = """
 import torch
 import nabla_b200 as nb
