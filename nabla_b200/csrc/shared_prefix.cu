@@ -9,7 +9,7 @@
 // each, in fp32, that does not depend on which block was first. Where sequences have so many rows that tiles of 128 are full with each alone, a
 // block walks over the keys of the prefix and then over the own ones (WHOLE), and there are no parts.
 //
-// 64 sequences of 50 to 1000 behind 8001 tokens, 16 heads over 4 of 128: 27 us (each alone over the whole text 226); 16 of up to 2000 behind 60001, 16 over 2: 43;
+// 64 sequences of 50 to 1000 behind 8001 tokens, 16 heads over 4 of 128: 27 us (each over its whole text 71); 16 of up to 2000 behind 60001, 16 over 2: 43;
 // 4 behind 1000: 9 on the device. What bounds it: the start and end of blocks (7 us of those of 128-row tiles) and the chain of product, exponentials and product
 // of few tiles of keys for each block; for the last, starts. Prompts of 32 x 200 behind 2048: 193 us, exponentials (cached_attention_tcgen05.cu).
 #include "cached_attention_few.cuh"
