@@ -22,6 +22,8 @@ class OpShardingRule:
     input_mappings: list[Mapping]
     output_mappings: list[Mapping]
     factor_sizes: dict[str, int] = field(default_factory=dict)
+    # of an output, the factors that it is a sum over; None, or behind the end of the list: all input factors that it does not carry
+    summed: list[set[str] | None] = field(default_factory=list)
 
     def get_all_factors(self) -> set[str]:
         out: set[str] = set()
@@ -239,7 +241,8 @@ def infer_from_rule(rule: OpShardingRule, input_specs: Sequence[ShardingSpec | N
     # was summed away on the way to it (e.g. the row factors for LayerNorm's dgamma)
     own = {f for fs in out_map.values() for f in fs}
     in_factors = {f for m in rule.input_mappings for fs in m.values() for f in fs}
-    contracting = in_factors - own
+    summed = rule.summed[output_index] if output_index < len(rule.summed) else None
+    contracting = (in_factors if summed is None else in_factors & summed) - own
     rank = max(out_map.keys(), default=-1) + 1
     used: set[str] = set()
     dims: list[DimSpec] = []

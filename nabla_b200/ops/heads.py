@@ -120,8 +120,8 @@ class NormRotaryOp(_Heads):
         return tuple(_forward(x, g, angles, eps, rotary_dim, interleaved) for x, g in zip((q, k), gains))
 
     def sharding_rule(self, input_shapes, output_shapes, **kw):
-        m, p = _rules(input_shapes[2], ("b", "s", "h", "bcast_d"))
-        return OpShardingRule([dict(m), dict(m), p] + [{0: ["bcast_g"]} for _ in input_shapes[3:]], [dict(m), dict(m)])
+        (q, k), p = _head_rules(input_shapes[:2], input_shapes[2])
+        return OpShardingRule([dict(q), dict(k), p] + [{0: ["bcast_g"]} for _ in input_shapes[3:]], [dict(q), dict(k)], summed=[set(), set()])
 
     def vjp_rule(self, primals, cot, outputs, kwargs):
         if cot[0] is None and cot[1] is None:
@@ -154,10 +154,12 @@ class NormRotaryBwdOp(_Heads):
         (a, ga), (b, gb) = (_backward(dy, x, g, angles, eps, rotary_dim, interleaved) for dy, x, g in zip((dq, dk), (q, k), gains))
         return (a, b, *(g for g in (ga, gb) if g is not None))
 
-    def sharding_rule(self, input_shapes, output_shapes, **kw):
-        m, p = _rules(input_shapes[4], ("b", "s", "h", "bcast_d"))
-        n = len(input_shapes) - 5
-        return OpShardingRule([dict(m) for _ in range(4)] + [p] + [{0: ["bcast_g"]} for _ in range(n)], [dict(m), dict(m)] + [{0: ["gn"]} for _ in range(n)])
+    def sharding_rule(self, input_shapes, output_shapes, *, which: str, **kw):
+        (q, k), p = _head_rules(input_shapes[2:4], input_shapes[4])
+        # a gain's gradient is a sum over its own heads: one head, which every device has whole beside others that are split, adds no sum over devices
+        of = {"q": q, "k": k}
+        return OpShardingRule([dict(q), dict(k), dict(q), dict(k), p] + [{0: ["bcast_g"]} for _ in which], [dict(q), dict(k)] + [{0: ["gn"]} for _ in which],
+                              summed=[set(), set()] + [{f for fs in of[name].values() for f in fs} for name in which])
 
     def decomposed(self, dq, dk, q, k, positions, *gains, which, **kw):
         from ..transforms.vjp import vjp
@@ -232,6 +234,12 @@ class PackedNormRotaryBwdOp(_Heads):
 
         _, pull = vjp(lambda x, *g: _packed.decomposed(x, positions, *g, which=which, **kw), qkv, *gains)
         return tuple(pull(dy))
+
+
+def _head_rules(shapes, positions_shape):
+    """Rules of q and k, whose heads are split alike, but one head, which is not split, and of the positions."""
+    m, p = _rules(positions_shape, ("b", "s", "h", "bcast_d"))
+    return [m if int(s[2]) != 1 else {**m, 2: ["bcast_h"]} for s in shapes], p
 
 
 def _rules(positions_shape, factors):

@@ -312,6 +312,32 @@ def test_split_over_a_mesh(axes, mesh_2x4, monkeypatch):
         assert (a - c).abs().max() <= 2.0 ** -15 * c.abs().max()         # the same fp32 sums in parts
 
 
+@pytest.mark.parametrize("heads_", [(8, 1), (1, 8), (8, 2), (6, 3), (1, 1)])
+@pytest.mark.parametrize("axes", [("dp", None, "tp"), (None, "dp", "tp"), (None, "tp", None)])
+def test_unlike_counts_of_heads_split_over_a_mesh(axes, heads_, mesh_2x4, monkeypatch):
+    """One head is whole on every device and others are not: its gain's gradient is a sum over tokens, not over devices."""
+    monkeypatch.setenv("NABLA_B200_FUSED", "1")
+    g = torch.Generator().manual_seed(5)
+    b, t, d = 2, 8, 32
+    xs = [torch.randn((b, t, n, d), generator=g) for n in heads_] + [torch.randn((d,), generator=g) for _ in range(2)]
+    cots = [torch.randn((b, t, n, d), generator=g) for n in heads_]
+    pos = T(torch.arange(t))
+
+    def value(q, k, gq, gk):
+        y = F.norm_rotary(q, k, pos, gq, gk)
+        return (y[0] * T(cots[0])).sum() + (y[1] * T(cots[1])).sum()
+
+    plain = nb.grad(value, argnums=(0, 1, 2, 3))(*(T(x) for x in xs))
+    for k_axes in (axes, (*axes[:2], None)):
+        split = [T(xs[0]).shard(mesh_2x4, (*axes, None)), T(xs[1]).shard(mesh_2x4, (*k_axes, None))] + [T(x).shard(mesh_2x4, (None,)) for x in xs[2:]]
+        y = F.norm_rotary(*split[:2], pos, *split[2:])
+        for a, c in zip(y, F.norm_rotary(*(T(x) for x in xs[:2]), pos, *(T(x) for x in xs[2:]))):
+            assert torch.equal(torch.from_numpy(a.to_numpy()), c.to_torch())         # the same operations, head by head
+        for a, c in zip(nb.grad(value, argnums=(0, 1, 2, 3))(*split), plain):
+            a, c = torch.from_numpy(a.to_numpy()).double(), c.to_torch().double()
+            assert (a - c).abs().max() <= 2.0 ** -15 * c.abs().max()     # the same fp32 sums in parts
+
+
 def test_refusals():
     q, k, pos = T(torch.zeros(2, 3, 4, 64)), T(torch.zeros(2, 3, 2, 64)), T(torch.zeros(3, dtype=torch.int32))
     gain = T(torch.ones(64))
