@@ -7,7 +7,8 @@ no block (negative, or not below the number of blocks) is a place without tokens
 sees no key there. Sequences may share blocks that are only read; a block that a call writes belongs to one sequence.
 
 Each is one ``Operation`` with hand-written kernels on CUDA (``csrc/kv_cache.cu``, ``cached_attention.cu``, ``shared_prefix.cu``,
-``logits.cu``, ``sample.cu``) and an equivalent torch expression on the CPU. They have no derivatives. On a mesh the heads of the cache may be split as those of the model are.
+``logits.cu``, ``sample.cu``) and an equivalent torch expression on the CPU. They have no derivatives. On a mesh the heads of the cache may be split as those of the model are, where
+every device then has the query heads of its own heads of the cache (attention refuses other splits).
 """
 from __future__ import annotations
 
@@ -367,6 +368,19 @@ def _same_device(*ts: Tensor) -> None:
     _need(len(devices) == 1, f"operands on several devices: {', '.join(sorted(str(d) for d in devices))}")
 
 
+def _need_split_groups(q: Tensor, parts: tuple[Tensor, ...], hq: int, heads: int) -> None:
+    """On a mesh every device has the query heads of its own heads of the cache. One head of the cache is whole on all of them."""
+    from ..core.sharding.propagation import _assign_factor_axes
+
+    specs = [t._impl.sharding for t in (q, *parts)]
+    mesh = next((s.mesh for s in specs if s is not None), None)
+    if mesh is None or heads == 1:
+        return
+    axes = _assign_factor_axes(_attend.sharding_rule([_shape(t) for t in (q, *parts)], None), specs).get("h", [])
+    n = math.prod(mesh.get_axis_size(a) for a in axes)
+    _need(-(-hq // n) == hq // heads * -(-heads // n), f"{hq} query heads and {heads} heads of the cache, split over {n} devices, would part queries from their keys")
+
+
 def _now(out) -> tuple[Tensor, ...]:
     """What reads or writes a cache is computed at once, so that writes and reads take place in the order of the program; in a function that is
     being compiled, its recording keeps that order."""
@@ -447,6 +461,7 @@ def cached_attention(q: Tensor, cache: dict[str, Tensor], block_table: Tensor, p
     batch, _, hq, _ = _shape(q)
     _need(hq >= heads and hq % heads == 0, f"{hq} query heads cannot share {heads} heads of the cache evenly")
     _places(block_table, past, count, batch, "past", n)
+    _need_split_groups(q, parts, hq, heads)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _need(scale > 0 and math.isfinite(scale), "scale has to be positive")
     more = () if count is None else (count,)
@@ -472,6 +487,7 @@ def shared_prefix_attention(q: Tensor, cache: dict[str, Tensor], prefix_table: T
     _need(_shape(prefix_table)[0] * n < 1 << 30, "a prefix has fewer than 2^30 positions")
     _tensor(prefix_length, "prefix_length", _WHOLE, (1,))
     _places(block_table, past, count, batch, "past", n)
+    _need_split_groups(q, parts, hq, heads)
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     _need(scale > 0 and math.isfinite(scale), "scale has to be positive")
     more = () if count is None else (count,)

@@ -291,6 +291,25 @@ def test_over_a_mesh(mesh_2x4):
     assert (torch.from_numpy(got.to_numpy()) - want).abs().max() <= 2.0 ** -20 * want.abs().max()
 
 
+@pytest.mark.parametrize("hq,h,axis,fine", [(12, 3, "dp", False), (8, 2, "tp", False), (12, 6, "tp", False), (6, 3, "dp", False),
+                                            (8, 4, "tp", True), (6, 3, "tp", True), (5, 5, "tp", True), (8, 1, "tp", True), (12, 6, "dp", True)])
+def test_groups_of_heads_over_a_mesh(hq, h, axis, fine, mesh_2x4):
+    """A split that would give a device query heads without the heads of the cache that they share is refused, with a prefix and without."""
+    q, cache, prefix_table, prefix, table, past, count = make((3, 2, hq, h, 64, 16, 40, [0, 5, 9], None, "fp32", True, "int32"), "cpu")
+    assert count is None
+    for q_axis, c_axis in ((axis, axis), (axis, None), (None, axis)):
+        split = {k: T(v).shard(mesh_2x4, (None, c_axis, None, None)[:v.dim()]) for k, v in cache.items()}
+        sq = T(q).shard(mesh_2x4, (None, None, q_axis, None))
+        for f, rest in ((F.shared_prefix_attention, (prefix_table, prefix, table, past)), (F.cached_attention, (table, past))):
+            if not fine:
+                with pytest.raises(ValueError, match="split over"):
+                    f(sq, split, *(T(x) for x in rest))
+                continue
+            want = f(T(q), {k: T(v) for k, v in cache.items()}, *(T(x) for x in rest)).to_torch()
+            got = torch.from_numpy(f(sq, split, *(T(x) for x in rest)).to_numpy())
+            assert (got - want).abs().max() <= 2.0 ** -20 * want.abs().max()       # as above: the same fp32 sums head by head
+
+
 def test_refusals():
     cache = F.init_kv_cache(8, 2, 64, 16)
     q = T(torch.zeros(3, 1, 4, 64))
