@@ -8,8 +8,8 @@
 // take two to four. A group of lanes keeps its head, and so its gain, for all tokens of its block; what it reads next is on its way into a ring in shared
 // memory, each lane's own, so that no lane waits for another and no registers hold it. The angles of a token are the same for all its heads: the block
 // puts their cosines and sines into shared memory first. An angle is taken in turns, in 64 bits, and only what is left of a whole turn goes into
-// 32 (a position of 10^6 would be off by 0.06 in 32 bits); that remainder is carried in two parts, so cosines and sines are off by about a unit in
-// the last place.
+// 32 (a position of 10^6 would be off by 0.06 in 32 bits); that remainder is carried in two parts, so cosines and sines are off by two units in
+// the last place, those of small angles too.
 //
 // Bound by memory: 8 x 2048 tokens of 16 heads of 128 with their values in bf16 take 73 us forward, 403 MB, 5.5 TB/s, and 103 us backward, 537 MB, 5.2 TB/s (a plain
 // copy 6.5); 4 x 2048 tokens of 16 + 16 heads in fp32 54 and 83, 4.9 TB/s. Before the ring, with 2 or 4 tokens in registers, 90 to 108 and 165 to 378 (spilled). Three
@@ -60,11 +60,12 @@ __device__ __forceinline__ void fill_angles(const RotaryArgs& a, const unsigned 
   const int more_t = blockDim.x / half, more_k = blockDim.x - more_t * half;
   int t = threadIdx.x / half, k = threadIdx.x - t * half;
   for (int i = threadIdx.x; t < n; i += blockDim.x) {
-    // the upper half of the fraction, from -2^31 to 2^31, is a number of half turns; what a float does not hold of it goes into the second part
-    const int rest = static_cast<int>((static_cast<unsigned long long>(at[t]) * turns[k]) >> 32);
-    const float hi = static_cast<float>(rest), lo = static_cast<float>(static_cast<int>(rest - static_cast<long long>(hi))) * (3.14159265f / 2147483648.f);
+    // the fraction, from -2^63 to 2^63, in half turns: all of it, for the angle of a slow pair is in its lower bits. What a float does not hold goes into the second
+    // part (2^63 itself, which the float may be, comes back as the number below it)
+    const long long rest = static_cast<long long>(static_cast<unsigned long long>(at[t]) * turns[k]);
+    const float hi = __ll2float_rn(rest), lo = __ll2float_rn(rest - __float2ll_rn(hi)) * (3.14159265f / 9223372036854775808.f);
     float s, c;
-    sincospif(hi * (1.f / 2147483648.f), &s, &c);
+    sincospif(hi * (1.f / 9223372036854775808.f), &s, &c);
     angles[i] = fmaf(-lo, s, c), angles[ANGLES + i] = fmaf(lo, c, s);
     t += more_t, k += more_k;
     if (k >= half) k -= half, ++t;

@@ -6,6 +6,7 @@ products and a sum: below 2^5 units of 2^-24, so 2^-18 of the pair's length cove
 """
 from __future__ import annotations
 
+import decimal
 import math
 
 import pytest
@@ -15,6 +16,7 @@ import nabla_b200 as nb
 from nabla_b200.nn import functional as F
 from nabla_b200.ops import heads
 
+D = decimal.Decimal
 DEVICES = ["cpu", "primitive", pytest.param("cuda", marks=pytest.mark.gpu)]
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
 EPS = 1e-6
@@ -185,6 +187,40 @@ def test_gradients_against_differences(interleaved, on):
     # third derivatives of the norm times h^2 / 6 (of order one for entries of about one), and the rounding of two values over 2 h
     values = math.sqrt(cq.numel() + ck.numel()) * 1.5 * 2.0 ** -23 / (2 * h)
     assert abs(slope - want) <= 20 * h * h * size + values
+
+
+def exact_turn(position, base, rotary):
+    """Cosines and sines of a position's angles, which are reduced in 120 digits."""
+    with decimal.localcontext() as c:
+        c.prec = 120
+        # pi by Machin's formula: 16 atan(1/5) - 4 atan(1/239)
+        atan = lambda n: sum((-1) ** i * D(1) / (D(n) ** (2 * i + 1) * (2 * i + 1)) for i in range(180))  # noqa: E731
+        whole = 2 * (16 * atan(5) - 4 * atan(239))
+        rest = [(D(position) * (D(base).ln() * (-2 * i) / rotary).exp()) % whole for i in range(rotary // 2)]
+        return torch.tensor([[math.cos(x), math.sin(x)] for x in rest], dtype=torch.float64)
+
+
+def ones_turned(on, positions, base, d=64):
+    """(cos, sin) of ``positions`` by pairs (0, 1) that are turned, and by their gradients, which are turned back: two tensors (tokens, d / 2, 2)."""
+    x = torch.zeros((1, len(positions), 1, d), device=on)
+    x[..., d // 2:] = 1.0
+    pos = T(torch.tensor(positions, dtype=torch.int64, device=on))
+    y, pull = nb.vjp(lambda q, k: F.norm_rotary(q, k, pos, base=base), T(x), T(x.clone()), create_graph=False)
+    (dq, _), y = pull((T(x), T(x.clone()))), y[0].to_torch()
+    y, dq = (z.double().cpu()[0, :, 0].view(-1, 2, d // 2) for z in (y, dq.to_torch()))
+    return torch.stack([y[:, 1], -y[:, 0]], -1), torch.stack([dq[:, 1], dq[:, 0]], -1)
+
+
+@pytest.mark.parametrize("on", DEVICES, indirect=True)
+@pytest.mark.parametrize("base", [1e4, 5e5, 1e6])
+def test_slow_pairs_keep_their_bits(base, on):
+    """The sine of a small angle is as good, beside itself, as others beside 1: two units of 2^-24 for the sine, one for its correction by what a float
+    does not hold of the angle, one to spare; and what an angle in 64 bits is off by, 2^-50 for each position."""
+    positions = [1, 2, 999, -7]
+    want = torch.stack([exact_turn(p, base, 64) for p in positions])
+    for got in ones_turned(on, positions, base):
+        tol = 2.0 ** -22 * want.abs() + 2.0 ** -50 * torch.tensor(positions).abs()[:, None, None]
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / want.abs()).max().item()
 
 
 @pytest.mark.gpu
