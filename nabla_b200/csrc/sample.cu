@@ -53,23 +53,24 @@ __device__ __forceinline__ u64 order_of(float z, int v) { return z > -INFINITY ?
 __device__ __forceinline__ int token_of(u64 order) { return static_cast<int>(0xffffffffu - static_cast<uint32_t>(order)); }
 
 struct Weigher {
-  float top, per_octave;         // the largest logit; octaves of w for a unit of logit
+  float top, half_top, per_half; // the largest logit, half of it (two logits may be further apart than the largest number); octaves of w for half a unit of logit
   double top64, rate;            // 32 octaves
   const double* roots;           // 2^(-i / 32), in shared memory
   bool alone;                    // the largest logit, or what a unit of logit is worth, is infinite: only tokens with that logit have a weight
 
-  __device__ __forceinline__ Weigher(float largest, float temperature, const double* table) : top(largest), top64(largest), roots(table) {
+  __device__ __forceinline__ Weigher(float largest, float temperature, const double* table) : top(largest), half_top(0.5f * largest), top64(largest), roots(table) {
     rate = 46.166241308446828 / static_cast<double>(temperature);                        // 32 log2(e)
-    per_octave = static_cast<float>(rate / 32.0);
-    alone = top == INFINITY || per_octave == INFINITY;
+    per_half = static_cast<float>(rate / 16.0);
+    alone = top == INFINITY || per_half == INFINITY;
   }
+  __device__ __forceinline__ float octaves(float z) const { return fmaf(z, -0.5f, half_top) * per_half; }
   // The step of the histogram that a logit falls into, BINS: behind its end, or nowhere. Monotone.
   __device__ __forceinline__ int bin(float z) const {
     if (alone) return z == top ? 0 : BINS;
-    const float x = (top - z) * per_octave;
+    const float x = octaves(z);
     return x < FAR ? __float_as_int(fmaf(x, (BINS - 1) / FAR, 8388608.f)) & 0xfff : BINS;        // + 2^23: the nearest whole number is in the low bits
   }
-  __device__ __forceinline__ float about(float z) const { return alone ? (z == top ? 1.f : 0.f) : exp2f((z - top) * per_octave); }
+  __device__ __forceinline__ float about(float z) const { return alone ? (z == top ? 1.f : 0.f) : exp2f(-octaves(z)); }
   // w in multiples of 2^-43. With t in 32nds of octaves and n the whole number next to it: exp(-(t - n) ln 2 / 32) by its series (the term behind the last is
   // below 2^-48), times a root of 2, put where its last bit is 2^-43 by adding 2^52. A logit of -inf and NaN have none.
   __device__ __forceinline__ u64 fixed(float z) const {

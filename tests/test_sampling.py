@@ -153,6 +153,25 @@ def test_numbers_at_the_ends(device):
     assert draw(z, some, top_k=k) == oracle(z, some, top_k=k)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("v", [300, 1300, 9001])
+def test_logits_further_apart_than_the_largest_number(v, dtype, device):
+    """Differences of logits past fp32's largest number, and temperatures that bring them back to a few units."""
+    g = torch.Generator().manual_seed(v)
+    z = ((torch.rand((6, v), generator=g) * 2 - 1) * 3.3e38).to(dtype)
+    z[3, ::2] = -math.inf
+    z[4] = torch.where(torch.rand(v, generator=g) < 0.5, 3e38, -3e38).to(dtype)
+    t = torch.tensor([1e38, 3e38, math.inf, 2e38, 3e38, 5e37])
+    u = torch.tensor([0.5, 0.03, 0.98, 0.7, 0.999, 0.6])
+    k = torch.tensor([v - 40, v // 2, 7, v // 3, 0, 0])
+    p = torch.tensor([0.9, 0.97, 0.999, 0.51, 0.95, 0.6])
+    m = torch.tensor([0.01, 0.2, 0.5, 0.3, 0.1, 1e-4])
+    z, t, u, k, p, m = (x.to(device) for x in (z, t, u, k, p, m))
+    for kw in ({}, {"top_k": k}, {"top_p": p}, {"min_p": m}, {"top_k": k, "top_p": p, "min_p": m}):
+        assert draw(z, u, temperature=t, **kw) == oracle(z, u, temperature=t, **kw, clear=v < 9001)       # (which is slow for long rows)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("v,dtype,std", [(131072, torch.float32, 3.0), (32001, torch.bfloat16, 3.0), (1 << 20, torch.bfloat16, 1.0), (100003, torch.float32, 0.01),
                                          (65537, torch.bfloat16, 0.0)])
