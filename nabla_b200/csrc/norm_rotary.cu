@@ -7,9 +7,10 @@
 // A head is held by D / 16 lanes (rounded up to a power of two), 16 numbers each: both halves of eight pairs, so a rotation needs no exchange and the means
 // take two to four. A group of lanes keeps its head, and so its gain, for all tokens of its block; what it reads next is on its way into a ring in shared
 // memory, each lane's own, so that no lane waits for another and no registers hold it. The angles of a token are the same for all its heads: the block
-// puts their cosines and sines into shared memory first. An angle is taken in turns, in 64 bits, and only what is left of a whole turn goes into
-// 32 (a position of 10^6 would be off by 0.06 in 32 bits); that remainder is carried in two parts, so cosines and sines are off by two units in
-// the last place, those of small angles too.
+// puts their cosines and sines into shared memory first. An angle is a fraction of a turn in whole numbers of 2^-64, which the caller has rounded from more bits
+// (an exponential in 64 bits is off by 2^-54 and more, a position of 2^33 by 10^-6 then), and only what is left of a whole turn becomes a number of 32 bits
+// (a position of 10^6 would be off by 0.06 in 32 bits); that remainder is carried in two parts, so cosines and sines are off by two units in the last place, those
+// of small angles too, and by 2^-62 for each position.
 //
 // Bound by memory: 8 x 2048 tokens of 16 heads of 128 with their values in bf16 take 73 us forward, 403 MB, 5.5 TB/s, and 103 us backward, 537 MB, 5.2 TB/s (a plain
 // copy 6.5); 4 x 2048 tokens of 16 + 16 heads in fp32 54 and 83, 4.9 TB/s. Before the ring, with 2 or 4 tokens in registers, 90 to 108 and 165 to 378 (spilled). Three
@@ -37,19 +38,13 @@ struct RotaryArgs {
   int heads, abreast, chunk, chunks;       // of a block: heads, tokens at once; tokens of a chunk, chunks of a sequence
   Whole positions;
   int positions_shared;          // one row of positions for the whole batch
-  double log2_base;
   float eps;
   float* sums;                   // backward: [blocks][2][dim] parts of the gradients of the gains
+  unsigned long long turns[MOST_DIM / 2];        // of pairs, for a position, in 2^-64 of a turn: products with positions are taken modulo whole turns by themselves
 };
 
-// Turns per position, in units of 2^-64 of a turn: their products with positions are taken modulo whole turns by themselves.
 __device__ __forceinline__ void fill_turns(const RotaryArgs& a, unsigned long long* turns) {
-  const double rate = -2.0 * a.log2_base / a.rotary;
-  for (int i = threadIdx.x; i < a.rotary / 2; i += blockDim.x) {
-    double turn = exp2(rate * i) * 0.15915494309189535;                // 1 / (2 pi)
-    turn -= floor(turn);
-    turns[i] = static_cast<unsigned long long>(turn * 18446744073709551616.0);
-  }
+  for (int i = threadIdx.x; i < a.rotary / 2; i += blockDim.x) turns[i] = a.turns[i];
 }
 // cosines and, ANGLES behind them, sines of n tokens from the first, [token][rotary / 2]. All threads.
 __device__ __forceinline__ void fill_angles(const RotaryArgs& a, const unsigned long long* turns, float* angles, long long* at, int first, int n) {
@@ -380,13 +375,13 @@ extern "C" long long nb_norm_rotary_scratch(int batch, int tokens, int all_heads
   return 2ll * dim * c.blocks * c.across;
 }
 
-// Parts q, k and, where v_heads > 0, v, which is copied. strides: in elements, [x, dy][q, k, v][batch, token, head]. Results are dense (batch, tokens, heads,
+// Parts q, k and, where v_heads > 0, v, which is copied. turns: see RotaryArgs. strides: in elements, [x, dy][q, k, v][batch, token, head]. Results are dense (batch, tokens, heads,
 // dim) each or, `packed`, one (batch, tokens, heads, {q, k, v}, dim). Backward where dy of q is given: results are gradients then. -1: sizes that the
 // kernels do not take.
 extern "C" int nb_norm_rotary(const void* q, const void* k, const void* v, const void* q_dy, const void* k_dy, const void* v_dy, void* q_out, void* k_out,
                               void* v_out, const void* q_gain, const void* k_gain, void* q_gain_grad, void* k_gain_grad, const void* positions, int wide,
                               int positions_shared, int batch, int tokens, int q_heads, int k_heads, int v_heads, int dim, int rotary, int neighbours,
-                              double log2_base, float eps, const long long* strides, int packed, float* scratch, int fp32, void* stream) {
+                              const unsigned long long* turns, float eps, const long long* strides, int packed, float* scratch, int fp32, void* stream) {
   using namespace nbc;
   const long long n = (long long)batch * tokens;
   if (n < 1 || n >= 1ll << 30 || dim < 16 || dim > MOST_DIM || dim % 16 || rotary < 16 || rotary > dim || rotary % 16) return -1;
@@ -405,7 +400,8 @@ extern "C" int nb_norm_rotary(const void* q, const void* k, const void* v, const
     for (int i = 0; i < 3; ++i) h.x_s[i] = strides[3 * p + i], h.dy_s[i] = strides[9 + 3 * p + i];
   }
   a.batch = batch, a.tokens = tokens, a.dim = dim, a.rotary = rotary, a.all_heads = q_heads + k_heads + v_heads;
-  a.positions = Whole{positions, wide}, a.positions_shared = positions_shared, a.log2_base = log2_base, a.eps = eps;
+  a.positions = Whole{positions, wide}, a.positions_shared = positions_shared, a.eps = eps;
+  for (int i = 0; i < rotary / 2; ++i) a.turns[i] = turns[i];
   const bool back = q_dy != nullptr, sums = back && (q_gain_grad != nullptr || k_gain_grad != nullptr);
   if (sums && scratch == nullptr) return -1;
   a.sums = sums ? scratch : nullptr;

@@ -7,7 +7,6 @@ from __future__ import annotations
 
 import ctypes
 import functools
-import math
 
 import torch
 
@@ -16,7 +15,7 @@ from .serving import _rows
 
 _lib = None
 launch_count = 0
-c_int, c_ll, c_f, c_d, c_vp = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_double, ctypes.c_void_p
+c_int, c_ll, c_f, c_vp = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
 _Strides = c_ll * 18
 
 
@@ -24,7 +23,7 @@ def _L():
     global _lib
     if _lib is None:
         lib = load("libnb_heads.so")
-        lib.nb_norm_rotary.argtypes = [c_vp] * 14 + [c_int] * 10 + [c_d, c_f, c_vp, c_int, c_vp, c_int, c_vp]
+        lib.nb_norm_rotary.argtypes = [c_vp] * 14 + [c_int] * 10 + [c_vp, c_f, c_vp, c_int, c_vp, c_int, c_vp]
         lib.nb_norm_rotary.restype = c_int
         lib.nb_norm_rotary_scratch.argtypes = [c_int] * 6
         lib.nb_norm_rotary_scratch.restype = c_ll
@@ -37,6 +36,13 @@ def _L():
 def _scratch(*sizes: int) -> int:
     """A function of the sizes alone."""
     return _L().nb_norm_rotary_scratch(*sizes)
+
+
+@functools.lru_cache(256)
+def _turns(base: float, rotary_dim: int):
+    from ..ops.heads import turns
+
+    return (ctypes.c_ulonglong * (rotary_dim // 2))(*turns(base, rotary_dim))
 
 
 def norm_rotary(parts, dys, positions, gains, *, eps: float, base: float, rotary_dim: int, interleaved: bool, packed: bool):
@@ -69,7 +75,7 @@ def norm_rotary(parts, dys, positions, gains, *, eps: float, base: float, rotary
     dy = [ptr(y) for y in dys] + [c_vp(0)] * (3 - len(dys)) if dys is not None else [c_vp(0)] * 3
     rc = _L().nb_norm_rotary(ptr(parts[0]), ptr(parts[1]), ptr(v), *dy, *outs, ptr(gains[0]), ptr(gains[1]), ptr(grads[0]), ptr(grads[1]),
                              ptr(positions), int(positions.dtype == torch.int64), int(positions.dim() == 1), b, t, hq, parts[1].shape[2],
-                             0 if v is None else v.shape[2], d, rotary_dim, int(interleaved), math.log2(base), float(eps), strides, int(packed),
+                             0 if v is None else v.shape[2], d, rotary_dim, int(interleaved), _turns(base, rotary_dim), float(eps), strides, int(packed),
                              ptr(scratch), int(x.dtype == torch.float32), stream_ptr())
     if rc != 0:
         raise RuntimeError(f"norm_rotary failed with code {rc}")

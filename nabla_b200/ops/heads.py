@@ -2,7 +2,8 @@
 
 For the D numbers x of a head at position t:  n = x / sqrt(mean x^2 + eps),  z = n * gain,  y = R(t) z; without a gain z = x. R(t) turns the pairs
 (z_i, z_(i + rotary_dim / 2)), or with ``interleaved`` the neighbours (z_2i, z_(2i + 1)), of the first ``rotary_dim`` numbers by the angle
-t * base^(-2 i / rotary_dim), and leaves the others. Sums and angles are taken in fp32 (angles reduced from 64 bits), results rounded once.
+t * base^(-2 i / rotary_dim), and leaves the others. Sums are taken in fp32, results rounded once. Angles are fractions of a turn in whole numbers of 64
+bits, whose products with a position wrap at whole turns: they are off by 2^-62 for each position, so cosines and sines hold fp32's bits up to some 2^38.
 
 ``norm_rotary`` takes queries and keys as two tensors (views of a projection, fewer heads of keys than of queries), ``packed_norm_rotary``
 the packed projection that ``packed_self_attention`` reads. Both have the hand-written kernels of ``csrc/norm_rotary.cu`` on CUDA, with a backward
@@ -10,8 +11,11 @@ pass of their own, and an equivalent torch expression elsewhere; derivatives bey
 """
 from __future__ import annotations
 
+import decimal
+import functools
 import math
 
+import numpy as np
 import torch
 
 from ..core.sharding.propagation import OpShardingRule
@@ -30,11 +34,43 @@ def _runs_native(x: torch.Tensor) -> bool:
     return x.device.type != "meta" and native.use_native(x) and x.numel() > 0
 
 
+# ---------------------------------------------------------------- angles
+@functools.lru_cache(256)
+def turns(base: float, rotary_dim: int) -> tuple[int, ...]:
+    """What each pair turns by for a position, the fraction of a turn, base^(-2 i / rotary_dim) / (2 pi) less its whole part, in whole numbers of 2^-64, rounded:
+    0 <= n < 2^64. (An exponential in 64 bits is off by 2^-54 of a turn and more.)"""
+    with decimal.localcontext() as c:
+        c.prec = digits = 50 + max(0, -math.floor(math.log10(base)))             # in front of the point too, where base is below 1
+
+        def atan_of_one_over(n: int) -> int:                                       # its series, in units of 10^-(digits + 10)
+            term, total, k = 10 ** (digits + 10) // n, 0, 1
+            while term:
+                total += term // k if k % 4 == 1 else -(term // k)
+                term //= n * n
+                k += 2
+            return total
+
+        two_pi = decimal.Decimal(2 * (16 * atan_of_one_over(5) - 4 * atan_of_one_over(239))).scaleb(-(digits + 10))         # Machin
+        log = decimal.Decimal(base).ln()
+        return tuple(int((((log * (-2 * i) / rotary_dim).exp() / two_pi) % 1 * 2 ** 64).to_integral_value()) % 2 ** 64 for i in range(rotary_dim // 2))
+
+
+def _signed_turns(base: float, rotary_dim: int) -> list[int]:
+    return [n - 2 ** 64 if n >> 63 else n for n in turns(base, rotary_dim)]
+
+
+_RADIANS = 2.0 * math.pi / 2.0 ** 64
+
+
+@functools.lru_cache(64)
+def _turns_on(base: float, rotary_dim: int, device: torch.device) -> torch.Tensor:
+    return torch.tensor(_signed_turns(base, rotary_dim), dtype=torch.int64, device=device)
+
+
 # ---------------------------------------------------------------- torch expressions
 def _angles(positions, base: float, rotary_dim: int):
     """cos, sin (..., tokens, 1, rotary_dim / 2) in fp32."""
-    rate = torch.exp(torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=positions.device) * (-math.log(base) / rotary_dim))
-    angle = positions.double()[..., None, None] * rate
+    angle = (positions.long()[..., None, None] * _turns_on(base, rotary_dim, positions.device)).double() * _RADIANS       # (the product wraps)
     return angle.cos().float(), angle.sin().float()
 
 
@@ -283,9 +319,9 @@ def _angles_reference(positions: Tensor, base: float, rotary_dim: int):
     from .unary import cast, cos, sin
     from .view import unsqueeze
 
-    rate = torch.exp(torch.arange(0, rotary_dim, 2, dtype=torch.float64) * (-math.log(base) / rotary_dim))
-    rate = constant(rate.numpy(), dtype=DType.float64, device=positions.device)
-    angle = unsqueeze(unsqueeze(cast(positions, DType.float64), axis=-1), axis=-1) * rate
+    per = constant(np.array(_signed_turns(base, rotary_dim), dtype=np.int64), dtype=DType.int64, device=positions.device)
+    radians = constant(np.array(_RADIANS), dtype=DType.float64, device=positions.device)
+    angle = cast(unsqueeze(unsqueeze(cast(positions, DType.int64), axis=-1), axis=-1) * per, DType.float64) * radians
     return cast(cos(angle), DType.float32), cast(sin(angle), DType.float32)
 
 
@@ -358,7 +394,7 @@ def norm_rotary(q: Tensor, k: Tensor, positions: Tensor, q_gain: Tensor | None =
     """Queries (batch, tokens, heads, head_dim) and keys (batch, tokens, kv_heads, head_dim), bf16 or fp32, views included, as attention is to see
     them: each head normed by its root mean square and multiplied by its gain (head_dim,), where one is given, then turned by its position.
 
-    ``positions`` (tokens,) or (batch, tokens): whole numbers of any size. ``rotary_dim`` (head_dim by default): how many numbers of a head are turned;
+    ``positions`` (tokens,) or (batch, tokens): whole numbers; an angle is off by 2^-62 for each, which fp32 begins to see at 2^38. ``rotary_dim`` (head_dim by default): how many numbers of a head are turned;
     ``interleaved``: neighbours are pairs, not halves. Gradients of queries, keys and gains."""
     from ..nn.functional.layers import use_fused
 

@@ -223,6 +223,26 @@ def test_slow_pairs_keep_their_bits(base, on):
         assert ((got - want).abs() <= tol).all(), ((got - want).abs() / want.abs()).max().item()
 
 
+@pytest.mark.parametrize("on", DEVICES, indirect=True)
+@pytest.mark.parametrize("base", [1e4, 1e6])
+def test_far_positions(base, on):
+    """As above; a fraction in whole numbers of 2^-64 of a turn is off by half of that at most, 2 pi 2^-65 < 2^-62 for each position."""
+    positions = [(1 << 28) + 1, (1 << 33) + 7, (1 << 38) - 5, -(1 << 36) + 11, (1 << 40) + 3, -(1 << 44)]
+    want = torch.stack([exact_turn(p, base, 64) for p in positions])
+    for got in ones_turned(on, positions, base):
+        tol = 2.0 ** -22 * want.abs() + 2.0 ** -62 * torch.tensor(positions).double().abs()[:, None, None] + 2.0 ** -50
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max().item()
+
+
+@pytest.mark.parametrize("base", [1e4, 0.5, 1e-30, 3e38, 1.0])
+def test_fractions_of_turns(base):
+    """Against the angles of a position in 120 digits: half a unit of 2^-64 of a turn, and what a double holds of their sines."""
+    n = torch.tensor([x / 2.0 ** 64 for x in heads.turns(base, 32)], dtype=torch.float64) * (2 * math.pi)
+    assert len(n) == 16 and all(0 <= x < 1 << 64 for x in heads.turns(base, 32))
+    want = exact_turn(1, base, 32)
+    assert (n.cos() - want[:, 0]).abs().max() <= 2.0 ** -50 and (n.sin() - want[:, 1]).abs().max() <= 2.0 ** -50
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("off", [1, 4, 8])
 def test_views_off_boundaries_and_strides(off, monkeypatch):
