@@ -86,9 +86,6 @@ def move(cache: dict[str, Tensor], table: Tensor, count: Tensor, max_tokens: int
     return F.kv_cache_write(other, k, v, other_table, zero, count)
 
 
-_FILTERS = ("temperature", "top_k", "top_p", "min_p")
-
-
 @functools.lru_cache(8)
 def _steps(layers: int, dim: int, heads: int, hidden: int, vocab: int, max_seq: int, rotary_base: float | None = None, qk_norm: bool = False):
     """Compiled once per model: the call for prompts and steps, and the choice of the next tokens, the likeliest or drawn."""
@@ -157,8 +154,9 @@ def generate(params: dict[str, Any], prompts: list[list[int]], cfg: TransformerC
     history, prompt_length, length = history.to(dev), put(lengths + P), lengths.to(dev)
     one, rows = put(torch.ones(B, dtype=torch.int32)), torch.arange(B, device=dev)
     uniform = torch.rand((max_new, B), generator=torch.Generator().manual_seed(seed)).to(dev) if temperature > 0 else None
-    given = {"temperature": float(temperature), "top_k": int(top_k), "top_p": float(top_p), "min_p": float(min_p)}
-    filters = {k: put(torch.full((B,), given[k], dtype=torch.int32 if k == "top_k" else torch.float32)) for k in _FILTERS}
+    # filters that let all through are left out: a draw without top-k and top-p has a kernel of its own
+    given = {"temperature": (float(temperature), True), "top_k": (int(top_k), top_k > 0), "top_p": (float(top_p), top_p < 1), "min_p": (float(min_p), min_p > 0)}
+    filters = {k: put(torch.full((B,), x, dtype=torch.int32 if k == "top_k" else torch.float32)) for k, (x, used) in given.items() if used}
     for step in range(max_new):
         args = (Tensor.from_torch(last), Tensor.from_torch(history), Tensor.from_torch(length + P), prompt_length, *numbers, *(() if allowed is None else (allowed,)))
         if uniform is None:

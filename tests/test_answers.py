@@ -158,3 +158,21 @@ def test_drawn_answers(device):
     words[2, 3] = 0b1000
     b = G.generate(params, prompts, cfg, 12, block_size=16, allowed=T(words.to(device)), **hot)
     assert set(b[0]) <= {97, 99} and b[1] == [0] * 12 and b[2] == [99] * 12
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_a_draw_gets_the_filters_in_effect(device, monkeypatch):
+    """Those that let all through are not handed on; a share of 0 leaves the likeliest, as no other filter does."""
+    cfg, params = small(device, nb.DType.float32, max_seq=97)            # (compiled for itself: the calls are seen while they are)
+    seen, sample = [], G.F.sample_tokens
+    monkeypatch.setattr(G.F, "sample_tokens", lambda logits, uniform, **kw: (seen.append(set(kw)), sample(logits, uniform, **kw))[1])
+    prompts = [[5, 7, 9], [1]]
+    for kw, want in (({}, set()), ({"top_k": 0, "top_p": 1.0, "min_p": 0.0}, set()), ({"top_k": 5}, {"top_k"}), ({"top_p": 0.5}, {"top_p"}),
+                     ({"min_p": 0.1}, {"min_p"}), ({"top_k": 9, "top_p": 0.0, "min_p": 0.2}, {"top_k", "top_p", "min_p"}), ({"top_k": -3, "min_p": -1.0}, set())):
+        seen.clear()
+        G._steps.cache_clear()
+        answers = G.generate(params, prompts, cfg, 5, block_size=16, temperature=0.7, seed=2, **kw)
+        assert seen and all(names == want | {"temperature"} for names in seen)
+        if kw.get("top_p") == 0.0:
+            assert answers == G.generate(params, prompts, cfg, 5, block_size=16)
+    G._steps.cache_clear()
