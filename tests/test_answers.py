@@ -176,3 +176,55 @@ def test_a_draw_gets_the_filters_in_effect(device, monkeypatch):
         if kw.get("top_p") == 0.0:
             assert answers == G.generate(params, prompts, cfg, 5, block_size=16)
     G._steps.cache_clear()
+
+
+def misfits(cfg, params, device, texts, answers, uniform, temperature, top_k=0, top_p=1.0, min_p=0.0):
+    """How many tokens of ``answers`` the logits of ``texts`` with these answers do not bear out.
+
+    Logits of the cache are off by 2 % of their rms (``test_decoding_behind_a_prefix``), four times that is allowed: ``off``. Where nothing is filtered the random number
+    has to lie in the token's share of the sum, which an error e of logits moves by no more than the mean of |e| / T. A filter's border and the token's own logit are
+    each off by ``off``; for top-p, the share in front of the token as above. Shares in the order of ids say little of a text: where nothing is filtered, the logarithms of the
+    drawn tokens' shares also have to add up to what draws give, to four standard deviations, or none of them fits."""
+    bad, less, variance, allowed = 0, 0.0, 0.0, 0.0
+    for i, (text, answer) in enumerate(zip(texts, answers)):
+        z = M.forward(params, T(torch.tensor([text + answer]).to(device)), cfg).to_torch()[0, len(text) - 1:-1].double().cpu()
+        off = 4 * 0.02 * z.pow(2).mean().sqrt().item()
+        for step, token in enumerate(answer):
+            w = torch.softmax(z[step] / temperature, 0)
+            own = z[step, token]
+            if not top_k and top_p >= 1 and not min_p:
+                upto = w.cumsum(0)[token]
+                bad += not upto - w[token] - off / temperature <= uniform[step, i] <= upto + off / temperature
+                log = torch.log_softmax(z[step] / temperature, 0)
+                mean = (w * log).sum()
+                less, variance, allowed = less + mean - log[token], variance + (w * (log - mean) ** 2).sum(), allowed + off / temperature
+                continue
+            fits = not top_k or own >= z[step].topk(top_k).values[-1] - 2 * off
+            fits &= top_p >= 1 or w[z[step] > own + 2 * off].sum() < top_p + off / temperature
+            fits &= not min_p or (own - z[step].max()) / temperature >= np.log(min_p) - 2 * off / temperature
+            bad += not fits
+    return bad if less <= 4 * variance ** 0.5 + allowed else uniform.numel()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("rotary", [None, 10000.0])
+def test_draws_fit_the_logits_of_their_own_texts(rotary, device):
+    """Steep distributions (logits of some 3 T): drawn tokens fit the texts that they stand behind, and not those behind another prefix, nor does a draw
+    that does not look at the logits."""
+    cfg, params = small(device, nb.DType.float32, rotary is not None, rotary_base=rotary)
+    params["lm_head"] = T(params["lm_head"].to_torch() * 8.0)
+    for p in params["layers"]:                        # what attention adds outweighs the tokens themselves
+        p["wo"] = T(p["wo"].to_torch() * 16.0)
+    g = torch.Generator().manual_seed(14)
+    prefix, other = (torch.randint(0, cfg.vocab, (41,), generator=g).tolist() for _ in range(2))
+    prompts = [torch.randint(0, cfg.vocab, (n,), generator=g).tolist() for n in (5, 1, 33)]
+    texts, seed, n = [prefix + p for p in prompts], 6, 12
+    uniform = torch.rand((n, 3), generator=torch.Generator().manual_seed(seed))
+    for kw in ({}, {"top_k": 3}, {"top_p": 0.3}, {"min_p": 0.3}, {"top_k": 20, "top_p": 0.5, "min_p": 0.1}):
+        kw = {"temperature": 0.8, **kw}
+        fit = lambda answers: misfits(cfg, params, device, texts, answers, uniform, **kw)  # noqa: E731
+        assert fit(G.generate(params, prompts, cfg, n, block_size=16, prefix=prefix, seed=seed, **kw)) == 0
+        assert fit(G.generate(params, texts, cfg, n, block_size=16, seed=seed, **kw)) == 0
+        assert fit(G.generate(params, prompts, cfg, n, block_size=16, prefix=other, seed=seed, **kw)) >= 3
+        assert fit(G.generate(params, prompts, cfg, n, block_size=16, seed=seed, **kw)) >= 3
+        assert fit([[int(u * cfg.vocab) for u in uniform[:, i]] for i in range(3)]) >= 3
