@@ -151,7 +151,7 @@ struct SampleShared {
   u64 exchange[2][MOST_BLOCKS][3];         // what the blocks tell each other, in turn
   u64 joined[3][SAMPLE_WARPS];
   u64 edges[2];
-  int found, before, entries, total, turn;
+  int found, before, entries, total;
 };
 
 __device__ __forceinline__ u64 over_warp_max(u64 x) {
@@ -387,8 +387,8 @@ __device__ __noinline__ u64 last_kept(Team<CLUSTER>& team, const LogitRow<T>& ro
       const u64 n = s.bins[i], middle = at.high - (static_cast<u64>(i) << shift) - (shift ? 1ull << (shift - 1) : 0);
       return n ? static_cast<float>(n) * weigh.about(number_of(static_cast<uint32_t>(middle >> 32))) : 0.f;
     });
-    const int first = max(s.found, 0), last = first;          // (the estimate is seldom off by a bin: what it names is checked)
-    Stretch x = cut(first, last);
+    const int named = max(s.found, 0);                        // (the estimate is seldom off by a bin: what it names is checked)
+    Stretch x = cut(named, named);
     u64 above = 0, within = 0, none = 0;
     row.each([&](int v, float z) {
       const u64 q = order_of(z, v);
@@ -399,13 +399,13 @@ __device__ __noinline__ u64 last_kept(Team<CLUSTER>& team, const LogitRow<T>& ro
     team.sums_of(above, within, none);
     above += at.sum;
     if (static_cast<double>(above) >= want) {                // it lies in front
-      x = cut(0, first - 1);
-      x.sum = at.sum, x.n = tokens_before(s, first);
+      x = cut(0, named - 1);
+      x.sum = at.sum, x.n = tokens_before(s, named);
     } else if (static_cast<double>(above + within) < want) {
-      x = cut(last + 1, BINS - 1);
-      x.sum = above + within, x.n = at.n - tokens_before(s, last + 1);
+      x = cut(named + 1, BINS - 1);
+      x.sum = above + within, x.n = at.n - tokens_before(s, named + 1);
     } else {
-      x.sum = above, x.n = tokens_before(s, last + 1) - tokens_before(s, first);
+      x.sum = above, x.n = static_cast<int>(s.bins[named]);
     }
     at = x;
   }
@@ -528,10 +528,10 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, FILTERED ? 2 : 3) sample_kerne
     const bool cut = by_count && total > asked;
     if (before + static_cast<int>(s.bins[c]) <= LIST)
       return finish(team.list(row, weigh, false, [&](int v, float z) { return weigh.bin(z) <= c; }), cut ? asked : 0);
-    const auto stretch = [&](int first, int last_bin) {      // of bins [first, last_bin]: bins fall as keys grow
+    const auto stretch = [&](int first_bin, int last_bin) {  // of bins [first_bin, last_bin]: bins fall as keys grow
       __syncthreads();
       if (warp < 2) {
-        const int b = warp ? last_bin + 1 : first;
+        const int b = warp ? last_bin + 1 : first_bin;
         const u64 at = least_key(key_of(-INFINITY), key_of(top) + 1, [&](float z) { return weigh.bin(z) < b; });
         if (lane == 0) s.edges[warp] = at;
       }
@@ -550,8 +550,8 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, FILTERED ? 2 : 3) sample_kerne
     }
     if (by_share) {
       find_bin<float, true>(s, p, [&](int i) { return i > end ? 0.f : static_cast<float>(i == end ? end_tokens : static_cast<int>(s.bins[i])) * about(i); });
-      const int first = max(s.found, 0), last_bin = first;     // (the estimate is seldom off by a bin: what it names is checked)
-      Stretch x = stretch(first, last_bin);
+      const int named = max(s.found, 0);                       // (the estimate is seldom off by a bin: what it names is checked)
+      Stretch x = stretch(named, named);
       least_order = least_border();
       // the border of top-k as a number and an id, and the stretch as numbers (above the largest: no number, nothing is at least that)
       const float z_last = last ? number_of(static_cast<uint32_t>(last >> 32)) : -INFINITY, z_low = number_of(static_cast<uint32_t>(x.low >> 32)),
@@ -572,13 +572,13 @@ __global__ void __launch_bounds__(SAMPLE_THREADS, FILTERED ? 2 : 3) sample_kerne
       const double want = fmax(static_cast<double>(p) * static_cast<double>(all), 0.5);     // (the first is kept)
       bool here = false;
       if (static_cast<double>(above) >= want) {
-        x = stretch(0, first - 1);
-        x.sum = 0, x.n = tokens_before(s, first);
+        x = stretch(0, named - 1);
+        x.sum = 0, x.n = tokens_before(s, named);
       } else if (static_cast<double>(above + within) < want) {
-        x = stretch(last_bin + 1, BINS - 1);
-        x.sum = above + within, x.n = total - tokens_before(s, last_bin + 1);
+        x = stretch(named + 1, BINS - 1);
+        x.sum = above + within, x.n = total - tokens_before(s, named + 1);
       } else {
-        x.sum = above, x.n = tokens_before(s, last_bin + 1) - tokens_before(s, first);
+        x.sum = above, x.n = static_cast<int>(s.bins[named]);
         here = true;
       }
       x.low = max(x.low, last);
