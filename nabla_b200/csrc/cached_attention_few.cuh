@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(32 * FEW_WARPS, RT == 1 ? 3 : 2) attend_few_ke
   constexpr bool EXACT = sizeof(T) == 4;              // fp32: two parts, codes less their offset before the product
   constexpr int PARTS = EXACT ? 2 : 1, KSTEPS = D / 16, PIECES = D / 64, MT = D / 16, ROWS = 8 * RT;
   extern __shared__ __align__(16) uint8_t smem[];
-  // SECOND works while the prefix is still being worked on, and waits before it stores (launch.cuh says on what grounds): what it reads until then goes past L1
+  // SECOND works while the prefix is still being worked on, and waits before it stores results (launch.cuh says on what grounds): what it reads until then goes past L1
   constexpr bool PAST = ROLE == SECOND;
   if (!PAST) follow_grid();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;

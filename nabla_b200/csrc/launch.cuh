@@ -26,7 +26,9 @@
 //    are on the chip then. A second kernel of this kind directly behind it would not have that ground to stand on.
 //  - attend_few_kernel as SECOND, the own keys of sequences behind a shared prefix, works before it has waited for the kernel of the prefix, which is
 //    always the launch ahead of it, writes nothing but parts, and begins it only behind its own wait. What SECOND reads until its wait goes past L1, so
-//    no line is older than that; all its blocks wait before they read a part, store a result or end, and only then let the next launch begin.
+//    no line is older than that; all its blocks wait before they read a part, store a result or end, and only then let the next launch begin. All that SECOND
+//    writes before it waits is a table of its own lines (FLAT, block 0), to scratch that the kernel of the prefix neither reads nor writes, and whose users before are
+//    over: that kernel had waited for them when it let SECOND begin.
 #pragma once
 #include <cuda_runtime.h>
 

@@ -14,11 +14,12 @@
 // that the rest works on. Else a pass makes the sums exact and checks the border; the tokens of its steps, some tens, are ranked in a list, and another
 // pass makes the draw. Where too many are left (equal logits, flat rows) steps are cut into 2048 finer ones of the order, down to single tokens.
 //
-// What bounds it is instructions, not memory: some 35 for each weight (12 of them in 64 bits) and 10 for each of the other passes, and rounds of exchange between
-// the threads of a row, of which a call with all filters has about 15 (a row of 1000 takes 8 us). 256 rows of 32001 in bf16 with filters of their own 56 us, as long as its
-// slowest rows, those with top-p alone; with top-k alone 33; 32 rows of 131072 with top-p 60; 512 rows of 8192 without filters 19 (floors of memory 2.5, 2.5, 2.6,
-// 1.3). Slower were a list of all that a bin of the threads' largest logits lets through in place of the histogram (61 us for the first), and three steps around the
-// border of top-p in place of one (65).
+// What bounds it is neither memory nor the number of instructions but rows that wait. 256 rows of 32001 in bf16 with filters of their own take 54 to 75 us with the
+// seed (85 seen), of which issue is 16: 17.9 million of a warp, four to a clock (1.9 were reached). The time is that of the slowest rows, those with top-p alone,
+// each with the block or cluster that its index gave it, when rows with top-k alone (33 us for a call of them) are long done and their SMs idle; and a row waits at
+// barriers, at some 15 rounds of exchange between its threads (a row of 1000 takes 8 us) and for loads, with 24 warps to an SM. 32 rows of 131072 with top-p 59 to 76;
+// 512 rows of 8192 without filters 19, in 1.15 waves of blocks (floors of memory 2.5, 2.6, 1.3). Slower were, in turn on one box and seed, a list of all that a bin of the
+// threads' largest logits lets through in place of the histogram (61 us for the first, against 56) and three steps around the border of top-p in place of one (65).
 //
 // A row is read two to four times, all but the first from the caches, by one block of threads or by a cluster of up to eight, which exchange sums,
 // histograms and lists over distributed shared memory. Warps own stretches of ids.

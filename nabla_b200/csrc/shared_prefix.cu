@@ -11,7 +11,9 @@
 //
 // 64 sequences of 50 to 1000 behind 8001 tokens, 16 heads over 4 of 128: 27 us (each over its whole text 71); 16 of up to 2000 behind 60001, 16 over 2: 43;
 // 4 behind 1000: 9 on the device. What bounds it: the start and end of blocks (7 us of those of 128-row tiles) and the chain of product, exponentials and product
-// of few tiles of keys for each block; for the last, starts. Prompts of 32 x 200 behind 2048: 193 us, exponentials (cached_attention_tcgen05.cu).
+// of few tiles of keys for each block; for the last, starts. Prompts of 32 x 200 behind 2048: 193 us, exponentials (cached_attention_tcgen05.cu). Far from
+// their floors are many sequences with some tokens each behind a short prefix, whose blocks pay their start and end for one or two steps of keys (81 x 10 behind 50, 24
+// heads over 8, 74 us; 27 x 301 behind 50, 119), and fp32 of more than 32 rows, which widens the codes again for every 16 rows (32 x 200 behind 2048 1187 us).
 #include "cached_attention_few.cuh"
 
 namespace nbc {
@@ -20,7 +22,9 @@ namespace nbc {
 struct FirstCut {
   int rows, q_tiles, splits;
 };
-// `c`: how the own keys are cut, in lines of at most `room` keys.
+// `c`: how the own keys are cut, in lines of at most `room` keys. That is the rule of cached_attention, whose borders were measured for a kernel that has the chip to itself;
+// here it shares the chip with the prefix. The times below are those of bf16 and heads of 128, of one step of keys and of a block's start and end; heads of 64 and
+// fp32 go by them too, which was not measured for itself (results do not depend on the cut but by the order of sums).
 static FirstCut cut_first(int rows, int kv_heads, long long prefix_room, int fp32, const Cut& c, int batch, int own_rows, long long room) {
   // Tiles of 128 rows start late and are soon quicker. us, tiles of 16 and of 128, behind 500, 2001 and 8001 tokens: 2 heads with 40 rows 10.8 and 15.6, 11.3 and
   // 16.0, 20.0 and 17.1, with 128 rows 9.2 and 14.8, 15.3 and 15.0, 20.0 and 16.6; 4 heads with 96 rows 9.5 and 14.6, 17.3 and 15.0, 22.6 and 19.3; 16 heads with
